@@ -11,6 +11,10 @@ the work in hand-written gfx950 HIP kernels (``libhcp_mi355x.so``, C ABI in
 * ``HcpRingAttentionBackend`` / ``HcpRingAttentionImpl`` registered as the
   vLLM ``CUSTOM`` attention backend by ``register()`` (__init__.py:34-54)
 * batched varlen / paged prefill and split-KV decode (``varlen``)
+* around the attention of a serving step: ``build_step_tables`` (block table,
+  slots and positions from the requests' lengths), ``qk_norm_rope`` (head norms,
+  rotation and cache write) and a KV cache in 4 bits (``kv_cache``, ``decode_fp4``,
+  ``HcpRingAttentionImpl(kv_cache_dtype="fp4")``)
 
 Importing the package does not import vLLM; ``register()`` does.
 """
@@ -18,7 +22,10 @@ Importing the package does not import vLLM; ``register()`` does.
 from __future__ import annotations
 
 from .merge import merge_attn_states, merge_pair
+from .qk_rope import qk_norm_rope
 from .ring_attn import ring_attn_merged, ring_attn_with_lse
+from .step_tables import build_step_tables
+from .varlen import decode_fp4
 
 __all__ = [
     "register",
@@ -26,6 +33,9 @@ __all__ = [
     "ring_attn_merged",
     "merge_attn_states",
     "merge_pair",
+    "build_step_tables",
+    "qk_norm_rope",
+    "decode_fp4",
     "BACKEND_PATH",
 ]
 

@@ -76,9 +76,16 @@ EXPORTED_SYMBOLS = (
     "hcp_merge_attn_states",
     "hcp_reshape_and_cache",
     "hcp_gather_paged_kv",
+    "hcp_fp4_write",
+    "hcp_fp4_read",
+    "hcp_fp4_gather",
+    "hcp_decode_fp4_workspace",
+    "hcp_decode_fp4",
+    "hcp_qk_norm_rope",
+    "hcp_step_tables",
 )
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 class KvSegment(ctypes.Structure):
@@ -238,8 +245,97 @@ class DecodePagedArgs(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("keep_nan", ctypes.c_int32),
         ("scale", ctypes.c_float),
+        ("seq_starts", ctypes.c_uint64),
     ]
 
+
+class Fp4CacheDesc(ctypes.Structure):
+    """``hcp_fp4_cache`` (include/hcp_mi355x.h)."""
+
+    _fields_ = [
+        ("addr", ctypes.c_uint64),
+        ("stride_block", ctypes.c_int64),
+        ("stride_head", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+class QkRopeArgs(ctypes.Structure):
+    """``hcp_qk_rope_args`` (include/hcp_mi355x.h)."""
+
+    _fields_ = [
+        ("q", ctypes.c_uint64),
+        ("q_stride_tok", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k", ctypes.c_uint64),
+        ("k_stride_tok", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v", ctypes.c_uint64),
+        ("v_stride_tok", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("q_out", ctypes.c_uint64),
+        ("qo_stride_tok", ctypes.c_int64),
+        ("qo_stride_head", ctypes.c_int64),
+        ("k_out", ctypes.c_uint64),
+        ("ko_stride_tok", ctypes.c_int64),
+        ("ko_stride_head", ctypes.c_int64),
+        ("q_weight", ctypes.c_uint64),
+        ("k_weight", ctypes.c_uint64),
+        ("positions", ctypes.c_uint64),
+        ("cos_sin", ctypes.c_uint64),
+        ("table_stride", ctypes.c_int64),
+        ("max_positions", ctypes.c_int64),
+        ("slot_mapping", ctypes.c_uint64),
+        ("num_slots", ctypes.c_int64),
+        ("cache", ctypes.c_uint64),
+        ("fp4", ctypes.c_uint64),
+        ("num_tokens", ctypes.c_int64),
+        ("eps", ctypes.c_double),
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rot", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("table_dtype", ctypes.c_int32),
+        ("pos_dtype", ctypes.c_int32),
+        ("slot_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("cache_kind", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class StepTablesArgs(ctypes.Structure):
+    """``hcp_step_tables_args`` (include/hcp_mi355x.h)."""
+
+    _fields_ = [
+        ("ctx_lens", ctypes.c_uint64),
+        ("new_lens", ctypes.c_uint64),
+        ("ctx_stride", ctypes.c_int64),
+        ("new_stride", ctypes.c_int64),
+        ("block_table", ctypes.c_uint64),
+        ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("free_blocks", ctypes.c_uint64),
+        ("num_free", ctypes.c_int64),
+        ("num_tokens", ctypes.c_int64),
+        ("query_start_loc", ctypes.c_uint64),
+        ("seq_lens", ctypes.c_uint64),
+        ("blocks_used", ctypes.c_uint64),
+        ("positions", ctypes.c_uint64),
+        ("slot_mapping", ctypes.c_uint64),
+        ("ctx_dtype", ctypes.c_int32),
+        ("new_dtype", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+    ]
+
+
+# include/hcp_mi355x.h HCP_STEP_MAX_SEQS
+STEP_MAX_SEQS = 4096
 
 # include/hcp_mi355x.h HCP_DECODE_PAGED_MAX_SEQS
 DECODE_PAGED_MAX_SEQS = 1024
@@ -344,6 +440,22 @@ def _declare(lib: ctypes.CDLL) -> None:
     ]
     lib.hcp_gather_paged_kv.restype = ctypes.c_int
     lib.hcp_gather_paged_kv.argtypes = [_P, _I32, _P, _I64, _I32, _I32, _I32, _P, _P, _P]
+    lib.hcp_fp4_write.restype = ctypes.c_int
+    lib.hcp_fp4_write.argtypes = [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I32, _I64, _I32, _P, _I32, _P,
+    ]
+    lib.hcp_fp4_read.restype = ctypes.c_int
+    lib.hcp_fp4_read.argtypes = [_P, _I32, _I64, _I32, _P, _I32, _P, _P, _P]
+    lib.hcp_fp4_gather.restype = ctypes.c_int
+    lib.hcp_fp4_gather.argtypes = [_P, _I32, _P, _I64, _I32, _P, _I32, _P, _P, _P, _P]
+    lib.hcp_decode_fp4_workspace.restype = ctypes.c_size_t
+    lib.hcp_decode_fp4_workspace.argtypes = [_I32, _I32, _I32, _I32]
+    lib.hcp_decode_fp4.restype = ctypes.c_int
+    lib.hcp_decode_fp4.argtypes = [_P, _P]
+    lib.hcp_qk_norm_rope.restype = ctypes.c_int
+    lib.hcp_qk_norm_rope.argtypes = [_P, _P]
+    lib.hcp_step_tables.restype = ctypes.c_int
+    lib.hcp_step_tables.argtypes = [_P, _P]
     lib.hcp_merge_attn_states.restype = ctypes.c_int
     lib.hcp_merge_attn_states.argtypes = [
         _P, _I64, _I64, _I32, _P, _I64,

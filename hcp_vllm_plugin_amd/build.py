@@ -29,6 +29,10 @@ OBJECTS = [
     ("abi.hip", []),
     ("merge.hip", []),
     ("cache.hip", []),
+    ("decode_fp4.hip", []),
+    ("fp4_cache.hip", []),
+    ("qk_rope.hip", []),
+    ("step_tables.hip", []),
 ]
 
 HIPCC_FLAGS = [

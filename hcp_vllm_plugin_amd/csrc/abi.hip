@@ -1168,25 +1168,54 @@ int hcp_decode_launch(const hcp_decode_args* a, void* stream) {
                      a->num_heads, a->num_kv_heads, a->head_dim, a->scale, a->dtype, stream, x);
 }
 
-// Workgroups per KV head and head chunk of hcp_decode_paged: one round of the
-// machine (a workgroup's chunk buffers take 128 KB of a CU's LDS).
-static int32_t paged_wgs(int32_t num_heads, int32_t num_kv_heads) {
+// Workgroups per KV head and head chunk of an unplanned decode launch: one round
+// of the machine, per_cu workgroups to a CU.
+static int32_t paged_wgs(int32_t num_heads, int32_t num_kv_heads, int32_t per_cu) {
   const int32_t chunks = (num_heads / num_kv_heads + 15) / 16;
-  return std::max(1, kNumCus / (num_kv_heads * chunks));
+  return std::max(1, per_cu * kNumCus / (num_kv_heads * chunks));
+}
+constexpr int32_t kPagedPerCu = 1;  // a workgroup's chunk buffers take 128 KB of a CU's LDS
+constexpr int32_t kFp4PerCu = 2;    // chunks in registers: two waves to a SIMD
+
+static size_t unplanned_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                  int32_t head_dim, int32_t per_cu) {
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads ||
+      head_dim <= 0)
+    return 0;
+  const size_t parts = hcp_decode_workspace_bytes(
+      num_seqs + paged_wgs(num_heads, num_kv_heads, per_cu), num_heads, head_dim);
+  return ((parts + 15) & ~static_cast<size_t>(15)) + 2 * sizeof(int32_t) * num_seqs;
 }
 
 size_t hcp_decode_paged_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                   int32_t head_dim) {
-  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads ||
-      head_dim <= 0)
-    return 0;
-  const size_t parts =
-      hcp_decode_workspace_bytes(num_seqs + paged_wgs(num_heads, num_kv_heads), num_heads, head_dim);
-  return ((parts + 15) & ~static_cast<size_t>(15)) + 2 * sizeof(int32_t) * num_seqs;
+  return unplanned_workspace(num_seqs, num_heads, num_kv_heads, head_dim, kPagedPerCu);
 }
 
-int hcp_decode_paged(const hcp_decode_paged_args* a, void* stream) {
-  const char* who = "hcp_decode_paged";
+size_t hcp_decode_fp4_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                int32_t head_dim) {
+  return unplanned_workspace(num_seqs, num_heads, num_kv_heads, head_dim, kFp4PerCu);
+}
+
+// A region of the 4-bit cache: what the kernels' 32-bit offsets and 16-byte
+// loads take.
+static int check_fp4(uint64_t addr, int64_t stride_block, int64_t stride_head, int64_t num_blocks,
+                     int32_t block_size, int32_t head_dim, const char* who) {
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 32)
+    return fail(HCP_EUNSUPPORTED, "%s: head_dim %d not supported by the 4-bit cache (a multiple "
+                "of 32 up to 256)", who, head_dim);
+  if (block_size < 16 || block_size > 65536 || (block_size & (block_size - 1)))
+    return fail(HCP_EUNSUPPORTED, "%s: block_size %d not supported by the 4-bit cache (a power of "
+                "two from 16 to 65536)", who, block_size);
+  if (num_blocks < 0 || num_blocks > INT32_MAX)
+    return fail(HCP_EINVAL, "%s: bad num_blocks", who);
+  if (!addr || (addr & 15) || stride_block % 16 || stride_head % 16)
+    return fail(HCP_EINVAL, "%s: the cache must be 16-byte aligned, strides too", who);
+  return HCP_OK;
+}
+
+static int decode_unplanned(const hcp_decode_paged_args* a, bool fp4, const char* who,
+                            void* stream) {
   if (!a) return fail(HCP_EINVAL, "%s: null arguments", who);
   int rc = check_heads(a->num_heads, a->num_kv_heads, a->head_dim, a->dtype, who);
   if (rc) return rc;
@@ -1206,13 +1235,23 @@ int hcp_decode_paged(const hcp_decode_paged_args* a, void* stream) {
   hcp_kv_segment kv = a->kv;
   kv.start = 0;
   kv.len = 1;
-  if ((rc = check_segment(kv, a->head_dim, who, 0))) return rc;
+  if (fp4) {
+    rc = check_fp4(kv.k_addr, kv.stride_block, kv.stride_head, kv.num_blocks, kv.block_size,
+                   a->head_dim, who);
+    if (!rc && kv.num_blocks == 0) rc = fail(HCP_EINVAL, "%s: a cache without blocks", who);
+  } else {
+    rc = check_segment(kv, a->head_dim, who, 0);
+    if (!rc && a->seq_starts)
+      rc = fail(HCP_EUNSUPPORTED, "%s: seq_starts need a 4-bit cache", who);
+  }
+  if (rc) return rc;
   // the kernel sums chunks of 32 keys in 32 bits
   if (a->block_table_width > ((int64_t{1} << 34) / kv.block_size) / a->num_seqs ||
       a->block_table_width * kv.block_size > INT32_MAX)
     return fail(HCP_EUNSUPPORTED, "%s: block table names too many keys", who);
+  const int32_t per_cu = fp4 ? kFp4PerCu : kPagedPerCu;
   const size_t need =
-      hcp_decode_paged_workspace(a->num_seqs, a->num_heads, a->num_kv_heads, a->head_dim);
+      unplanned_workspace(a->num_seqs, a->num_heads, a->num_kv_heads, a->head_dim, per_cu);
   if (!a->workspace || a->workspace_bytes < need)
     return fail(HCP_EWORKSPACE, "%s: workspace %zu bytes < %zu needed", who,
                 static_cast<size_t>(a->workspace_bytes), need);
@@ -1222,7 +1261,7 @@ int hcp_decode_paged(const hcp_decode_paged_args* a, void* stream) {
   dp.q = a->q;
   dp.q_stride_tok = a->q_stride_tok;
   dp.q_stride_head = a->q_stride_head;
-  dp.num_wgs = paged_wgs(a->num_heads, a->num_kv_heads);
+  dp.num_wgs = paged_wgs(a->num_heads, a->num_kv_heads, per_cu);
   const size_t slots = static_cast<size_t>(a->num_seqs + dp.num_wgs) * a->num_heads;
   const size_t o_al = (slots * hcp::padded_head_dim(a->head_dim) * sizeof(float) + 255) &
                       ~static_cast<size_t>(255);
@@ -1243,6 +1282,7 @@ int hcp_decode_paged(const hcp_decode_paged_args* a, void* stream) {
   p.bt_stride = a->block_table_stride;
   p.max_len = a->block_table_width * kv.block_size;
   p.window = a->window;
+  p.starts = a->seq_starts;
   p.seq_slots = reinterpret_cast<int32_t*>(ws + need - 2 * sizeof(int32_t) * a->num_seqs);
   hcp::RedParams rp{};
   rp.ws_o = dp.ws_o;
@@ -1257,9 +1297,18 @@ int hcp_decode_paged(const hcp_decode_paged_args* a, void* stream) {
   rp.lse_stride_head = a->lse_stride_head;
   rp.num_heads = a->num_heads;
   rp.head_dim = a->head_dim;
-  return launch_status(hcp::launch_decode_paged(p, rp, a->head_dim, a->dtype,
-                                                static_cast<hipStream_t>(stream)),
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return launch_status(fp4 ? hcp::launch_decode_fp4(p, rp, a->dtype, st)
+                           : hcp::launch_decode_paged(p, rp, a->head_dim, a->dtype, st),
                        who);
+}
+
+int hcp_decode_paged(const hcp_decode_paged_args* a, void* stream) {
+  return decode_unplanned(a, false, "hcp_decode_paged", stream);
+}
+
+int hcp_decode_fp4(const hcp_decode_paged_args* a, void* stream) {
+  return decode_unplanned(a, true, "hcp_decode_fp4", stream);
 }
 
 int hcp_merge_attn_states(void* out, int64_t o_stride_tok, int64_t o_stride_head,
@@ -1447,6 +1496,283 @@ int hcp_gather_paged_kv(const hcp_varlen_entry* entries, int32_t num_entries,
   p.v_out = v_out;
   (void)dtype;  // a 16-bit copy: the bytes are moved as they are
   return launch_status(hcp::launch_gather(p, static_cast<hipStream_t>(stream)), who);
+}
+
+// log2 of a power of two, else -1
+static int32_t shift_of(int32_t x) {
+  return (x & (x - 1)) ? -1 : 31 - __builtin_clz(static_cast<unsigned>(x));
+}
+
+static bool index_dtype(int32_t d) { return d == HCP_DTYPE_I32 || d == HCP_DTYPE_I64; }
+
+// What hcp_fp4_write and hcp_fp4_read share.
+static int fp4_params(hcp::Fp4Params& p, const void* slots, int32_t slot_dtype, int64_t num_tokens,
+                      int32_t num_kv_heads, const hcp_fp4_cache* cache, int32_t dtype,
+                      const char* who) {
+  if (num_tokens < 0 || num_kv_heads <= 0) return fail(HCP_EINVAL, "%s: bad sizes", who);
+  if (!dtype16(dtype)) return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, dtype);
+  if (!index_dtype(slot_dtype))
+    return fail(HCP_EUNSUPPORTED, "%s: slot dtype %d (int32 or int64)", who, slot_dtype);
+  if (!cache) return fail(HCP_EINVAL, "%s: null cache descriptor", who);
+  const hcp_fp4_cache& c = *cache;
+  const int rc = check_fp4(c.addr, c.stride_block, c.stride_head, c.num_blocks, c.block_size,
+                           c.head_dim, who);
+  if (rc) return rc;
+  if (num_tokens > 0 && !slots) return fail(HCP_EINVAL, "%s: null pointer", who);
+  // one thread per eight columns, 256 to a workgroup: the grid stays within 32 bits
+  if (num_tokens > (int64_t{1} << 31) / (num_kv_heads * (c.head_dim / 8)) * 128)
+    return fail(HCP_EINVAL, "%s: too many rows", who);
+  p.slots = slots;
+  p.slots_wide = slot_dtype == HCP_DTYPE_I64;
+  p.num_tokens = num_tokens;
+  p.num_kv_heads = num_kv_heads;
+  p.opr_shift = shift_of(c.head_dim / 8);
+  p.cache = reinterpret_cast<char*>(c.addr);
+  p.stride_block = c.stride_block;
+  p.stride_head = c.stride_head;
+  p.num_slots = c.num_blocks * c.block_size;
+  p.bs_shift = shift_of(c.block_size);
+  p.r = hcp::Fp4Region{c.head_dim, c.block_size};
+  return HCP_OK;
+}
+
+int hcp_fp4_write(const void* key, int64_t k_stride_tok, int64_t k_stride_head, const void* value,
+                  int64_t v_stride_tok, int64_t v_stride_head, const void* slot_mapping,
+                  int32_t slot_dtype, int64_t num_tokens, int32_t num_kv_heads,
+                  const hcp_fp4_cache* cache, int32_t dtype, void* stream) {
+  const char* who = "hcp_fp4_write";
+  hcp::Fp4Params p{};
+  const int rc = fp4_params(p, slot_mapping, slot_dtype, num_tokens, num_kv_heads, cache, dtype, who);
+  if (rc) return rc;
+  if (num_tokens == 0 || p.num_slots == 0) return HCP_OK;
+  if (!key || !value) return fail(HCP_EINVAL, "%s: null pointer", who);
+  if (!aligned16(key) || !aligned16(value))
+    return fail(HCP_EINVAL, "%s: key/value must be 16-byte aligned", who);
+  if ((k_stride_tok | k_stride_head | v_stride_tok | v_stride_head) % 8)
+    return fail(HCP_EINVAL, "%s: strides must be multiples of 8 elements", who);
+  p.key = key;
+  p.k_stride_tok = k_stride_tok;
+  p.k_stride_head = k_stride_head;
+  p.value = value;
+  p.v_stride_tok = v_stride_tok;
+  p.v_stride_head = v_stride_head;
+  return launch_status(hcp::launch_fp4_write(p, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int hcp_fp4_read(const void* slot_mapping, int32_t slot_dtype, int64_t num_tokens,
+                 int32_t num_kv_heads, const hcp_fp4_cache* cache, int32_t dtype, void* k_out,
+                 void* v_out, void* stream) {
+  const char* who = "hcp_fp4_read";
+  hcp::Fp4Params p{};
+  const int rc = fp4_params(p, slot_mapping, slot_dtype, num_tokens, num_kv_heads, cache, dtype, who);
+  if (rc) return rc;
+  if (num_tokens == 0) return HCP_OK;
+  if (!k_out || !v_out) return fail(HCP_EINVAL, "%s: null pointer", who);
+  if (!aligned16(k_out) || !aligned16(v_out))
+    return fail(HCP_EINVAL, "%s: k_out/v_out must be 16-byte aligned", who);
+  p.k_out = k_out;
+  p.v_out = v_out;
+  return launch_status(hcp::launch_fp4_read(p, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries, const int64_t* out_start,
+                   int64_t max_len, int32_t num_kv_heads, const hcp_fp4_cache* cache,
+                   int32_t dtype, void* k_out, void* v_out, hcp_varlen_entry* entries_out,
+                   void* stream) {
+  const char* who = "hcp_fp4_gather";
+  if (num_entries < 0 || max_len < 0 || num_kv_heads <= 0)
+    return fail(HCP_EINVAL, "%s: bad sizes", who);
+  if (!dtype16(dtype)) return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, dtype);
+  if (!cache) return fail(HCP_EINVAL, "%s: null cache descriptor", who);
+  const hcp_fp4_cache& c = *cache;
+  const int rc = check_fp4(c.addr, c.stride_block, c.stride_head, c.num_blocks, c.block_size,
+                           c.head_dim, who);
+  if (rc) return rc;
+  if (num_entries > 65535) return fail(HCP_EINVAL, "%s: more than 65535 entries", who);
+  if (num_entries == 0 || (max_len == 0 && !entries_out)) return HCP_OK;
+  if (c.num_blocks == 0) return fail(HCP_EINVAL, "%s: a cache without blocks", who);
+  if (!entries || !out_start || !k_out || !v_out) return fail(HCP_EINVAL, "%s: null pointer", who);
+  if (!aligned8(entries) || !aligned8(out_start) || !aligned16(k_out) || !aligned16(v_out) ||
+      !aligned8(entries_out))
+    return fail(HCP_EINVAL, "%s: misaligned pointer", who);
+  if (max_len > (int64_t{1} << 31) / (num_kv_heads * (c.head_dim / 8)) * 128)
+    return fail(HCP_EINVAL, "%s: too many rows", who);
+  hcp::Fp4GatherParams p{};
+  p.entries = entries;
+  p.out_start = out_start;
+  p.max_len = max_len;
+  p.num_entries = num_entries;
+  p.num_kv_heads = num_kv_heads;
+  p.opr_shift = shift_of(c.head_dim / 8);
+  p.cache = reinterpret_cast<const char*>(c.addr);
+  p.stride_block = c.stride_block;
+  p.stride_head = c.stride_head;
+  p.num_blocks = static_cast<uint32_t>(c.num_blocks);
+  p.bs_shift = shift_of(c.block_size);
+  p.r = hcp::Fp4Region{c.head_dim, c.block_size};
+  p.k_out = k_out;
+  p.v_out = v_out;
+  p.entries_out = entries_out;
+  return launch_status(hcp::launch_fp4_gather(p, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int hcp_qk_norm_rope(const hcp_qk_rope_args* a, void* stream) {
+  const char* who = "hcp_qk_norm_rope";
+  if (!a) return fail(HCP_EINVAL, "%s: null arguments", who);
+  if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads > 65536 || a->num_kv_heads > 65536)
+    return fail(HCP_EINVAL, "%s: bad num_heads / num_kv_heads", who);
+  if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8)
+    return fail(HCP_EUNSUPPORTED, "%s: head_dim %d not supported (a multiple of 8 up to 256)", who,
+                a->head_dim);
+  if (a->rot < 0 || a->rot > a->head_dim || a->rot % 16)
+    return fail(HCP_EUNSUPPORTED, "%s: %d rotated columns not supported (a multiple of 16 up to "
+                "head_dim)", who, a->rot);
+  if (!dtype16(a->dtype)) return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
+  for (int32_t d : {a->weight_dtype, a->table_dtype})
+    if (d != HCP_DTYPE_F32 && d != a->dtype)
+      return fail(HCP_EUNSUPPORTED, "%s: weights and table must be float32 or of q's dtype", who);
+  if (!index_dtype(a->pos_dtype) || !index_dtype(a->slot_dtype))
+    return fail(HCP_EUNSUPPORTED, "%s: index dtype (int32 or int64)", who);
+  if (a->cache_kind < 0 || a->cache_kind > 2)
+    return fail(HCP_EINVAL, "%s: cache_kind %d", who, a->cache_kind);
+  if (a->num_tokens < 0 || a->num_tokens > INT32_MAX || a->num_slots < 0 ||
+      a->num_slots > a->num_tokens)
+    return fail(HCP_EINVAL, "%s: bad num_tokens / num_slots", who);
+  if (!(a->eps >= 0) || !std::isfinite(a->eps))
+    return fail(HCP_EINVAL, "%s: eps must be finite and >= 0", who);
+  if (a->num_tokens == 0) return HCP_OK;
+  if (!a->q || !a->k || !a->q_out || (a->rot && (!a->positions || !a->cos_sin)))
+    return fail(HCP_EINVAL, "%s: null pointer", who);
+  if (a->rot && a->max_positions <= 0) return fail(HCP_EINVAL, "%s: an empty table", who);
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->q_out) || !aligned16(a->k_out) ||
+      !aligned16(a->v) || !aligned16(a->q_weight) || !aligned16(a->k_weight) ||
+      !aligned16(a->cos_sin))
+    return fail(HCP_EINVAL, "%s: pointers must be 16-byte aligned", who);
+  if ((a->q_stride_tok | a->q_stride_head | a->k_stride_tok | a->k_stride_head |
+       a->qo_stride_tok | a->qo_stride_head | a->ko_stride_tok | a->ko_stride_head |
+       a->table_stride) % 8)
+    return fail(HCP_EINVAL, "%s: strides must be multiples of 8 elements", who);
+  hcp::RopeParams p{};
+  if (a->cache_kind) {
+    if (!a->v || (a->num_slots && !a->slot_mapping))
+      return fail(HCP_EINVAL, "%s: a cache write needs v and slot_mapping", who);
+    if ((a->v_stride_tok | a->v_stride_head) % 8)
+      return fail(HCP_EINVAL, "%s: strides must be multiples of 8 elements", who);
+    p.v = a->v;
+    p.v_stride_tok = a->v_stride_tok;
+    p.v_stride_head = a->v_stride_head;
+    p.slots = a->slot_mapping;
+    p.num_cached = a->num_slots;
+  } else if (!a->k_out) {
+    return fail(HCP_EINVAL, "%s: neither k_out nor a cache", who);
+  }
+  int32_t bs = 1;
+  if (a->cache_kind == hcp::kRopeCache16) {
+    if (!a->cache) return fail(HCP_EINVAL, "%s: null cache descriptor", who);
+    const hcp_paged_cache& c = *a->cache;
+    bs = c.block_size;
+    if (bs <= 0 || (bs & (bs - 1)))
+      return fail(HCP_EINVAL, "%s: block_size %d not a power of two", who, bs);
+    if (c.num_blocks < 0) return fail(HCP_EINVAL, "%s: negative num_blocks", who);
+    if (c.num_blocks && (!c.k_addr || !c.v_addr || (c.k_addr & 15) || (c.v_addr & 15) ||
+                         (c.stride_block | c.stride_head | c.stride_tok) % 8))
+      return fail(HCP_EINVAL, "%s: the cache must be 16-byte aligned, strides too", who);
+    p.k_cache = reinterpret_cast<void*>(c.k_addr);
+    p.v_cache = reinterpret_cast<void*>(c.v_addr);
+    p.stride_block = c.stride_block;
+    p.stride_head = c.stride_head;
+    p.stride_tok = c.stride_tok;
+    p.num_slots = c.num_blocks * bs;
+  } else if (a->cache_kind == hcp::kRopeCacheFp4) {
+    if (!a->fp4) return fail(HCP_EINVAL, "%s: null cache descriptor", who);
+    const hcp_fp4_cache& c = *a->fp4;
+    const int rc = check_fp4(c.addr, c.stride_block, c.stride_head, c.num_blocks, c.block_size,
+                             c.head_dim, who);
+    if (rc) return rc;
+    if (c.head_dim != a->head_dim)
+      return fail(HCP_EINVAL, "%s: the cache's head_dim %d is not %d", who, c.head_dim, a->head_dim);
+    bs = c.block_size;
+    p.k_cache = reinterpret_cast<void*>(c.addr);
+    p.stride_block = c.stride_block;
+    p.stride_head = c.stride_head;
+    p.num_slots = c.num_blocks * bs;
+  }
+  p.q = a->q;
+  p.q_stride_tok = a->q_stride_tok;
+  p.q_stride_head = a->q_stride_head;
+  p.k = a->k;
+  p.k_stride_tok = a->k_stride_tok;
+  p.k_stride_head = a->k_stride_head;
+  p.q_out = a->q_out;
+  p.qo_stride_tok = a->qo_stride_tok;
+  p.qo_stride_head = a->qo_stride_head;
+  p.k_out = a->k_out;
+  p.ko_stride_tok = a->ko_stride_tok;
+  p.ko_stride_head = a->ko_stride_head;
+  p.q_weight = a->q_weight;
+  p.k_weight = a->k_weight;
+  p.pos = a->positions;
+  p.table = a->cos_sin;
+  p.table_stride = a->table_stride;
+  p.max_pos = a->max_positions;
+  p.num_tokens = a->num_tokens;
+  p.eps = a->eps;
+  p.num_heads = a->num_heads;
+  p.num_kv_heads = a->num_kv_heads;
+  p.d = a->head_dim;
+  p.rot = a->rot;
+  p.bs_shift = shift_of(bs);
+  p.bs_mask = bs - 1;
+  p.w_wide = a->weight_dtype == HCP_DTYPE_F32;
+  p.pos_wide = a->pos_dtype == HCP_DTYPE_I64;
+  p.table_wide = a->table_dtype == HCP_DTYPE_F32;
+  p.slots_wide = a->slot_dtype == HCP_DTYPE_I64;
+  p.interleaved = a->interleaved != 0;
+  return launch_status(hcp::launch_qk_rope(p, a->dtype, a->cache_kind,
+                                           static_cast<hipStream_t>(stream)), who);
+}
+
+int hcp_step_tables(const hcp_step_tables_args* a, void* stream) {
+  const char* who = "hcp_step_tables";
+  if (!a) return fail(HCP_EINVAL, "%s: null arguments", who);
+  if (a->num_seqs < 0 || a->num_tokens < 0 || a->num_free < 0 || a->table_width < 0)
+    return fail(HCP_EINVAL, "%s: bad sizes", who);
+  if (a->num_seqs > HCP_STEP_MAX_SEQS)
+    return fail(HCP_EUNSUPPORTED, "%s: more than %d requests", who, HCP_STEP_MAX_SEQS);
+  if (a->block_size <= 0 || (a->block_size & (a->block_size - 1)))
+    return fail(HCP_EINVAL, "%s: block_size %d not a power of two", who, a->block_size);
+  if (!index_dtype(a->ctx_dtype) || !index_dtype(a->new_dtype))
+    return fail(HCP_EUNSUPPORTED, "%s: lengths must be int32 or int64", who);
+  // (the kernel sums table entries in 32 bits)
+  if (a->table_width >= (int64_t{1} << 32) / HCP_STEP_MAX_SEQS || a->num_tokens > INT32_MAX)
+    return fail(HCP_EUNSUPPORTED, "%s: too many tokens or table entries", who);
+  if (!a->query_start_loc || !a->blocks_used ||
+      (a->num_seqs > 0 && (!a->ctx_lens || !a->new_lens || !a->seq_lens)) ||
+      (a->num_seqs > 0 && a->table_width > 0 && !a->block_table) ||
+      (a->num_free > 0 && !a->free_blocks) ||
+      (a->num_tokens > 0 && (!a->positions || !a->slot_mapping)))
+    return fail(HCP_EINVAL, "%s: null pointer", who);
+  hcp::StepTablesParams p{};
+  p.ctx = a->ctx_lens;
+  p.fresh = a->new_lens;
+  p.ctx_stride = a->ctx_stride;
+  p.fresh_stride = a->new_stride;
+  p.ctx_wide = a->ctx_dtype == HCP_DTYPE_I64;
+  p.fresh_wide = a->new_dtype == HCP_DTYPE_I64;
+  p.num_seqs = a->num_seqs;
+  p.bs_shift = shift_of(a->block_size);
+  p.table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.width = a->table_width;
+  p.free = a->free_blocks;
+  p.num_free = a->num_free;
+  p.num_tokens = a->num_tokens;
+  p.starts = a->query_start_loc;
+  p.seq_lens = a->seq_lens;
+  p.used = a->blocks_used;
+  p.positions = a->positions;
+  p.slots = a->slot_mapping;
+  return launch_status(hcp::launch_step_tables(p, static_cast<hipStream_t>(stream)), who);
 }
 
 }  // extern "C"

@@ -28,6 +28,7 @@
 //    partials of the sequence -- every split of its local and peer segments --
 //    with the LSE merge of ring_decode.py:46-61, writing out in the model
 //    dtype and optionally the merged LSE.
+#include "decode_share.h"
 #include "params.h"
 
 namespace hcp {
@@ -508,25 +509,6 @@ decode_split_kernel(DecParams p) {
   }
 }
 
-// Inclusive prefix sum over the wave's lanes, by DPP moves (inside rows of 16
-// lanes, then row 0 -> 1 and 2 -> 3, then the lower half into the upper):
-// an add each, where six shuffles through LDS take about 100 cycles each.
-__device__ __forceinline__ int wave_prefix(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
-  return x;
-}
-
-// Length r as the caller gives it.
-__device__ __forceinline__ int64_t paged_len(const PagedDecParams& p, int r) {
-  return p.lens_wide ? global_ptr(reinterpret_cast<const int64_t*>(p.lens))[r]
-                     : global_ptr(reinterpret_cast<const int32_t*>(p.lens))[r];
-}
-
 // A pure decode batch without a plan: lengths and block tables come straight
 // from the step's metadata on the device, so the host neither waits for them
 // nor plans nor uploads.  The keys of all sequences are laid end to end in
@@ -546,7 +528,6 @@ decode_paged_kernel(PagedDecParams p_) {
   constexpr int CHB = DecShared<D>::CHB;
   constexpr int W = DecShared<D>::W;
   constexpr int NT = 64 * W;
-  constexpr int EPT = kDecMaxSeqs / NT;  // sequences per thread of the prefix sum
   constexpr int kStart = 8;              // a split's start and end, in chunks
   __shared__ __attribute__((aligned(1024))) char bufE[W][2 * CHB];
   __shared__ __attribute__((aligned(1024))) char bufO[W][2 * CHB];
@@ -563,73 +544,8 @@ decode_paged_kernel(PagedDecParams p_) {
   const int chunk = static_cast<int>(item % p_.d.head_chunks);
   const int wg = static_cast<int>(item / p_.d.head_chunks);
   const int n = p_.num_seqs;
-  {
-    // ---- prefix sums over the sequences: chunks, sequences with keys ----
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int c[EPT], cs = 0, zs = 0;
-#pragma unroll
-    for (int j = 0; j < EPT; ++j) {
-      const int r = tid * EPT + j;
-      const int64_t given = r < n ? paged_len(p_, r) : 0;
-      const int all =  // keys that the sequence's query sees; max_len < 2^31
-          static_cast<int>(given < 0 ? 0 : given < p_.max_len ? given : p_.max_len);
-      const int len = p_.window > 0 && all > p_.window ? p_.window : all;
-      if (r < n) {
-        sm_all[r] = given == HCP_LEN_NOT_RUN ? -1 : all;
-        sm_len[r] = len;
-      }
-      c[j] = (len >> 5) + ((len & 31) != 0);
-      cs += c[j];
-      zs += c[j] > 0;
-    }
-    const int ci = wave_prefix(cs), zi = wave_prefix(zs);
-    if (lane == 63) {
-      sm_w[0][wave] = ci;
-      sm_w[1][wave] = zi;
-    }
-    if (tid == 0) sm_cut[0] = -1;
-    __syncthreads();
-    int cb = ci - cs, zb = zi - zs;
-    unsigned total = 0, some = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w < wave) {
-        cb += sm_w[0][w];
-        zb += sm_w[1][w];
-      }
-      total += sm_w[0][w];
-      some += sm_w[1][w];
-    }
-    // ---- this workgroup's share: at least two chunks (64 keys) ----
-    const unsigned most = static_cast<unsigned>(p_.d.num_wgs), half = (total + 1) / 2;
-    const unsigned wgs = most < half ? most : half;
-    if (static_cast<unsigned>(wg) < wgs) {
-      const unsigned share = total / wgs;
-      const unsigned start = share < kStart ? share : kStart;
-      const unsigned span = total + start * some, q = span / wgs, rem = span - q * wgs;
-      // cuts at span * w / wgs; the thread whose sequence holds one says which
-      // of its chunks come before it (in steps of 4, one for each wave, where
-      // the shares are long)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const unsigned w = wg + i, x = q * w + rem * w / wgs;
-        unsigned base = cb + start * zb;
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-          const unsigned next = base + (c[j] > 0 ? c[j] + start : 0u);
-          if (x >= base && (x < next || (w == wgs && x == next && c[j] > 0))) {
-            unsigned in = x - base > start ? x - base - start : 0u;
-            if (share >= 16) in = (in + 2) & ~3u;
-            if (w == wgs || in > static_cast<unsigned>(c[j])) in = c[j];
-            sm_cut[2 * i] = tid * EPT + j;
-            sm_cut[2 * i + 1] = in;
-          }
-          base = next;
-        }
-      }
-    }
-    __syncthreads();
-  }
+  paged_shares<NT, kStart, 2, false>(p_, wg, sm_len, sm_all, sm_w, sm_cut,
+                              [](int, int len) { return (len >> 5) + ((len & 31) != 0); });
   const int r0 = __builtin_amdgcn_readfirstlane(sm_cut[0]);
   const int o0 = __builtin_amdgcn_readfirstlane(sm_cut[1]);
   const int r1 = r0 < 0 ? -2 : __builtin_amdgcn_readfirstlane(sm_cut[2]);  // -1, -2: no share
@@ -821,6 +737,34 @@ hipError_t launch_decode(const DecParams& dp, const RedParams& rp, int head_dim,
                                  : launch_dec_t<64, _Float16>(dp, rp, st);
 }
 
+// The merge of a launch whose num_wgs workgroups (per KV head and chunk) cut the
+// batch among themselves.
+template <int D, typename T>
+static hipError_t launch_reduce_t(RedParams rp, int num_wgs, hipStream_t st) {
+  const int per_seq = (num_wgs + rp.num_seqs) / rp.num_seqs;
+  rp.groups = per_seq >= 48 ? 4 : per_seq >= 24 ? 2 : 1;
+  hipLaunchKernelGGL((decode_reduce_kernel<D, T>),
+                     dim3(static_cast<unsigned>(rp.num_seqs * rp.num_heads)), dim3(D * rp.groups),
+                     0, st, rp);
+  return hipGetLastError();
+}
+
+hipError_t launch_decode_reduce(const RedParams& rp, int num_wgs, int head_dim, int dtype,
+                                hipStream_t st) {
+  const bool bf = dtype == HCP_DTYPE_BF16;
+  switch (padded_head_dim(head_dim)) {
+    case 256:
+      return bf ? launch_reduce_t<256, __bf16>(rp, num_wgs, st)
+                : launch_reduce_t<256, _Float16>(rp, num_wgs, st);
+    case 128:
+      return bf ? launch_reduce_t<128, __bf16>(rp, num_wgs, st)
+                : launch_reduce_t<128, _Float16>(rp, num_wgs, st);
+    default:
+      return bf ? launch_reduce_t<64, __bf16>(rp, num_wgs, st)
+                : launch_reduce_t<64, _Float16>(rp, num_wgs, st);
+  }
+}
+
 template <int D, typename T>
 static hipError_t launch_dec_paged_t(const PagedDecParams& p, const RedParams& rp,
                                      hipStream_t st) {
@@ -833,13 +777,7 @@ static hipError_t launch_dec_paged_t(const PagedDecParams& p, const RedParams& r
     hipLaunchKernelGGL((decode_paged_kernel<D, T, false>), g, b, 0, st, p);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  RedParams r = rp;
-  const int per_seq = (p.d.num_wgs + rp.num_seqs) / rp.num_seqs;
-  r.groups = per_seq >= 48 ? 4 : per_seq >= 24 ? 2 : 1;
-  hipLaunchKernelGGL((decode_reduce_kernel<D, T>),
-                     dim3(static_cast<unsigned>(rp.num_seqs * rp.num_heads)), dim3(D * r.groups),
-                     0, st, r);
-  return hipGetLastError();
+  return launch_reduce_t<D, T>(rp, p.d.num_wgs, st);
 }
 
 hipError_t launch_decode_paged(const PagedDecParams& p, const RedParams& rp, int head_dim,

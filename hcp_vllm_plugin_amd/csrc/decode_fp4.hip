@@ -1,0 +1,380 @@
+// Split-KV decode over the 4-bit cache: one query token per sequence, lengths
+// and block tables read on the device (no plan), as decode_paged_kernel.
+//
+// For query head h of KV head h / G: out = sum_j softmax_j(q . k_j * scale) v_j over
+// k_j[d] = code * 2^(b - 127), one scale byte b for 32 columns.  A key of a head is
+// d + d / 16 bytes where 16-bit values take 4 d, so the same HBM rate would ask for
+// 3.8 times the keys per second, and what a key costs in instructions counts:
+//  * the cache lies as the matrix operands do (fp4.h): a lane loads 32 columns of
+//    one key of K, or 8 columns of four keys of V, in 16 bytes straight into
+//    registers, a wave 1 KB in a row; one v_cvt_scalef32_pk makes two 16-bit
+//    operand values of a byte, exactly, its scale applied;
+//  * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32 as in decode_split_body:
+//    16 query heads are the columns, the contraction order of either product is
+//    free, so K's is the order of a lane's bytes and P stays in the registers S
+//    came in; V's keys are paired by one v_perm for two values;
+//  * the running maximum is raised, and O rescaled, only when a score is past it
+//    by 2^8 (fp32 sums and two 16-bit terms of P have room for that).
+// The 4 waves of a workgroup take the 32-key chunks of its share in turn (chunks
+// lie on multiples of 32 positions, so that 16 keys never cross a block), the next
+// chunk's loads in flight, and are combined through LDS; decode_reduce_kernel
+// merges a sequence's partials.
+#include "decode_share.h"
+
+namespace hcp {
+
+// What a wave holds of a chunk (32 keys: two tiles of 16).
+template <int D>
+struct Fp4Chunk {
+  static constexpr int KW = D / 32;           // dwords of K per lane and tile
+  static constexpr int KS = D == 256 ? 2 : 1; // K scales per lane and tile
+  static constexpr int VP = D == 256 ? 2 : 1; // octets of V per lane and tile
+  uint32_t k[2][KW];
+  uint32_t ks[2][KS];
+  uint32_t v[2][VP][4];  // [key of the quad]
+  uint32_t vs[2];
+};
+
+template <typename T>
+__device__ __forceinline__ T ldnt(const char* p) {
+  return __builtin_nontemporal_load(
+      (const __attribute__((address_space(1))) T*)(reinterpret_cast<uintptr_t>(p)));
+}
+
+constexpr float kRaise = 8.f;  // how far (in powers of two) a score may pass the running maximum
+
+template <int D, typename T, bool KEEP_NAN>
+__device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_in, int chunk_in,
+                                               int slot_out, int r, int first, int all,
+                                               int kb, int ke, float (*sm_o)[16][D + 4],
+                                               float (*sm_m)[16], float (*sm_l)[16]) {
+  using E = Elem<T>;
+  using V8 = typename E::vec8;
+  using Chunk = Fp4Chunk<D>;
+  constexpr int QSTEPS = D / 32;
+  constexpr int NU = D / 16;
+  constexpr int W = 4;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, g4 = lane >> 4;
+  const int kvh = __builtin_amdgcn_readfirstlane(kvh_in);
+  const int chunk = __builtin_amdgcn_readfirstlane(chunk_in);
+  const int G = p.d.group - 16 * chunk < 16 ? p.d.group - 16 * chunk : 16;
+  const int h0 = kvh * p.d.group + 16 * chunk;
+  const int dv = p.d.head_dim;
+
+  // Q^T: column c16 = query head h0 + c16; the lane's columns of k-step s are
+  // (D / 4) g4 + 8 s .. + 7, the order of its K bytes
+  V8 qf[QSTEPS];
+  {
+    const bool hv = c16 < G;
+    const char* qrow = reinterpret_cast<const char*>(p.d.q) +
+                       (r * p.d.q_stride_tok +
+                        static_cast<int64_t>(h0 + (hv ? c16 : 0)) * p.d.q_stride_head) * 2;
+#pragma unroll
+    for (int s = 0; s < QSTEPS; ++s) {
+      const int d0 = D / 4 * g4 + 8 * s;
+      qf[s] = as_vec8<V8>(hv && d0 < dv ? ldg16(qrow + d0 * 2) : u32x4{0, 0, 0, 0});
+    }
+  }
+
+  // Lane offsets in a tile's bytes.  A piece past the row's dv columns is
+  // fetched from the row's first instead: it meets zeros of Q, or lands in
+  // columns of O that are not stored.
+  const Fp4Region reg{dv, p.kv.block_size};
+  int koff[Chunk::KS], ksoff[Chunk::KS], voff[Chunk::VP];
+#pragma unroll
+  for (int i = 0; i < Chunk::KS; ++i) {
+    const int d0 = D / 4 * g4 + 32 * i;
+    const bool in = d0 < dv;
+    koff[i] = c16 * (dv / 2) + (in ? d0 / 2 : 0);
+    ksoff[i] = ((c16 >> 2) * (dv / 32) + (in ? d0 / 32 : 0)) * 4 + (c16 & 3);
+  }
+#pragma unroll
+  for (int i = 0; i < Chunk::VP; ++i) {
+    const int oct = NU * c16 / 8 + i;
+    voff[i] = (g4 * (dv / 8) + (oct < dv / 8 ? oct : 0)) * 16;
+  }
+  const int vgrp = NU * c16 / 32;
+  const int vsoff = (g4 * (dv / 32) + (vgrp < dv / 32 ? vgrp : 0)) * 4;
+  const int bs = p.kv.block_size, bs_shift = 31 - __builtin_clz(bs);
+  const auto* bt = (const __attribute__((address_space(4))) int32_t*)(
+      p.kv.block_table + static_cast<uint64_t>(r) * p.bt_stride * 4);
+  const uint32_t id_max = static_cast<uint32_t>(p.kv.num_blocks) - 1;
+  const char* head = reinterpret_cast<const char*>(p.kv.k_addr) + kvh * p.kv.stride_head;
+
+  auto load = [&](int x0, Chunk& ch) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int x = x0 + 16 * t;
+      uint32_t id = bt[(x < all ? x : all - 1) >> bs_shift];
+      id = id < id_max ? id : id_max;  // past the cache: its last block
+      const int off = x & (bs - 1);
+      const char* kc = head + id * p.kv.stride_block + off * (dv / 2);
+      const char* sc = head + id * p.kv.stride_block + bs * dv + off * (dv / 32);
+      const char* vc = kc + bs * (dv / 2);
+#pragma unroll
+      for (int i = 0; i < Chunk::KS; ++i) {
+        if constexpr (D == 64) {
+          const u32x2 a = ldnt<u32x2>(kc + koff[0]);
+          ch.k[t][0] = a[0];
+          ch.k[t][1] = a[1];
+        } else {
+          const u32x4 a = ldnt<u32x4>(kc + koff[i]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) ch.k[t][4 * i + w] = a[w];
+        }
+        ch.ks[t][i] = ldnt<uint8_t>(sc + ksoff[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < Chunk::VP; ++i) {
+        const u32x4 a = ldnt<u32x4>(vc + voff[i]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ch.v[t][i][w] = a[w];
+      }
+      ch.vs[t] = ldnt<uint32_t>(sc + bs * (dv / 32) + vsoff);
+    }
+  };
+
+  const float c = p.d.scale_log2;
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x4 oacc[NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) oacc[u] = f32x4{};
+
+  auto compute = [&](int x0, Chunk& ch) __attribute__((always_inline)) {
+    f32x4 s[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int q = 0; q < QSTEPS; ++q)
+        s[t] = E::mfma16(as_vec8<V8>(fp4_values<T>(
+                             ch.k[t][q], __uint_as_float(ch.ks[t][Chunk::KS == 1 ? 0 : q / 4] << 23))),
+                         qf[q], s[t]);
+    if (x0 < first || x0 + 32 > ke) {
+      // keys outside the split: no weight, and a finite value whatever their
+      // bytes say (0 times a NaN would stay one)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = x0 + 16 * t + 4 * g4 + i;
+          if (key < first || key >= ke) {
+            s[t][i] = -INFINITY;
+            ch.vs[t] &= ~(0xffu << (8 * i));
+          }
+        }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c;
+    if (__builtin_amdgcn_ballot_w64(mx > m_run + kRaise) != 0) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) oacc[u] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    u32x4 pw, rw;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] = fast_exp2(__builtin_fmaf(s[t][i], c, -m_use));
+        l_run += s[t][i];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // P in two 16-bit terms, as in decode_split_body
+        uint32_t hi, lo;
+        two_terms<T>(s[t][2 * i], s[t][2 * i + 1], hi, lo);
+        pw[2 * t + i] = hi;
+        rw[2 * t + i] = lo;
+      }
+    }
+    const V8 pf = as_vec8<V8>(pw), rf = as_vec8<V8>(rw);
+    float vs[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      vs[j] = __uint_as_float(((ch.vs[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
+    // columns 2 u and 2 u + 1 of 8 keys -> two operands
+    auto pv = [&](auto sel, auto piece, int u) __attribute__((always_inline)) {
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t w = ch.v[j >> 2][decltype(piece)::value][j & 3];
+        if constexpr (D == 64) w >>= 16 * (c16 & 1);
+        x[j] = fp4_pair<T, decltype(sel)::value>(w, vs[j]);
+      }
+      u32x4 a, b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
+        b[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+      }
+      oacc[2 * u] = E::mfma16(as_vec8<V8>(a), pf, oacc[2 * u]);
+      oacc[2 * u] = E::mfma16(as_vec8<V8>(a), rf, oacc[2 * u]);
+      oacc[2 * u + 1] = E::mfma16(as_vec8<V8>(b), pf, oacc[2 * u + 1]);
+      oacc[2 * u + 1] = E::mfma16(as_vec8<V8>(b), rf, oacc[2 * u + 1]);
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+    pv(I0{}, I0{}, 0);
+    pv(I1{}, I0{}, 1);
+    if constexpr (D > 64) {
+      pv(I2{}, I0{}, 2);
+      pv(I3{}, I0{}, 3);
+    }
+    if constexpr (D > 128) {
+      pv(I0{}, I1{}, 4);
+      pv(I1{}, I1{}, 5);
+      pv(I2{}, I1{}, 6);
+      pv(I3{}, I1{}, 7);
+    }
+  };
+
+  // the wave's chunks: kb + 32 (wave, wave + W, ..)
+  int x = kb + 32 * wave;
+  if (x < ke) {
+    Chunk a, b;
+    load(x, a);
+    while (true) {
+      if (x + 32 * W >= ke) {
+        compute(x, a);
+        break;
+      }
+      load(x + 32 * W, b);
+      compute(x, a);
+      x += 32 * W;
+      if (x + 32 * W >= ke) {
+        compute(x, b);
+        break;
+      }
+      load(x + 32 * W, a);
+      compute(x, b);
+      x += 32 * W;
+    }
+  }
+
+  // ---- combine the W waves ----
+  float l_tot = l_run + __shfl_xor(l_run, 16);
+  l_tot += __shfl_xor(l_tot, 32);
+  if (g4 == 0) {
+    sm_m[wave][c16] = m_run;
+    sm_l[wave][c16] = l_tot;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int u = 0; u < NU; u += 4)
+      *reinterpret_cast<f32x4*>(&sm_o[wave][c16][NU * (4 * g4 + i) + u]) =
+          f32x4{oacc[u][i], oacc[u + 1][i], oacc[u + 2][i], oacc[u + 3][i]};
+  __syncthreads();
+  for (int idx = tid; idx < G * D; idx += 64 * W) {
+    const int h = idx / D, d = idx % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm_m[w][h]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float sc = fast_exp2(sm_m[w][h] - Mu);
+      L += sm_l[w][h] * sc;
+      O += sm_o[w][h][d] * sc;
+    }
+    const int64_t slot = static_cast<int64_t>(slot_out) * p.d.num_heads + h0 + h;
+    const bool some = KEEP_NAN ? L != 0.f : L > 0.f;
+    global_ptr(p.d.ws_o)[slot * D + d] = some ? O / L : 0.f;
+    if (d == 0) global_ptr(p.d.ws_lse)[slot] = some ? M * kLn2 + __logf(L) : -INFINITY;
+  }
+}
+
+// The batch is cut as for decode_paged_kernel; a chunk costs a quarter of the
+// bytes, so a split's start counts for more of them, and a share is at least one
+// chunk for each wave.
+template <int D, typename T, bool KEEP_NAN>
+__global__ __launch_bounds__(256, 2) void decode_fp4_kernel(PagedDecParams p) {
+  constexpr int W = 4;
+  __shared__ float sm_o[W][16][D + 4];
+  __shared__ float sm_m[W][16], sm_l[W][16];
+  __shared__ int sm_len[kDecMaxSeqs], sm_all[kDecMaxSeqs];  // keys seen, in the cache (-1: not run)
+  __shared__ int sm_w[2][W];
+  __shared__ int sm_cut[4];
+  int kvh;
+  int64_t item;
+  if (!xcd_remap(blockIdx.x, static_cast<int64_t>(p.d.num_wgs) * p.d.head_chunks,
+                 p.d.num_kv_heads, &kvh, &item))
+    return;
+  const int chunk = static_cast<int>(item % p.d.head_chunks);
+  const int wg = static_cast<int>(item / p.d.head_chunks);
+  auto first_chunk = [](int all, int len) { return (all - len) & ~31; };
+  paged_shares<64 * W, 16, 4, true>(p, wg, sm_len, sm_all, sm_w, sm_cut, [&](int all, int len) {
+    return len > 0 ? (all - first_chunk(all, len) + 31) >> 5 : 0;
+  });
+  const int r0 = __builtin_amdgcn_readfirstlane(sm_cut[0]);
+  const int o0 = __builtin_amdgcn_readfirstlane(sm_cut[1]);
+  const int r1 = r0 < 0 ? -2 : __builtin_amdgcn_readfirstlane(sm_cut[2]);  // -1, -2: no share
+  const int o1 = __builtin_amdgcn_readfirstlane(sm_cut[3]);
+  for (int r = r0; r <= r1; ++r) {
+    const int len = __builtin_amdgcn_readfirstlane(sm_len[r]);
+    if (len <= 0) continue;
+    const int all = __builtin_amdgcn_readfirstlane(sm_all[r]);
+    const int base = first_chunk(all, len), c = (all - base + 31) >> 5;
+    const int b = r == r0 ? o0 : 0, e = r == r1 ? o1 : c;
+    if (b >= e) continue;
+    if (kvh == 0 && chunk == 0 && threadIdx.x == 0) {
+      if (b == 0) global_ptr(p.seq_slots)[2 * r] = wg + r;
+      if (e == c) global_ptr(p.seq_slots)[2 * r + 1] = wg + r;
+    }
+    const int end = base + 32 * e;
+    fp4_split_body<D, T, KEEP_NAN>(p, kvh, chunk, wg + r, r, all - len, all, base + 32 * b,
+                                   end < all ? end : all, sm_o, sm_m, sm_l);
+    __syncthreads();  // this split has been combined out of the buffers
+  }
+  // the reduce goes by the slots alone: a sequence without keys says so
+  if (wg == 0 && kvh == 0 && chunk == 0) {
+    for (int r = threadIdx.x; r < p.num_seqs; r += 64 * W) {
+      if (sm_len[r] > 0) continue;
+      global_ptr(p.seq_slots)[2 * r] = 0;
+      global_ptr(p.seq_slots)[2 * r + 1] = sm_all[r] < 0 ? -2 : -1;
+    }
+  }
+}
+
+template <int D, typename T>
+static hipError_t launch_fp4_t(const PagedDecParams& p, const RedParams& rp, int dtype,
+                               hipStream_t st) {
+  const int64_t grid = xcd_grid_size(static_cast<int64_t>(p.d.num_wgs) * p.d.head_chunks,
+                                     p.d.num_kv_heads);
+  const dim3 g(static_cast<unsigned>(grid)), b(256);
+  if (p.d.keep_nan)
+    hipLaunchKernelGGL((decode_fp4_kernel<D, T, true>), g, b, 0, st, p);
+  else
+    hipLaunchKernelGGL((decode_fp4_kernel<D, T, false>), g, b, 0, st, p);
+  const hipError_t err = hipGetLastError();
+  return err != hipSuccess ? err : launch_decode_reduce(rp, p.d.num_wgs, p.d.head_dim, dtype, st);
+}
+
+hipError_t launch_decode_fp4(const PagedDecParams& p, const RedParams& rp, int dtype,
+                             hipStream_t st) {
+  const bool bf = dtype == HCP_DTYPE_BF16;
+  switch (padded_head_dim(p.d.head_dim)) {
+    case 256:
+      return bf ? launch_fp4_t<256, __bf16>(p, rp, dtype, st)
+                : launch_fp4_t<256, _Float16>(p, rp, dtype, st);
+    case 128:
+      return bf ? launch_fp4_t<128, __bf16>(p, rp, dtype, st)
+                : launch_fp4_t<128, _Float16>(p, rp, dtype, st);
+    default:
+      return bf ? launch_fp4_t<64, __bf16>(p, rp, dtype, st)
+                : launch_fp4_t<64, _Float16>(p, rp, dtype, st);
+  }
+}
+
+}  // namespace hcp

@@ -2,7 +2,7 @@
 // translation units and the extern "C" layer (abi.hip).
 #pragma once
 
-#include "common.h"
+#include "fp4.h"
 
 namespace hcp {
 
@@ -142,6 +142,7 @@ struct PagedDecParams {
   int64_t bt_stride;     // elements between block-table rows
   int64_t max_len;       // keys a block-table row can name
   int32_t window;        // 0: none
+  const void* starts;    // first key seen, as lens (NULL: 0); decode_fp4_kernel alone
   int32_t* seq_slots;    // [2 * num_seqs]: first and last slot of each sequence (0, -1: no keys;
                          // 0, -2: HCP_LEN_NOT_RUN)
 };
@@ -163,6 +164,9 @@ struct MergeParams {
   int32_t num_heads, head_dim;
   int32_t out_dtype, p_dtype, s_dtype;
 };
+
+// What a rope launch writes K and V into.
+enum { kRopeNoCache = 0, kRopeCache16 = 1, kRopeCacheFp4 = 2 };
 
 struct CacheParams {
   const void* key;
@@ -210,6 +214,93 @@ struct MetaParams {
   int64_t* dev;  // [2 n] or NULL: the lengths of a plain decode batch, the lengths
 };
 
+// Rows into the 4-bit cache, or its rows at `slots` as 16-bit values (fp4.h).
+struct Fp4Params {
+  const void* key;
+  int64_t k_stride_tok, k_stride_head;
+  const void* value;
+  int64_t v_stride_tok, v_stride_head;
+  void* k_out;  // reading: [num_tokens, Hkv, d]
+  void* v_out;
+  const void* slots;
+  bool slots_wide;  // int64, else int32
+  int64_t num_tokens;
+  int32_t num_kv_heads;
+  int32_t opr_shift;  // log2(d / 8) when it is a power of two, else -1
+  char* cache;
+  int64_t stride_block, stride_head;  // bytes
+  int64_t num_slots;
+  int32_t bs_shift;
+  Fp4Region r;
+};
+
+// Paged segments of the 4-bit cache into one contiguous [total, Hkv, d] K and V.
+struct Fp4GatherParams {
+  const hcp_varlen_entry* entries;
+  const int64_t* out_start;
+  int64_t max_len;
+  int32_t num_entries, num_kv_heads;
+  int32_t opr_shift;
+  const char* cache;
+  int64_t stride_block, stride_head;  // bytes
+  uint32_t num_blocks;
+  int32_t bs_shift;
+  Fp4Region r;
+  void* k_out;
+  void* v_out;
+  hcp_varlen_entry* entries_out;  // NULL: not wanted
+};
+
+// Norms, rotation and cache write of a step's q, k and v (qk_rope.hip).
+struct RopeParams {
+  const void* q;
+  int64_t q_stride_tok, q_stride_head;
+  const void* k;
+  int64_t k_stride_tok, k_stride_head;
+  const void* v;
+  int64_t v_stride_tok, v_stride_head;
+  void* q_out;
+  int64_t qo_stride_tok, qo_stride_head;
+  void* k_out;  // NULL: only into the cache
+  int64_t ko_stride_tok, ko_stride_head;
+  const void* q_weight;  // NULL: no norm
+  const void* k_weight;
+  const void* pos;
+  const void* table;  // [max_pos, rot]: cosines, sines
+  const void* slots;  // of the first num_cached tokens
+  void* k_cache;      // 4-bit: the cache
+  void* v_cache;
+  int64_t table_stride, max_pos;
+  int64_t stride_block, stride_head, stride_tok;  // elements; 4-bit: bytes
+  int64_t num_slots, num_cached, num_tokens;
+  double eps;
+  int32_t num_heads, num_kv_heads, d, rot;
+  int32_t bs_shift, bs_mask;
+  int32_t lpr_shift, wpt;  // set by the launch: lanes of a row, waves of a token
+  bool w_wide, pos_wide, table_wide, slots_wide;  // 32-bit floats, 64-bit indices
+  bool interleaved;
+};
+
+constexpr int kStepMaxSeqs = HCP_STEP_MAX_SEQS;
+
+// Tables of a step (step_tables.hip).
+struct StepTablesParams {
+  const void* ctx;
+  const void* fresh;  // new tokens
+  int64_t ctx_stride, fresh_stride;
+  bool ctx_wide, fresh_wide;  // int64, else int32
+  int32_t num_seqs, bs_shift;
+  int32_t* table;
+  int64_t table_stride, width;
+  const int32_t* free;
+  int64_t num_free, num_tokens;
+  int32_t* starts;
+  int32_t* seq_lens;
+  int32_t* used;
+  int64_t* positions;
+  int64_t* slots;
+};
+
 // Prefill in D columns (padded_head_dim): the attention kernel and, when p
 // carries a KV split, the merge of its partials into out / lse (and acc).
 template <int D>
@@ -233,6 +324,16 @@ hipError_t launch_decode(const DecParams& dp, const RedParams& rp, int head_dim,
                          int dtype, hipStream_t st);
 hipError_t launch_decode_paged(const PagedDecParams& p, const RedParams& rp, int head_dim,
                                int dtype, hipStream_t st);
+// The merge of a launch whose num_wgs workgroups (per KV head and head chunk) cut the batch.
+hipError_t launch_decode_reduce(const RedParams& rp, int num_wgs, int head_dim, int dtype,
+                                hipStream_t st);
+hipError_t launch_decode_fp4(const PagedDecParams& p, const RedParams& rp, int dtype,
+                             hipStream_t st);
+hipError_t launch_fp4_write(const Fp4Params& p, int dtype, hipStream_t st);
+hipError_t launch_fp4_read(const Fp4Params& p, int dtype, hipStream_t st);
+hipError_t launch_fp4_gather(const Fp4GatherParams& p, int dtype, hipStream_t st);
+hipError_t launch_qk_rope(RopeParams p, int dtype, int cache, hipStream_t st);
+hipError_t launch_step_tables(const StepTablesParams& p, hipStream_t st);
 hipError_t launch_merge(const MergeParams& p, hipStream_t st);
 hipError_t launch_cache_write(const CacheParams& p, bool slots_i64, hipStream_t st);
 hipError_t launch_fetch_metadata(const MetaParams& p, hipStream_t st);

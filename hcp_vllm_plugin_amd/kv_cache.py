@@ -10,6 +10,13 @@ paged local-segment reader consumes (file_connector.py:13-16).  Rows ``t <
 len(slot_mapping)`` of key/value are written (key may be padded past that, as
 in the reference's ``key[:n]``); a negative slot is a padding token and is
 skipped.
+
+The 4-bit cache (``fp4_cache_shape``) holds K and V as 4-bit codes (sign, two
+bits of exponent, one of mantissa) with a power-of-two scale for 32 columns of a
+head's row, 17 / 32 byte a value; the format is in include/hcp_mi355x.h
+(``hcp_fp4_cache``).  ``reshape_and_cache`` writes it, ``gather_kv`` reads back
+what it stands for, ``varlen.decode_fp4`` and the backend with
+``kv_cache_dtype="fp4"`` attend over it.
 """
 
 from __future__ import annotations
@@ -21,7 +28,7 @@ import torch
 from . import _lib
 from .varlen import PagedCache
 
-__all__ = ["reshape_and_cache"]
+__all__ = ["reshape_and_cache", "fp4_cache_shape", "gather_kv"]
 
 # Cache descriptors by (address, shape, strides, dtype): the write runs once per
 # layer and step, and building the descriptor each time was a third of its
@@ -50,10 +57,88 @@ def _cache_desc(kv_cache: torch.Tensor):
     return ent
 
 
+def fp4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int,
+                    head_dim: int) -> tuple[int, int, int, int]:
+    """Shape of the uint8 tensor that is a 4-bit cache of these sizes."""
+    if head_dim % 32 or not 0 < head_dim <= 256:
+        raise ValueError(f"4-bit cache: head_dim {head_dim} is not a multiple of 32 up to 256")
+    if block_size & (block_size - 1) or not 16 <= block_size <= 65536:
+        raise ValueError(f"4-bit cache: block_size {block_size} is not a power of two from 16 to 65536")
+    return (num_blocks, num_kv_heads, block_size, head_dim + head_dim // 16)
+
+
+def fp4_desc(pc: PagedCache) -> "_lib.Fp4CacheDesc":
+    return _lib.Fp4CacheDesc(pc.k_addr, pc.stride_block, pc.stride_head, pc.num_blocks,
+                             pc.block_size, pc.head_dim)
+
+
+def _check_slots(slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> None:
+    if slot_mapping.dtype not in (torch.int32, torch.int64) or slot_mapping.dim() != 1:
+        raise ValueError("slot_mapping must be int32 or int64, of one dimension")
+    if not kv_cache.is_cuda or slot_mapping.device != kv_cache.device:
+        raise ValueError("slot_mapping must be on the cache's GPU")
+
+
+def _write_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
+               slot_mapping: torch.Tensor) -> None:
+    pc = PagedCache.from_tensor(kv_cache)
+    n = slot_mapping.numel()
+    if key.shape != value.shape or key.dim() != 3:
+        raise ValueError("key/value must be [N, Hkv, D] of one shape")
+    if key.shape[0] < n:
+        raise ValueError(f"{n} slots for {key.shape[0]} key rows")
+    if key.shape[1] != pc.num_kv_heads or key.shape[2] != pc.head_dim:
+        raise ValueError("key/value heads or head_dim do not match the cache")
+    if key.dtype not in (torch.float16, torch.bfloat16) or value.dtype != key.dtype:
+        raise ValueError("key/value must both be float16 or bfloat16")
+    if key.stride(-1) != 1 or value.stride(-1) != 1:
+        raise ValueError("key/value head_dim must be contiguous")
+    _check_slots(slot_mapping, kv_cache)
+    if key.device != kv_cache.device or value.device != kv_cache.device:
+        raise ValueError("key/value must be on the cache's GPU")
+    if n == 0:
+        return
+    slots, desc = slot_mapping.contiguous(), fp4_desc(pc)
+    with _lib.on_device(key.device):
+        rc = _lib.lib().hcp_fp4_write(
+            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+            value.stride(1), slots.data_ptr(),
+            _lib.DTYPE_I64 if slots.dtype == torch.int64 else _lib.DTYPE_I32, n, pc.num_kv_heads,
+            ctypes.addressof(desc), _lib.dtype_code(key.dtype), _lib.stream_ptr(key.device))
+    _lib.check(rc, "hcp_fp4_write")
+
+
+def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
+              dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V ``[n, Hkv, D]`` that a 4-bit cache stands for at ``slot_mapping``,
+    in the 16-bit ``dtype`` they were written in (exactly: a code's value has two
+    significant bits).  A slot that is negative or past the cache reads as zeros."""
+    if kv_cache.dtype != torch.uint8:
+        raise ValueError("gather_kv reads a 4-bit cache (uint8)")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("dtype must be float16 or bfloat16")
+    pc = PagedCache.from_tensor(kv_cache)
+    _check_slots(slot_mapping, kv_cache)
+    slots, desc = slot_mapping.contiguous(), fp4_desc(pc)
+    kv = torch.empty((2, slots.shape[0], pc.num_kv_heads, pc.head_dim), dtype=dtype,
+                     device=kv_cache.device)
+    k, v = kv[0], kv[1]
+    with _lib.on_device(kv_cache.device):
+        rc = _lib.lib().hcp_fp4_read(
+            slots.data_ptr(), _lib.DTYPE_I64 if slots.dtype == torch.int64 else _lib.DTYPE_I32,
+            slots.shape[0], pc.num_kv_heads, ctypes.addressof(desc), _lib.dtype_code(dtype),
+            k.data_ptr(), v.data_ptr(), _lib.stream_ptr(kv_cache.device))
+    _lib.check(rc, "hcp_fp4_read")
+    return k, v
+
+
 def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
                       slot_mapping: torch.Tensor) -> None:
     """Write ``key``/``value`` ``[N, Hkv, D]`` rows ``[0, n)``, ``n =
-    slot_mapping.numel()``, into ``kv_cache`` at ``slot_mapping``."""
+    slot_mapping.numel()``, into ``kv_cache`` at ``slot_mapping``; into a 4-bit
+    cache (uint8) as its codes."""
+    if kv_cache.dtype == torch.uint8:
+        return _write_fp4(key, value, kv_cache, slot_mapping)
     _, desc_addr, hkv, d = _cache_desc(kv_cache)
     n = slot_mapping.numel()
     if key.shape != value.shape or key.dim() != 3:

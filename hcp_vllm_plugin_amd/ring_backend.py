@@ -35,6 +35,11 @@ Drop-in for hcp_vllm_plugin/ring_backend.py's hot path:
   decode growth is sharded by ``ring_decode.growth_assignee``.  In a pure
   decode batch the owner partials run in the same split-KV launch as the
   other rows.
+* ``kv_cache_dtype="fp4"``: the paged cache holds 4-bit codes (``kv_cache``).
+  Decode rows read them as they lie; prefill chunks run on their keys expanded
+  to 16 bits, per layer, in scratch.  Staged peers stay 16-bit and merge with
+  either as ever; the decode ring and ``HCP_RING_SPLIT_TOKENS`` need a 16-bit
+  cache.
 * ``IMPL_STATS`` evidence counters (ring_backend.py:295-306).  ``attn_hip`` /
   ``merge_hip`` count kernel launches and merges (a merge done inside the
   local pass counts as one); the legacy keys ``attn_triton`` /
@@ -620,6 +625,11 @@ def _merge(
     return out
 
 
+# Most bytes of scratch that a prefill launch over a 4-bit cache expands keys into
+# (more for a single request with more keys than fit).
+_FP4_SCRATCH = 1 << 30
+
+
 # ---------------------------------------------------------------------------
 # Backend class (registered as CUSTOM)
 # ---------------------------------------------------------------------------
@@ -723,8 +733,12 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
             raise NotImplementedError("HCP ring backend: soft cap not supported")
         if sliding_window is not None and int(sliding_window) <= 0:
             raise ValueError("sliding_window must be a positive number of keys")
-        if kv_cache_dtype not in ("auto", "float16", "bfloat16"):
+        if kv_cache_dtype not in ("auto", "float16", "bfloat16", "fp4"):
             raise NotImplementedError(f"kv_cache_dtype {kv_cache_dtype} not supported")
+        if kv_cache_dtype == "fp4" and head_size % 32:
+            raise NotImplementedError(
+                f"HCP ring backend: head_size {head_size} not supported by the 4-bit cache "
+                "(a multiple of 32 up to 256)")
         # the paged cache is read in place in 16-byte pieces (vLLM's flash
         # backends take the same head sizes)
         if head_size % 8 or not 0 < head_size <= 256:
@@ -856,7 +870,9 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
     def _plan(self, layer_name, qsl, seq_lens, block_table, first_blocks, pc, split):
         plan = _Plan()
         n = len(seq_lens)
-        apart = qsl != list(range(n + 1)) and self._decode_rows_apart(qsl, seq_lens, True)
+        # (a 4-bit cache's keys are expanded for the launch of the others anyway)
+        apart = qsl != list(range(n + 1)) and pc.layout != "fp4" and \
+            self._decode_rows_apart(qsl, seq_lens, True)
         ring_on = _decode_ring_enabled() and bool(DECODE_RING_MAP)
         for r in range(len(seq_lens)):
             qs, qe = qsl[r], qsl[r + 1]
@@ -930,8 +946,10 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
             raise NotImplementedError("fused output quant not supported")
         if attn_metadata is None:  # profiling run
             if output.is_cuda and not _capturing():
-                # the partials of a cut launch, so that the engine's peak has them
-                _lib.scratch(_lib.split_limits(self.head_size).max_workspace, output.device)
+                # the partials of a cut launch and a 4-bit cache's expanded keys, so
+                # that the engine's peak has them
+                _lib.scratch(_lib.split_limits(self.head_size).max_workspace +
+                             (_FP4_SCRATCH if self.kv_cache_dtype == "fp4" else 0), output.device)
             return output.fill_(0)
         if self.attn_type != AttentionType.DECODER:
             raise NotImplementedError("HCP ring backend supports decoder attention only")
@@ -944,6 +962,8 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
         pc = PagedCache.from_tensor(kv_cache)
         if pc.num_kv_heads != self.num_kv_heads or pc.head_dim != self.head_size:
             raise ValueError("kv_cache shape does not match the layer's heads/head_size")
+        if (pc.layout == "fp4") != (self.kv_cache_dtype == "fp4"):
+            raise ValueError(f"a {kv_cache.dtype} cache for kv_cache_dtype {self.kv_cache_dtype!r}")
         ring_on = _ring_enabled()
         split = _split_tokens() if ring_on else 0
         # One token per request and nothing that gives a request peers: a
@@ -971,6 +991,14 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
                               ring_on, split)
 
         is_decode = n > 0 and qsl == list(range(n + 1))
+        if pc.layout == "fp4":
+            if split > 0:
+                raise NotImplementedError("HCP_RING_SPLIT_TOKENS needs a 16-bit cache")
+            if _decode_ring_enabled() and any(fb in DECODE_RING_MAP for fb in first_blocks):
+                raise NotImplementedError("the decode ring needs a 16-bit cache")
+            if is_decode:
+                self._forward_decode_fp4(query, out, step, pc, layer_name)
+                return output
         if is_decode and self._forward_decode_staged(query, out, step, pc, layer_name, ring_on,
                                                      split):
             return output
@@ -1221,7 +1249,9 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
             dec = fast[key] = self._plan_rows(query, qsl, seq_lens, block_table, pc, lens)
         _check_base(pc)
         if dec is not None:
-            if isinstance(dec, tuple):  # a run of rows, unplanned
+            if isinstance(dec, list):  # a 4-bit cache's
+                self._run_fp4_rows(dec, query, out, pc, keep_nan=qsl != list(range(n + 1)))
+            elif isinstance(dec, tuple):  # a run of rows, unplanned
                 a, b, rows = dec
                 rows.run(query[a:b], out[a:b], pc, self.scale, keep_nan=True)
             else:
@@ -1274,7 +1304,19 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
     def _chunk_launch(self, ent, query, block_table, pc):
         """The causal launch of entries with addresses relative to a layer's
         cache; over blocks under 16 tokens, which are gathered from absolute
-        addresses, the entries."""
+        addresses, the entries; over a 4-bit cache a list of launches, each with
+        keys that fit the scratch they are expanded into."""
+        if pc.layout == "fp4":
+            most = _FP4_SCRATCH // (4 * self.num_kv_heads * self.head_size)
+            launches, first, keys = [], 0, 0
+            for i, n in enumerate([*ent["len"].tolist(), most + 1]):
+                if keys + n > most and i > first:
+                    launches.append(VarlenLaunch(ent[first:i], True, True, query.device,
+                                                 keep=block_table, heads=self._heads,
+                                                 window=self.sliding_window, fp4=pc))
+                    first, keys = i, 0
+                keys += n
+            return launches
         if pc.block_size < _MIN_PAGED_BLOCK:
             return ent
         return VarlenLaunch(ent, True, True, query.device, keep=block_table, heads=self._heads,
@@ -1283,6 +1325,11 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
     def _run_chunks(self, pre, query, out, block_table, pc, acc=None):
         """A layer's run of what ``_chunk_launch`` made, merged with ``acc`` as
         its prefix."""
+        if isinstance(pre, list):
+            for launch in pre:
+                launch.run(query, out, None, self.num_kv_heads, self.scale, self.sliding_window,
+                           acc=acc, kv_base=pc.k_addr)
+            return
         if isinstance(pre, np.ndarray):
             ent = pre.copy()
             ent["k_addr"] = pc.k_addr
@@ -1316,6 +1363,8 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
                 PagedDecode.takes(block_table[a:b], lens[a:b], pc.block_size):
             return (int(qs[a]), int(qs[a]) + b - a,
                     PagedDecode(pc, block_table[a:b], lens[a:b], self.num_heads, w))
+        if pc.layout == "fp4":
+            return self._plan_fp4_rows(query, rows, qs[rows], tk[rows], block_table, pc)
         # one query at the end of its keys: all of them visible, or the last `w`
         # of them (ring_backend.py:397-398)
         start = np.zeros(len(rows), np.int64) if w is None else np.maximum(tk[rows] - w, 0)
@@ -1324,6 +1373,73 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
                               relative=True),
             self.num_heads, self.num_kv_heads, self.head_size, query.device, keep=block_table,
             rows=None if qsl == list(range(len(qsl))) else qs[rows])
+
+    # -- a 4-bit cache's single-token rows ---------------------------------------
+    def _plan_fp4_rows(self, query, rows, qs, keys, block_table, pc, starts=None):
+        """Launches of the batch's requests ``rows`` (query rows ``qs``, ``keys``
+        keys each, the first seen ``starts``): [(first, end of a run of query rows,
+        or their indices and None, launch)], each of as many as one takes."""
+        most = _lib.DECODE_PAGED_MAX_SEQS
+        words = [np.ascontiguousarray(x, dtype=np.int64) for x in (rows, qs, keys, starts)
+                 if x is not None]
+        dev, _ = _upload(words, query.device)
+        at, cols = 0, []
+        for x in words:
+            cols.append(dev[at:at + x.nbytes].view(torch.int64))
+            at += (x.nbytes + 255) & ~255
+        plans = []
+        for a in range(0, len(rows), most):
+            b = min(len(rows), a + most)
+            run = qs[b - 1] - qs[a] == b - 1 - a and rows[b - 1] - rows[a] == b - 1 - a
+            table = block_table[rows[a]:rows[a] + b - a] if run else block_table[cols[0][a:b]]
+            dec = PagedDecode(pc, table, cols[2][a:b], self.num_heads, self.sliding_window,
+                              None if starts is None else cols[3][a:b])
+            plans.append((int(qs[a]), int(qs[a]) + b - a, dec) if run else (cols[1][a:b], None, dec))
+        return plans
+
+    def _run_fp4_rows(self, plans, query, out, pc, keep_nan: bool, lse=None) -> None:
+        """``lse``: of query rows, all of them in one run."""
+        for a, b, dec in plans:
+            if b is None:
+                part = torch.empty((a.shape[0], *out.shape[1:]), dtype=out.dtype, device=out.device)
+                dec.run(query[a], part, pc, self.scale, keep_nan)
+                out[a] = part
+            else:
+                dec.run(query[a:b], out[a:b], pc, self.scale, keep_nan,
+                        None if lse is None else lse[:, a:b])
+
+    def _forward_decode_fp4(self, query, out, step, pc, layer_name) -> None:
+        """A pure decode batch with staged peers over a 4-bit cache: the local
+        keys past each prefix (or, inside it, all of them: ring_backend.py:811-830)
+        in the 4-bit decode, then the peers, which take that result as their
+        running accumulator."""
+        (_qsl, seq_lens, first_blocks), block_table = step.host, step.bt
+        _check_base(pc)
+        n = len(seq_lens)
+        staged = [self._peer_for_request(fb, layer_name, n) if _ring_enabled() else None
+                  for fb in first_blocks]
+        ends = [min(sum(int(kv[0].shape[0]) for kv in s), tk) if s else 0
+                for s, tk in zip(staged, seq_lens)]
+        starts = [0 if end >= tk else end for end, tk in zip(ends, seq_lens)]
+        key = (*self._layout_key("fp4_rows", pc), _lib.stream_ptr(query.device), tuple(starts))
+        plans = step.fast.get(key)
+        if plans is None:
+            if max(seq_lens) > block_table.shape[1] * pc.block_size:
+                raise ValueError("segment extends past the block-table row")
+            if min(seq_lens) < 0:
+                raise ValueError("negative segment start/length")
+            rows = np.arange(n)
+            plans = step.fast[key] = self._plan_fp4_rows(query, rows, rows, seq_lens, block_table,
+                                                         pc, starts)
+        lse = torch.empty((self.num_heads, n), dtype=torch.float32, device=query.device)
+        self._run_fp4_rows(plans, query, out, pc, False, lse)
+        _count("decode")
+        segs = [[segment_contiguous(k, v) for k, v in s if k.shape[0] > 0] if 0 < end < tk else []
+                for s, end, tk in zip(staged, ends, seq_lens)]
+        if any(segs):
+            DecodeBatch(segs, self.num_heads, self.num_kv_heads, self.head_size,
+                        query.device).run(query, out, None, self.scale, acc=(out, lse))
+            _count("decode")
 
     def _local_launch(self, query, plan: _Plan, step, pc):
         """The launch of a plan's local entries, shared by the layers that plan

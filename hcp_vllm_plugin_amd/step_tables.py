@@ -1,0 +1,84 @@
+"""A step's block table, slots and positions, built on the GPU.
+
+The reference's engine makes these on the host and uploads them each step.
+``build_step_tables`` makes them from the requests' lengths where those already
+are: it takes the new blocks of every request off a list of free ones, and gives
+the query starts, lengths, positions and slots that ``qk_rope.qk_norm_rope``,
+``kv_cache.reshape_and_cache`` and ``HcpRingAttentionImpl.forward`` read, in one
+launch and without waiting for the device.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+__all__ = ["StepTables", "build_step_tables"]
+
+_INDEX = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
+
+
+class StepTables(NamedTuple):
+    query_start_loc: torch.Tensor  # int32 [n + 1]
+    seq_lens: torch.Tensor         # int32 [n]
+    positions: torch.Tensor        # int64 [num_tokens]
+    slot_mapping: torch.Tensor     # int64 [num_tokens]
+    blocks_used: torch.Tensor      # int32 [1]
+
+
+def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                      free_blocks: torch.Tensor, block_size: int, num_tokens: int) -> StepTables:
+    """Tables of a step in which request r, with ``ctx_lens[r]`` tokens in the
+    cache, gets ``new_lens[r]`` more (int32 / int64 ``[n]``, at most 4096 requests).
+
+    ``block_table`` (int32, n rows or more) names the blocks that hold the cached
+    tokens; entries ``ceil(ctx / block_size)`` .. ``ceil((ctx + new) / block_size)
+    - 1`` of row r are written, with the next ids of ``free_blocks`` (int32), the
+    requests in order.  The step takes the first ``blocks_used`` of them; where
+    that is more than there are, the entries without a block become -1 and the
+    slots in them -1, which the cache writes skip, so a caller that may run out
+    looks at ``blocks_used`` before it uses the step.  Tokens past the keys that a
+    table row can name get slot -1 too, and take no block.
+
+    ``positions`` and ``slot_mapping`` have ``num_tokens`` rows: the new tokens,
+    then (padding) position 0 and slot -1.  Lengths below 0 count as 0."""
+    n = ctx_lens.shape[0] if ctx_lens.dim() == 1 else -1
+    dev = block_table.device
+    for name, x in (("ctx_lens", ctx_lens), ("new_lens", new_lens)):
+        if x.dtype not in _INDEX or tuple(x.shape) != (n,):
+            raise ValueError(f"{name} must be int32/int64 of one dimension, both of one length")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < n or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 with contiguous rows, one for each request")
+    if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
+        raise ValueError("free_blocks must be contiguous int32 of one dimension")
+    if not dev.type == "cuda" or any(x.device != dev for x in (ctx_lens, new_lens, free_blocks)):
+        raise ValueError("all tensors must be on one GPU")
+    if block_size <= 0 or block_size & (block_size - 1):
+        raise ValueError("block_size must be a power of two")
+    if num_tokens < 0:
+        raise ValueError("num_tokens must not be negative")
+    ints = torch.empty(2 * n + 2, dtype=torch.int32, device=dev)
+    wide = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
+    out = StepTables(ints[:n + 1], ints[n + 1:2 * n + 1], wide[0], wide[1], ints[2 * n + 1:])
+    a = _lib.StepTablesArgs()
+    a.ctx_lens, a.ctx_stride, a.ctx_dtype = ctx_lens.data_ptr(), ctx_lens.stride(0), \
+        _INDEX[ctx_lens.dtype]
+    a.new_lens, a.new_stride, a.new_dtype = new_lens.data_ptr(), new_lens.stride(0), \
+        _INDEX[new_lens.dtype]
+    a.block_table, a.table_stride, a.table_width = block_table.data_ptr(), \
+        block_table.stride(0), block_table.shape[1]
+    a.free_blocks, a.num_free = free_blocks.data_ptr(), free_blocks.shape[0]
+    base = ints.data_ptr()
+    a.query_start_loc, a.seq_lens, a.blocks_used = base, base + 4 * (n + 1), base + 4 * (2 * n + 1)
+    a.positions = wide.data_ptr()
+    a.slot_mapping = a.positions + 8 * num_tokens
+    a.num_tokens, a.num_seqs, a.block_size = num_tokens, n, block_size
+    with _lib.on_device(dev):
+        rc = _lib.lib().hcp_step_tables(ctypes.addressof(a), _lib.stream_ptr(dev))
+    _lib.check(rc, "hcp_step_tables")
+    return out

@@ -16,7 +16,10 @@ table) -- and runs one launch per segment kind:
 
 Paged layouts the reference reads: vLLM 0.31 ``[nb, Hkv, bs, 2*D]`` with
 K in ``[..., :D]`` and V in ``[..., D:]`` (file_connector.py:13-16,175-179),
-and vLLM 0.23 ``[nb, 2, bs, Hkv, D]`` (ring_backend.py:601,617-624).
+and vLLM 0.23 ``[nb, 2, bs, Hkv, D]`` (ring_backend.py:601,617-624).  A third
+one holds K and V in 4 bits: uint8 ``[nb, Hkv, bs, D + D / 16]`` (``kv_cache``).
+``PagedDecode`` reads it as it lies; ``VarlenLaunch`` expands the launch's
+segments into 16-bit scratch first.
 """
 
 from __future__ import annotations
@@ -41,6 +44,7 @@ __all__ = [
     "DecodeBatch",
     "PagedDecode",
     "decode_attn",
+    "decode_fp4",
     "head_major",
 ]
 
@@ -50,7 +54,9 @@ class PagedCache:
     """A paged KV cache and its element strides.
 
     ``layout`` is ``"v031"`` for ``[nb, Hkv, bs, 2*D]`` or ``"v023"`` for
-    ``[nb, 2, bs, Hkv, D]``; ``from_tensor`` infers it from the rank.
+    ``[nb, 2, bs, Hkv, D]``; ``from_tensor`` infers it from the rank.  uint8
+    ``[nb, Hkv, bs, D + D / 16]`` is ``"fp4"``, the 4-bit cache: a (block,
+    head)'s bytes lie together, ``v_addr`` is ``k_addr`` and ``stride_tok`` 0.
     """
 
     cache: torch.Tensor
@@ -73,6 +79,14 @@ class PagedCache:
         if cache.stride(-1) != 1:
             raise ValueError("paged cache: last dim must be contiguous")
         es = cache.element_size()
+        if cache.dtype == torch.uint8:
+            if cache.dim() != 4 or cache.shape[3] == 0 or cache.shape[3] % 34 or \
+                    cache.stride(2) != cache.shape[3]:
+                raise ValueError("4-bit cache: uint8 [blocks, Hkv, block_size, D + D / 16], the "
+                                 "bytes of a block and head contiguous")
+            nb, hkv, bs, row = cache.shape
+            return cls(cache, "fp4", hkv, row // 17 * 16, bs, cache.data_ptr(), cache.data_ptr(),
+                       0, cache.stride(1), cache.stride(0))
         if cache.dim() == 4:  # [nb, Hkv, bs, 2D]
             nb, hkv, bs, d2 = cache.shape
             d = d2 // 2
@@ -123,6 +137,21 @@ def _check_kv_layout(k_addr: int, v_addr: int, stride_tok: int, stride_head: int
         raise ValueError("k/v token stride must be in (0, 2^24) elements")
 
 
+def _check_cache(pc: PagedCache) -> None:
+    """The kernels can read the cache ``pc``."""
+    if pc.layout == "fp4":
+        if pc.k_addr % 16 or pc.stride_head % 16 or pc.stride_block % 16:
+            raise ValueError("the 4-bit cache must be 16-byte aligned, strides too")
+        if pc.head_dim > 256 or pc.block_size < 16 or pc.block_size > 65536:
+            raise ValueError("4-bit cache: head_dim a multiple of 32 up to 256, block_size from 16 "
+                             "to 65536")
+    else:
+        _check_kv_layout(pc.k_addr, pc.v_addr, pc.stride_tok, pc.stride_head, pc.stride_block,
+                         pc.cache.element_size())
+    if pc.block_size <= 0 or pc.block_size & (pc.block_size - 1):
+        raise ValueError("block_size must be a power of two")
+
+
 def segment_paged(pc: PagedCache, block_table_row: torch.Tensor, start: int,
                   length: int) -> KvSegment:
     """Segment over tokens ``[start, start+length)`` of one request's paged KV.
@@ -130,6 +159,8 @@ def segment_paged(pc: PagedCache, block_table_row: torch.Tensor, start: int,
     ``block_table_row`` is the request's int32 block-table row on the device
     (contiguous); token x lives in block ``row[x // bs]`` at ``x % bs``.
     """
+    if pc.layout == "fp4":
+        raise ValueError("a 4-bit cache has no segments: decode_fp4 and VarlenLaunch(fp4=...) read it")
     if block_table_row.dtype != torch.int32 or block_table_row.stride(-1) != 1:
         raise ValueError("block table row must be contiguous int32")
     _check_kv_layout(pc.k_addr, pc.v_addr, pc.stride_tok, pc.stride_head, pc.stride_block,
@@ -254,10 +285,7 @@ def paged_entry_array(pc: "PagedCache", block_table: torch.Tensor, rows, q_start
     ``kv_base``."""
     if block_table.dtype != torch.int32 or not block_table.is_contiguous():
         raise ValueError("block table must be contiguous int32")
-    _check_kv_layout(pc.k_addr, pc.v_addr, pc.stride_tok, pc.stride_head, pc.stride_block,
-                     pc.cache.element_size())
-    if pc.block_size <= 0 or pc.block_size & (pc.block_size - 1):
-        raise ValueError("block_size must be a power of two")
+    _check_cache(pc)
     rows = np.asarray(rows, dtype=np.int64)
     start = np.asarray(start, dtype=np.int64)
     length = np.asarray(length, dtype=np.int64)
@@ -348,14 +376,19 @@ class VarlenLaunch:
     """
 
     def __init__(self, entries, causal: bool, paged: bool, device: torch.device, keep=None,
-                 heads: tuple[int, int, int] | None = None, window: int | None = None):
+                 heads: tuple[int, int, int] | None = None, window: int | None = None,
+                 fp4: PagedCache | None = None):
         """``entries``: a list of VarlenEntry, or an ENTRY_DTYPE array (then
         ``keep`` holds the tensors its addresses point into).
 
         ``heads = (num_heads, num_kv_heads, head_dim)`` and ``window`` of the
         runs to come let the plan cut long key ranges over few query rows into
         pieces (``hcp_plan_varlen_split``); a run with other values, or a plan
-        built without them, takes the uncut launch."""
+        built without them, takes the uncut launch.
+
+        ``fp4``: the paged entries are of a 4-bit cache with this one's layout;
+        a run names its cache by ``kv_base`` and expands the entries' keys into
+        16-bit scratch (``2 * keys * Hkv * D`` values for as long as it runs)."""
         L = _lib.lib()
         self.causal = bool(causal)
         self.paged = bool(paged)
@@ -382,8 +415,27 @@ class VarlenLaunch:
         # cache with shorter blocks the segments are gathered into one
         # contiguous K/V buffer on the device first (hcp_gather_paged_kv, one
         # launch per run), and the attention runs over that copy.
-        self._gather = None
-        if self.paged and self.num_entries:
+        self._gather = self._fp4 = None
+        if fp4 is not None and self.num_entries:
+            if not self.paged or fp4.layout != "fp4":
+                raise ValueError("fp4 needs paged entries of a 4-bit cache")
+            host = np.frombuffer(arr, dtype=ENTRY_DTYPE, count=self.num_entries).copy()
+            lens = host["len"].astype(np.int64)
+            out_start = np.zeros(self.num_entries, dtype=np.int64)
+            out_start[1:] = np.cumsum(lens)[:-1]
+            self._fp4 = {"hkv": fp4.num_kv_heads, "dim": fp4.head_dim, "total": int(lens.sum()),
+                         "max_len": int(lens.max()), "block_size": fp4.block_size,
+                         "num_blocks": fp4.num_blocks, "stride_head": fp4.stride_head,
+                         "stride_block": fp4.stride_block}
+            arr = host.copy()
+            for f in ("block_table", "stride_block", "block_size", "num_blocks", "k_addr",
+                      "v_addr"):
+                arr[f] = 0
+            arr["start"] = out_start
+            arr["stride_tok"] = fp4.num_kv_heads * fp4.head_dim
+            arr["stride_head"] = fp4.head_dim
+            self.paged = False
+        elif self.paged and self.num_entries:
             host = np.frombuffer(arr, dtype=ENTRY_DTYPE, count=self.num_entries).copy()
             if int(host["block_size"].min()) < _MIN_PAGED_BLOCK:
                 lens = host["len"].astype(np.int64)
@@ -405,7 +457,12 @@ class VarlenLaunch:
         _lib.check(rc, "hcp_plan_varlen_tiles")
         self.num_tiles = rc
         split = self._plan_split(arr, heads, window)
-        if self._gather is None:
+        if self._fp4 is not None:
+            f = self._fp4
+            self._plan_dev, (f["paged_ptr"], f["start_ptr"], self.tiles_ptr, *sp) = _upload(
+                [host, out_start, tiles, *split], device)
+            self.entries_ptr = None
+        elif self._gather is None:
             self._plan_dev, (self.entries_ptr, self.tiles_ptr, *sp) = _upload(
                 [arr, tiles, *split], device)
         else:
@@ -470,6 +527,26 @@ class VarlenLaunch:
         _lib.check(rc, "hcp_gather_paged_kv")
         return ptr
 
+    def _expanded(self, q: torch.Tensor, cache_addr: int, stream: int):
+        """The entries' keys of the 4-bit cache at ``cache_addr`` as 16-bit values:
+        (scratch, device address of the entries over them), on the current
+        stream.  The scratch is the run's own."""
+        f = self._fp4
+        hkv, d = f["hkv"], f["dim"]
+        if q.shape[2] != d:
+            raise ValueError(f"q's head_dim {q.shape[2]} is not the cache's {d}")
+        side = (2 * f["total"] * hkv * d + 255) & ~255  # bytes of K (or V)
+        buf = torch.empty(2 * side + 96 * self.num_entries, dtype=torch.uint8, device=q.device)
+        base = buf.data_ptr()
+        desc = _lib.Fp4CacheDesc(cache_addr, f["stride_block"], f["stride_head"], f["num_blocks"],
+                                 f["block_size"], d)
+        rc = _lib.lib().hcp_fp4_gather(
+            f["paged_ptr"], self.num_entries, f["start_ptr"], f["max_len"], hkv,
+            ctypes.addressof(desc), _lib.dtype_code(q.dtype), base, base + side, base + 2 * side,
+            stream)
+        _lib.check(rc, "hcp_fp4_gather")
+        return buf, base + 2 * side
+
     def run(self, q: torch.Tensor, out: torch.Tensor, lse: torch.Tensor | None,
             num_kv_heads: int, scale: float, window: int | None = None,
             acc=None, acc_is_prefix: bool = True, kv_base: int = 0) -> None:
@@ -483,9 +560,12 @@ class VarlenLaunch:
         ``lse`` may then be None; otherwise it receives the merged LSE.
 
         ``kv_base``: added to the addresses of paged entries (planned with
-        addresses relative to a layer's cache)."""
+        addresses relative to a layer's cache); the cache of a launch over a
+        4-bit one."""
         if self.num_tiles == 0:
             return
+        if self._fp4 is not None and (not kv_base or num_kv_heads != self._fp4["hkv"]):
+            raise ValueError("a launch over a 4-bit cache needs its address and KV heads")
         if window is not None and window <= 0:
             raise ValueError("window must be a positive number of keys")
         if kv_base and self._gather is not None:
@@ -500,7 +580,8 @@ class VarlenLaunch:
         a.num_entries = self.num_entries
         a.num_heads, a.num_kv_heads, a.head_dim = num_heads, num_kv_heads, head_dim
         a.causal, a.window, a.paged = self.causal, win, self.paged
-        a.scale, a.dtype, a.kv_base = float(scale), _lib.dtype_code(q.dtype), kv_base
+        a.scale, a.dtype = float(scale), _lib.dtype_code(q.dtype)
+        a.kv_base = kv_base if self.paged else 0
         if acc is not None:
             a_o, a_lse = acc
             if a_o.dtype != q.dtype or a_o.stride(-1) != 1 or a_lse.dtype != torch.float32:
@@ -511,8 +592,13 @@ class VarlenLaunch:
             a.acc_is_prefix = bool(acc_is_prefix)
         sp = self._split
         with _lib.on_device(q.device):
-            a.entries = self.entries_ptr if self._gather is None else \
-                self._gathered(q, num_kv_heads)
+            keys = None  # expanded keys, held until the launch has been queued
+            if self._fp4 is not None:
+                keys, a.entries = self._expanded(q, kv_base, _lib.stream_ptr(q.device))
+            elif self._gather is not None:
+                a.entries = self._gathered(q, num_kv_heads)
+            else:
+                a.entries = self.entries_ptr
             # fp32 partials of a cut launch; without room for them it stays whole
             ws = None
             if sp is not None and sp["key"] == (num_heads, num_kv_heads, head_dim, win):
@@ -770,16 +856,14 @@ class PagedDecode:
     and block ids are read on the device when a run executes; a length past its
     table row counts as the row's keys, so a caller that refuses such a batch
     checks the lengths itself.  One object serves every layer whose cache has
-    ``pc``'s layout."""
+    ``pc``'s layout, the 4-bit one included (``hcp_decode_fp4``); over that,
+    ``starts`` (as ``seq_lens``) names the first key each query sees."""
 
     def __init__(self, pc: PagedCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                 num_heads: int, window: int | None):
+                 num_heads: int, window: int | None, starts: torch.Tensor | None = None):
         if block_table.dtype != torch.int32 or block_table.stride(-1) != 1:
             raise ValueError("block table must be int32 with contiguous rows")
-        _check_kv_layout(pc.k_addr, pc.v_addr, pc.stride_tok, pc.stride_head, pc.stride_block,
-                         pc.cache.element_size())
-        if pc.block_size <= 0 or pc.block_size & (pc.block_size - 1):
-            raise ValueError("block_size must be a power of two")
+        _check_cache(pc)
         n = seq_lens.shape[0]
         if block_table.dim() != 2 or block_table.shape[0] < n:
             raise ValueError("the block table has no row for a request")
@@ -793,9 +877,16 @@ class PagedDecode:
         a.lens_dtype = _lib.DTYPE_I64 if seq_lens.dtype == torch.int64 else _lib.DTYPE_I32
         a.num_seqs, a.window = n, int(window or 0)
         a.num_heads, a.num_kv_heads, a.head_dim = num_heads, pc.num_kv_heads, pc.head_dim
-        a.workspace_bytes = _lib.lib().hcp_decode_paged_workspace(n, num_heads, pc.num_kv_heads,
-                                                                  pc.head_dim)
-        self._keep = (block_table, seq_lens)
+        L = _lib.lib()
+        self._fp4 = pc.layout == "fp4"
+        size = L.hcp_decode_fp4_workspace if self._fp4 else L.hcp_decode_paged_workspace
+        a.workspace_bytes = size(n, num_heads, pc.num_kv_heads, pc.head_dim)
+        if starts is not None:
+            if starts.dtype != seq_lens.dtype or starts.shape != seq_lens.shape or \
+                    not starts.is_contiguous():
+                raise ValueError("starts must be as seq_lens")
+            a.seq_starts = starts.data_ptr()
+        self._keep = (block_table, seq_lens, starts)
 
     @staticmethod
     def takes(block_table: torch.Tensor, seq_lens: torch.Tensor, block_size: int) -> bool:
@@ -811,19 +902,73 @@ class PagedDecode:
                 and width * block_size < 1 << 31 and width <= ((1 << 34) // block_size) // n)
 
     def run(self, q: torch.Tensor, out: torch.Tensor, pc: PagedCache, scale: float,
-            keep_nan: bool = False) -> None:
-        """One layer: its q, out and cache.  ``keep_nan``: as ``DecodeBatch.run``."""
+            keep_nan: bool = False, lse: torch.Tensor | None = None) -> None:
+        """One layer: its q, out and cache (and ``lse`` float32 ``[H, S]``).
+        ``keep_nan``: as ``DecodeBatch.run``."""
         a = _lib.DecodePagedArgs.from_buffer_copy(self._args)
         a.q, a.q_stride_tok, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1)
         a.out, a.o_stride_tok, a.o_stride_head = out.data_ptr(), out.stride(0), out.stride(1)
         a.kv.k_addr, a.kv.v_addr = pc.k_addr, pc.v_addr
         a.scale, a.dtype, a.keep_nan = float(scale), _lib.dtype_code(q.dtype), keep_nan
+        if lse is not None:
+            a.lse, a.lse_stride_head = lse.data_ptr(), lse.stride(0)
+        L = _lib.lib()
+        launch = L.hcp_decode_fp4 if self._fp4 else L.hcp_decode_paged
         with _lib.on_device(q.device):
             # fp32 partials: stream-ordered scratch from torch's caching allocator
             ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=q.device)
             a.workspace = ws.data_ptr()
-            rc = _lib.lib().hcp_decode_paged(ctypes.addressof(a), _lib.stream_ptr(q.device))
-        _lib.check(rc, "hcp_decode_paged")
+            rc = launch(ctypes.addressof(a), _lib.stream_ptr(q.device))
+        _lib.check(rc, "hcp_decode_fp4" if self._fp4 else "hcp_decode_paged")
+
+
+def decode_fp4(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: float,
+    window: int | None = None,
+    out: torch.Tensor | None = None,
+    with_lse: bool = False,
+    keep_nan: bool = False,
+    starts: torch.Tensor | None = None,
+):
+    """Attention of single-token queries q ``[S, H, D]`` (fp16 / bf16, the type
+    the cache was written with) over a 4-bit cache: query r sees keys
+    ``[starts[r], seq_lens[r])`` (``starts`` None: from 0) of row r of
+    ``block_table``, the last ``window`` of them; lengths and block ids are
+    read on the device when the call executes.  A query that sees no key gets
+    out 0 and LSE -inf; a length past its table row counts as the row's keys.
+    ``keep_nan``: as ``DecodeBatch.run``.  Returns out (and lse float32 ``[H, S]``)."""
+    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or q.stride(-1) != 1:
+        raise ValueError("q must be float16/bfloat16 [S, H, D] with contiguous head_dim")
+    pc = PagedCache.from_tensor(kv_cache)
+    s, h, d = q.shape
+    if pc.layout != "fp4" or d != pc.head_dim or h % pc.num_kv_heads:
+        raise ValueError("kv_cache must be a 4-bit cache of q's head_dim, its heads dividing q's")
+    if window is not None and window <= 0:
+        raise ValueError("window must be a positive number of keys")
+    for name, t in (("seq_lens", seq_lens), ("starts", starts)):
+        if t is not None and (t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (s,)
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous int32/int64 [S]")
+    for t in (q, kv_cache, block_table, seq_lens, starts, out):
+        if t is not None and (not t.is_cuda or t.device != q.device):
+            raise ValueError("all tensors must be on q's GPU")
+    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+        raise ValueError("out must be as q, with contiguous head_dim")
+    lse = torch.empty((h, s), dtype=torch.float32, device=q.device) if with_lse else None
+    for a in range(0, s, _lib.DECODE_PAGED_MAX_SEQS):
+        b = min(s, a + _lib.DECODE_PAGED_MAX_SEQS)
+        part = None if starts is None else starts[a:b]
+        PagedDecode(pc, block_table[a:b], seq_lens[a:b], h, window, part).run(
+            q[a:b], out[a:b], pc, scale, keep_nan, None if lse is None else lse[:, a:b])
+    return (out, lse) if with_lse else out
 
 
 def decode_attn(

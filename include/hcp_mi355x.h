@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define HCP_ABI_VERSION 11
+#define HCP_ABI_VERSION 12
 
 typedef enum hcp_status {
   HCP_OK = 0,
@@ -516,6 +516,7 @@ typedef struct hcp_decode_paged_args {
   int32_t num_heads, num_kv_heads, head_dim, dtype;
   int32_t keep_nan; /* as in hcp_decode_args */
   float scale;
+  const void* seq_starts; /* hcp_decode_fp4: first key seen, DEVICE [num_seqs] of lens_dtype (NULL: 0) */
 } hcp_decode_paged_args;
 
 size_t hcp_decode_paged_workspace(int32_t num_seqs, int32_t num_heads,
@@ -673,6 +674,166 @@ int hcp_gather_paged_kv(const hcp_varlen_entry* entries, int32_t num_entries,
                         const int64_t* out_start, int64_t max_len,
                         int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                         void* k_out, void* v_out, void* stream);
+
+/*
+ * ---- The 4-bit KV cache ----
+ *
+ * K and V held as 4-bit codes (sign, two bits of exponent, one of mantissa: 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6) with a power-of-two scale for 32 columns of a head's
+ * row, 17 / 32 byte a value.  No counterpart in the reference, whose cache holds
+ * the model's type.  Block `blk` and KV head `h` own the head_dim * block_size *
+ * 17 / 16 bytes at addr + blk * stride_block + h * stride_head (strides in BYTES,
+ * multiples of 16), in this order, B = block_size, d = head_dim:
+ *   K codes   [B][d / 2]           a byte: two columns, the even one in the low half
+ *   V codes   [B / 4][d / 8][4 keys][4 bytes]
+ *   K scales  [B / 4][d / 32][4 keys]   byte b: 2^(b - 127); 255: NaN
+ *   V scales  [B / 4][d / 32][4 keys]
+ * head_dim is a multiple of 32 up to 256, block_size a power of two from 16 to
+ * 65536.  Writing takes the least scale of which the 32 values' largest magnitude
+ * is at most 7 times it and the nearest code, ties to the even one; 32 values with
+ * an infinity or a NaN among them become NaN.  What a code stands for is exact in
+ * the 16-bit type that was written (`dtype`; scales are kept to 2^-125 .. 2^125 for
+ * bf16 and 2^-23 .. 2^13 for fp16, magnitudes past 6 times the largest becoming 6
+ * times it): read it with the type it was written with.
+ */
+typedef struct hcp_fp4_cache {
+  uint64_t addr;
+  int64_t stride_block;
+  int64_t stride_head;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t head_dim;
+} hcp_fp4_cache;
+
+/*
+ * hcp_reshape_and_cache into a 4-bit cache: the same rows, slots and skipped
+ * slots.  `cache` is a HOST pointer.
+ */
+int hcp_fp4_write(const void* key, int64_t k_stride_tok, int64_t k_stride_head,
+                  const void* value, int64_t v_stride_tok, int64_t v_stride_head,
+                  const void* slot_mapping, int32_t slot_dtype, int64_t num_tokens,
+                  int32_t num_kv_heads, const hcp_fp4_cache* cache, int32_t dtype,
+                  void* stream);
+
+/*
+ * What a 4-bit cache stands for at num_tokens slots, as [num_tokens, Hkv,
+ * head_dim] contiguous K and V of `dtype` (16-byte aligned); a slot that is
+ * negative or past the cache reads as zeros.
+ */
+int hcp_fp4_read(const void* slot_mapping, int32_t slot_dtype, int64_t num_tokens,
+                 int32_t num_kv_heads, const hcp_fp4_cache* cache, int32_t dtype,
+                 void* k_out, void* v_out, void* stream);
+
+/*
+ * hcp_gather_paged_kv out of a 4-bit cache: entry e's keys [kv.start, kv.start +
+ * kv.len), through its kv.block_table alone (the other fields of kv are not read;
+ * an entry without one is skipped), become rows out_start[e] .. of k_out / v_out.
+ * A block id past the cache reads its last block.  entries_out [num_entries]
+ * (DEVICE, may be NULL) gets the entries with kv the contiguous segment of k_out /
+ * v_out that they now have, for hcp_varlen_launch to read behind this call.
+ */
+int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries,
+                   const int64_t* out_start, int64_t max_len, int32_t num_kv_heads,
+                   const hcp_fp4_cache* cache, int32_t dtype, void* k_out, void* v_out,
+                   hcp_varlen_entry* entries_out, void* stream);
+
+/*
+ * hcp_decode_paged over a 4-bit cache.  Of args->kv: k_addr, stride_block,
+ * stride_head (BYTES), block_size, num_blocks (> 0) and block_table, as in
+ * hcp_fp4_cache; v_addr and stride_tok are not read.  A block id past the cache
+ * reads its last block.  With seq_starts, sequence r sees keys seq_starts[r] ..
+ * seq_lens[r] - 1 (of these the last `window`): the keys behind a staged prefix.
+ */
+size_t hcp_decode_fp4_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                int32_t head_dim);
+int hcp_decode_fp4(const hcp_decode_paged_args* args, void* stream);
+
+/*
+ * Per-head norms of q and k, rotation by position and cache write, one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight over each head's row (weight NULL: as it is),
+ *   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s) over the pairs i, j = i + rot / 2
+ *   (interleaved: 2 i, 2 i + 1) of the first rot columns, c = table[pos][i],
+ *   s = table[pos][rot / 2 + i],
+ * computed in 32 bits (64 for keys into a 4-bit cache), then rounded.  No
+ * counterpart in the reference, whose model code does this before the backend.
+ *   positions    DEVICE [num_tokens], HCP_DTYPE_I32 or I64; one outside the table
+ *                takes its first or last row
+ *   cos_sin      DEVICE [max_positions, rot], `dtype` or F32 (table_dtype), rows
+ *                table_stride elements apart
+ *   weights      DEVICE [head_dim], `dtype` or F32 (weight_dtype), either may be NULL
+ *   q_out, k_out may be q and k; k_out may be NULL
+ *   cache_kind   0: none; 1: `cache`; 2: `fp4`.  The rotated key and the value of
+ *                token t < num_slots go to slot_mapping[t], slots outside the
+ *                cache skipped, as in hcp_reshape_and_cache
+ * head_dim a multiple of 8 up to 256, rot a multiple of 16 up to head_dim (0: no
+ * rotation); 16-byte aligned rows.  `cache` and `fp4` are HOST pointers.
+ */
+typedef struct hcp_qk_rope_args {
+  const void* q;
+  int64_t q_stride_tok, q_stride_head;
+  const void* k;
+  int64_t k_stride_tok, k_stride_head;
+  const void* v;
+  int64_t v_stride_tok, v_stride_head;
+  void* q_out;
+  int64_t qo_stride_tok, qo_stride_head;
+  void* k_out;
+  int64_t ko_stride_tok, ko_stride_head;
+  const void* q_weight;
+  const void* k_weight;
+  const void* positions;
+  const void* cos_sin;
+  int64_t table_stride, max_positions;
+  const void* slot_mapping;
+  int64_t num_slots;
+  const hcp_paged_cache* cache;
+  const hcp_fp4_cache* fp4;
+  int64_t num_tokens;
+  double eps;
+  int32_t num_heads, num_kv_heads, head_dim, rot;
+  int32_t dtype, weight_dtype, table_dtype, pos_dtype, slot_dtype;
+  int32_t interleaved, cache_kind, reserved;
+} hcp_qk_rope_args;
+
+int hcp_qk_norm_rope(const hcp_qk_rope_args* args, void* stream);
+
+/*
+ * Block table, slots and positions of a step, from the requests' lengths on the
+ * device: what the reference's engine makes on the host.  With held = ceil(ctx /
+ * block_size) and need = ceil((ctx + new) / block_size) blocks of a request,
+ * entries held .. need - 1 of its block-table row get the next free blocks, in the
+ * requests' order; its new tokens are at positions ctx .. ctx + new - 1.
+ *   ctx_lens, new_lens   DEVICE [num_seqs], HCP_DTYPE_I32 or I64; counted as 0
+ *                        below 0 and as 2^30 past that
+ *   block_table          DEVICE int32, num_seqs rows of table_width ids; updated
+ *   free_blocks          DEVICE int32 [num_free]
+ *   query_start_loc [num_seqs + 1], seq_lens [num_seqs], blocks_used [1]  DEVICE int32
+ *   positions, slot_mapping [num_tokens]  DEVICE int64; rows past the new tokens get
+ *                        position 0 and slot -1, tokens past the rows are not listed
+ * blocks_used is what the step takes; past num_free the entries become -1 and
+ * the slots in them -1 (not written by the cache writes).  Tokens past the keys a
+ * row can name get slot -1 and take no block.  At most HCP_STEP_MAX_SEQS requests.
+ */
+#define HCP_STEP_MAX_SEQS 4096
+typedef struct hcp_step_tables_args {
+  const void* ctx_lens;
+  const void* new_lens;
+  int64_t ctx_stride, new_stride;
+  int32_t* block_table;
+  int64_t table_stride, table_width;
+  const int32_t* free_blocks;
+  int64_t num_free;
+  int64_t num_tokens;
+  int32_t* query_start_loc;
+  int32_t* seq_lens;
+  int32_t* blocks_used;
+  int64_t* positions;
+  int64_t* slot_mapping;
+  int32_t ctx_dtype, new_dtype;
+  int32_t num_seqs, block_size;
+} hcp_step_tables_args;
+
+int hcp_step_tables(const hcp_step_tables_args* args, void* stream);
 
 #ifdef __cplusplus
 }
