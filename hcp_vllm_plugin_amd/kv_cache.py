@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .varlen import PagedCache
+from .varlen import PagedCache, fp4_desc
 
 __all__ = ["reshape_and_cache", "fp4_cache_shape", "gather_kv"]
 
@@ -67,44 +67,43 @@ def fp4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int,
     return (num_blocks, num_kv_heads, block_size, head_dim + head_dim // 16)
 
 
-def fp4_desc(pc: PagedCache) -> "_lib.Fp4CacheDesc":
-    return _lib.Fp4CacheDesc(pc.k_addr, pc.stride_block, pc.stride_head, pc.num_blocks,
-                             pc.block_size, pc.head_dim)
+_INDEX_CODES = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
 
-def _check_slots(slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> None:
-    if slot_mapping.dtype not in (torch.int32, torch.int64) or slot_mapping.dim() != 1:
+def check_slots(slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> torch.Tensor:
+    """``slot_mapping`` as the kernels read it."""
+    if slot_mapping.dtype not in _INDEX_CODES or slot_mapping.dim() != 1:
         raise ValueError("slot_mapping must be int32 or int64, of one dimension")
     if not kv_cache.is_cuda or slot_mapping.device != kv_cache.device:
         raise ValueError("slot_mapping must be on the cache's GPU")
+    return slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
 
 
 def _write_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
                slot_mapping: torch.Tensor) -> None:
-    pc = PagedCache.from_tensor(kv_cache)
-    n = slot_mapping.numel()
-    if key.shape != value.shape or key.dim() != 3:
+    desc, hkv, d = fp4_desc(kv_cache)
+    n, shape, dt, dev = slot_mapping.shape[0], key.shape, key.dtype, kv_cache.device
+    if shape != value.shape or len(shape) != 3:
         raise ValueError("key/value must be [N, Hkv, D] of one shape")
-    if key.shape[0] < n:
-        raise ValueError(f"{n} slots for {key.shape[0]} key rows")
-    if key.shape[1] != pc.num_kv_heads or key.shape[2] != pc.head_dim:
+    if shape[0] < n:
+        raise ValueError(f"{n} slots for {shape[0]} key rows")
+    if shape[1] != hkv or shape[2] != d:
         raise ValueError("key/value heads or head_dim do not match the cache")
-    if key.dtype not in (torch.float16, torch.bfloat16) or value.dtype != key.dtype:
+    if dt not in (torch.float16, torch.bfloat16) or value.dtype != dt:
         raise ValueError("key/value must both be float16 or bfloat16")
-    if key.stride(-1) != 1 or value.stride(-1) != 1:
+    ks, vs = key.stride(), value.stride()
+    if ks[2] != 1 or vs[2] != 1:
         raise ValueError("key/value head_dim must be contiguous")
-    _check_slots(slot_mapping, kv_cache)
-    if key.device != kv_cache.device or value.device != kv_cache.device:
+    slots = check_slots(slot_mapping, kv_cache)
+    if key.device != dev or value.device != dev:
         raise ValueError("key/value must be on the cache's GPU")
     if n == 0:
         return
-    slots, desc = slot_mapping.contiguous(), fp4_desc(pc)
-    with _lib.on_device(key.device):
+    with _lib.on_device(dev):
         rc = _lib.lib().hcp_fp4_write(
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-            value.stride(1), slots.data_ptr(),
-            _lib.DTYPE_I64 if slots.dtype == torch.int64 else _lib.DTYPE_I32, n, pc.num_kv_heads,
-            ctypes.addressof(desc), _lib.dtype_code(key.dtype), _lib.stream_ptr(key.device))
+            key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], slots.data_ptr(),
+            _INDEX_CODES[slots.dtype], n, hkv, ctypes.addressof(desc), _lib.dtype_code(dt),
+            _lib.stream_ptr(dev))
     _lib.check(rc, "hcp_fp4_write")
 
 
@@ -113,23 +112,19 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     """K and V ``[n, Hkv, D]`` that a 4-bit cache stands for at ``slot_mapping``,
     in the 16-bit ``dtype`` they were written in (exactly: a code's value has two
     significant bits).  A slot that is negative or past the cache reads as zeros."""
-    if kv_cache.dtype != torch.uint8:
-        raise ValueError("gather_kv reads a 4-bit cache (uint8)")
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("dtype must be float16 or bfloat16")
-    pc = PagedCache.from_tensor(kv_cache)
-    _check_slots(slot_mapping, kv_cache)
-    slots, desc = slot_mapping.contiguous(), fp4_desc(pc)
-    kv = torch.empty((2, slots.shape[0], pc.num_kv_heads, pc.head_dim), dtype=dtype,
-                     device=kv_cache.device)
-    k, v = kv[0], kv[1]
-    with _lib.on_device(kv_cache.device):
+    desc, hkv, d = fp4_desc(kv_cache)
+    slots, dev = check_slots(slot_mapping, kv_cache), kv_cache.device
+    n = slots.shape[0]
+    kv = torch.empty((2, n, hkv, d), dtype=dtype, device=dev)
+    base = kv.data_ptr()
+    with _lib.on_device(dev):
         rc = _lib.lib().hcp_fp4_read(
-            slots.data_ptr(), _lib.DTYPE_I64 if slots.dtype == torch.int64 else _lib.DTYPE_I32,
-            slots.shape[0], pc.num_kv_heads, ctypes.addressof(desc), _lib.dtype_code(dtype),
-            k.data_ptr(), v.data_ptr(), _lib.stream_ptr(kv_cache.device))
+            slots.data_ptr(), _INDEX_CODES[slots.dtype], n, hkv, ctypes.addressof(desc),
+            _lib.dtype_code(dtype), base, base + 2 * n * hkv * d, _lib.stream_ptr(dev))
     _lib.check(rc, "hcp_fp4_read")
-    return k, v
+    return kv.unbind(0)
 
 
 def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,

@@ -16,23 +16,25 @@ import ctypes
 import torch
 
 from . import _lib
-from .kv_cache import _cache_desc, _check_slots, fp4_desc
-from .varlen import PagedCache
+from .kv_cache import _cache_desc, check_slots
+from .varlen import fp4_desc
 
 __all__ = ["qk_norm_rope"]
 
 _INDEX = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
 
-def _rows(name: str, t: torch.Tensor, like: torch.Tensor, heads: int | None = None) -> None:
-    """``t`` [T, heads, D] with the kernel's rows, of like's tokens, width, type and device."""
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
-            (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit query and key")
-    if t.dtype != like.dtype or t.device != like.device:
+def _rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype,
+          device: torch.device) -> tuple[int, int]:
+    """Token and head stride of ``t``, which must have the kernel's rows."""
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, not {shape}")
+    if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be of query's dtype and device")
-    if t.stride(2) != 1 or t.data_ptr() % 16 or t.stride(0) % 8 or t.stride(1) % 8:
+    tok, head, col = t.stride()
+    if col != 1 or (t.data_ptr() | 2 * tok | 2 * head) & 15:
         raise ValueError(f"{name}: 16-byte aligned rows with contiguous head_dim")
+    return tok, head
 
 
 def qk_norm_rope(
@@ -67,89 +69,87 @@ def qk_norm_rope(
     into the cache at ``slot_mapping[t]`` (tokens past its length and negative
     slots are not written); the key then comes back only where ``key_out`` asks
     for it.  ``query_out`` / ``key_out`` may be query and key themselves."""
-    if query.dtype not in (torch.float16, torch.bfloat16) or not query.is_cuda:
-        raise ValueError("query must be float16/bfloat16 on the GPU")
-    _rows("query", query, query)
-    _rows("key", key, query)
+    dt, dev = query.dtype, query.device
+    if dt not in (torch.float16, torch.bfloat16) or dev.type != "cuda" or query.dim() != 3 or \
+            key.dim() != 3:
+        raise ValueError("query and key must be float16/bfloat16 [T, heads, D] on the GPU")
     t, h, d = query.shape
-    hkv, dev = key.shape[1], query.device
-    if positions.dtype not in _INDEX or tuple(positions.shape) != (t,) or \
-            not positions.is_contiguous() or positions.device != dev:
+    hkv = key.shape[1]
+    a = _lib.QkRopeArgs()
+    a.q_stride_tok, a.q_stride_head = _rows("query", query, (t, h, d), dt, dev)
+    a.k_stride_tok, a.k_stride_head = _rows("key", key, (t, hkv, d), dt, dev)
+    if positions.dtype not in _INDEX or positions.shape != (t,) or positions.device != dev or \
+            not positions.is_contiguous():
         raise ValueError("positions must be contiguous int32/int64 [T] on query's device")
     tab = cos_sin_cache
-    if tab.dim() != 2 or tab.stride(1) != 1 or tab.device != dev or \
-            tab.dtype not in (torch.float32, query.dtype):
+    if tab.dim() != 2 or tab.device != dev or tab.dtype not in (torch.float32, dt):
         raise ValueError("cos_sin_cache must be [max_positions, rot], float32 or query's dtype, on "
                          "query's device")
-    if tab.shape[1] % 16 or tab.shape[1] > d or (tab.shape[1] and tab.shape[0] == 0):
-        raise ValueError("rot must be a multiple of 16 up to head_dim, and the table not empty")
-    if tab.shape[1] and (tab.data_ptr() % 16 or tab.stride(0) % 8):
-        raise ValueError("cos_sin_cache: 16-byte aligned rows")
+    most, rot = tab.shape
+    if rot:
+        row, col = tab.stride()
+        if rot % 16 or rot > d or most == 0:
+            raise ValueError("rot must be a multiple of 16 up to head_dim, and the table not empty")
+        if col != 1 or tab.data_ptr() % 16 or row % 8:
+            raise ValueError("cos_sin_cache: 16-byte aligned rows")
+        a.cos_sin, a.table_stride, a.max_positions = tab.data_ptr(), row, most
     wide = None
     for w in (q_weight, k_weight):
         if w is None:
             continue
-        if tuple(w.shape) != (d,) or w.stride(0) != 1 or w.device != dev or w.data_ptr() % 16 or \
-                w.dtype not in (torch.float32, query.dtype) or w.dtype != (wide or w.dtype):
+        if w.shape != (d,) or w.stride(0) != 1 or w.device != dev or w.data_ptr() % 16 or \
+                w.dtype not in (torch.float32, dt) or w.dtype != (wide or w.dtype):
             raise ValueError("weights must be [head_dim] and of one dtype, float32 or query's, on "
                              "query's device")
         wide = w.dtype
-    a = _lib.QkRopeArgs()
-    a.slot_dtype, hold = _lib.DTYPE_I64, None
+    a.slot_dtype = _lib.DTYPE_I64
     if kv_cache is None:
         if value is not None or slot_mapping is not None:
             raise ValueError("value and slot_mapping go with a kv_cache")
         if key_out is None:
-            key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
+            key_out = torch.empty((t, hkv, d), dtype=dt, device=dev)
     else:
         if value is None or slot_mapping is None:
             raise ValueError("a cache write needs value and slot_mapping")
-        _rows("value", value, query, hkv)
-        _check_slots(slot_mapping, kv_cache)
+        a.v_stride_tok, a.v_stride_head = _rows("value", value, (t, hkv, d), dt, dev)
+        a.v = value.data_ptr()
+        slots = check_slots(slot_mapping, kv_cache)
         if kv_cache.device != dev:
             raise ValueError("kv_cache must be on query's device")
-        if slot_mapping.shape[0] > t:
-            raise ValueError(f"{slot_mapping.shape[0]} slots for {t} tokens")
-        slots = slot_mapping.contiguous()
+        if slots.shape[0] > t:
+            raise ValueError(f"{slots.shape[0]} slots for {t} tokens")
         a.slot_mapping, a.num_slots, a.slot_dtype = slots.data_ptr(), slots.shape[0], \
             _INDEX[slots.dtype]
-        a.v, a.v_stride_tok, a.v_stride_head = value.data_ptr(), value.stride(0), value.stride(1)
         if kv_cache.dtype == torch.uint8:
-            pc = PagedCache.from_tensor(kv_cache)
-            c_hkv, c_d, desc = pc.num_kv_heads, pc.head_dim, fp4_desc(pc)
+            desc, c_hkv, c_d = fp4_desc(kv_cache)
             a.cache_kind, a.fp4 = 2, ctypes.addressof(desc)
         else:
-            if kv_cache.dtype != query.dtype:
+            if kv_cache.dtype != dt:
                 raise ValueError("kv_cache must be of query's dtype, or a 4-bit cache (uint8)")
-            desc, addr, c_hkv, c_d = _cache_desc(kv_cache)
-            a.cache_kind, a.cache = 1, addr
+            desc, a.cache, c_hkv, c_d = _cache_desc(kv_cache)
+            a.cache_kind = 1
         if c_hkv != hkv or c_d != d:
             raise ValueError("key heads or head_dim do not match the cache")
-        hold = (slots, desc)
     if query_out is None:
-        query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        query_out = torch.empty((t, h, d), dtype=dt, device=dev)
+        a.qo_stride_tok, a.qo_stride_head = h * d, d
     else:
-        _rows("query_out", query_out, query, h)
+        a.qo_stride_tok, a.qo_stride_head = _rows("query_out", query_out, (t, h, d), dt, dev)
     if key_out is not None:
-        _rows("key_out", key_out, query, hkv)
-        a.k_out, a.ko_stride_tok, a.ko_stride_head = key_out.data_ptr(), key_out.stride(0), \
-            key_out.stride(1)
-    a.q, a.q_stride_tok, a.q_stride_head = query.data_ptr(), query.stride(0), query.stride(1)
-    a.k, a.k_stride_tok, a.k_stride_head = key.data_ptr(), key.stride(0), key.stride(1)
-    a.q_out, a.qo_stride_tok, a.qo_stride_head = query_out.data_ptr(), query_out.stride(0), \
-        query_out.stride(1)
+        a.ko_stride_tok, a.ko_stride_head = _rows("key_out", key_out, (t, hkv, d), dt, dev)
+        a.k_out = key_out.data_ptr()
+    a.q, a.k, a.q_out = query.data_ptr(), key.data_ptr(), query_out.data_ptr()
     if q_weight is not None:
         a.q_weight = q_weight.data_ptr()
     if k_weight is not None:
         a.k_weight = k_weight.data_ptr()
     a.positions, a.pos_dtype = positions.data_ptr(), _INDEX[positions.dtype]
-    if tab.shape[1]:
-        a.cos_sin, a.table_stride, a.max_positions = tab.data_ptr(), tab.stride(0), tab.shape[0]
-    a.num_tokens, a.eps = t, eps
-    a.num_heads, a.num_kv_heads, a.head_dim, a.rot = h, hkv, d, tab.shape[1]
-    a.dtype, a.table_dtype = _lib.dtype_code(query.dtype), _lib.dtype_code(tab.dtype)
-    a.weight_dtype = _lib.dtype_code(wide or query.dtype)
-    a.interleaved = bool(interleaved)
+    a.num_tokens, a.eps, a.interleaved = t, eps, bool(interleaved)
+    a.num_heads, a.num_kv_heads, a.head_dim, a.rot = h, hkv, d, rot
+    a.dtype = a.weight_dtype = _lib.dtype_code(dt)
+    if wide == torch.float32:
+        a.weight_dtype = _lib.DTYPE_F32
+    a.table_dtype = _lib.DTYPE_F32 if tab.dtype == torch.float32 else a.dtype
     with _lib.on_device(dev):
         rc = _lib.lib().hcp_qk_norm_rope(ctypes.addressof(a), _lib.stream_ptr(dev))
     _lib.check(rc, "hcp_qk_norm_rope")

@@ -80,13 +80,9 @@ class PagedCache:
             raise ValueError("paged cache: last dim must be contiguous")
         es = cache.element_size()
         if cache.dtype == torch.uint8:
-            if cache.dim() != 4 or cache.shape[3] == 0 or cache.shape[3] % 34 or \
-                    cache.stride(2) != cache.shape[3]:
-                raise ValueError("4-bit cache: uint8 [blocks, Hkv, block_size, D + D / 16], the "
-                                 "bytes of a block and head contiguous")
-            nb, hkv, bs, row = cache.shape
-            return cls(cache, "fp4", hkv, row // 17 * 16, bs, cache.data_ptr(), cache.data_ptr(),
-                       0, cache.stride(1), cache.stride(0))
+            desc, hkv, d = fp4_desc(cache)
+            return cls(cache, "fp4", hkv, d, desc.block_size, desc.addr, desc.addr, 0,
+                       desc.stride_head, desc.stride_block)
         if cache.dim() == 4:  # [nb, Hkv, bs, 2D]
             nb, hkv, bs, d2 = cache.shape
             d = d2 // 2
@@ -99,6 +95,18 @@ class PagedCache:
                        cache.data_ptr() + cache.stride(1) * es,
                        cache.stride(2), cache.stride(3), cache.stride(0))
         raise ValueError(f"unrecognised paged cache shape {tuple(cache.shape)}")
+
+
+def fp4_desc(cache: torch.Tensor) -> tuple["_lib.Fp4CacheDesc", int, int]:
+    """(descriptor, KV heads, head_dim) of a 4-bit cache."""
+    shape, stride = cache.shape, cache.stride()
+    if cache.dtype != torch.uint8 or len(shape) != 4 or shape[3] == 0 or shape[3] % 34 or \
+            stride[3] != 1 or stride[2] != shape[3]:
+        raise ValueError("4-bit cache: uint8 [blocks, Hkv, block_size, D + D / 16], the bytes of a "
+                         "block and head contiguous")
+    nb, hkv, bs, row = shape
+    d = row // 17 * 16
+    return _lib.Fp4CacheDesc(cache.data_ptr(), stride[0], stride[1], nb, bs, d), hkv, d
 
 
 def segment_contiguous(k: torch.Tensor, v: torch.Tensor, start: int = 0,
@@ -922,6 +930,9 @@ class PagedDecode:
         _lib.check(rc, "hcp_decode_fp4" if self._fp4 else "hcp_decode_paged")
 
 
+_INDEX_CODES = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
+
+
 def decode_fp4(
     q: torch.Tensor,
     kv_cache: torch.Tensor,
@@ -941,33 +952,63 @@ def decode_fp4(
     read on the device when the call executes.  A query that sees no key gets
     out 0 and LSE -inf; a length past its table row counts as the row's keys.
     ``keep_nan``: as ``DecodeBatch.run``.  Returns out (and lse float32 ``[H, S]``)."""
-    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or q.stride(-1) != 1:
+    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or q.stride(2) != 1:
         raise ValueError("q must be float16/bfloat16 [S, H, D] with contiguous head_dim")
-    pc = PagedCache.from_tensor(kv_cache)
+    desc, hkv, dim = fp4_desc(kv_cache)
     s, h, d = q.shape
-    if pc.layout != "fp4" or d != pc.head_dim or h % pc.num_kv_heads:
+    if d != dim or h % hkv:
         raise ValueError("kv_cache must be a 4-bit cache of q's head_dim, its heads dividing q's")
     if window is not None and window <= 0:
         raise ValueError("window must be a positive number of keys")
+    dev = q.device
     for name, t in (("seq_lens", seq_lens), ("starts", starts)):
-        if t is not None and (t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (s,)
+        if t is not None and (t.dtype not in _INDEX_CODES or t.shape != (s,) or t.device != dev
                               or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous int32/int64 [S]")
-    for t in (q, kv_cache, block_table, seq_lens, starts, out):
-        if t is not None and (not t.is_cuda or t.device != q.device):
-            raise ValueError("all tensors must be on q's GPU")
+            raise ValueError(f"{name} must be contiguous int32/int64 [S] on q's GPU")
+    if starts is not None and starts.dtype != seq_lens.dtype:
+        raise ValueError("starts must be of seq_lens' dtype")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < s or \
+            block_table.stride(1) != 1 or block_table.device != dev:
+        raise ValueError("block_table must be int32 with contiguous rows, one for each query, on q's "
+                         "GPU")
+    if not q.is_cuda or kv_cache.device != dev:
+        raise ValueError("all tensors must be on one GPU")
     if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
         q = q.contiguous()
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+        out = torch.empty((s, h, d), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
         raise ValueError("out must be as q, with contiguous head_dim")
-    lse = torch.empty((h, s), dtype=torch.float32, device=q.device) if with_lse else None
-    for a in range(0, s, _lib.DECODE_PAGED_MAX_SEQS):
-        b = min(s, a + _lib.DECODE_PAGED_MAX_SEQS)
-        part = None if starts is None else starts[a:b]
-        PagedDecode(pc, block_table[a:b], seq_lens[a:b], h, window, part).run(
-            q[a:b], out[a:b], pc, scale, keep_nan, None if lse is None else lse[:, a:b])
+    lse = torch.empty((h, s), dtype=torch.float32, device=dev) if with_lse else None
+    L = _lib.lib()
+    a = _lib.DecodePagedArgs()
+    a.q_stride_tok, a.q_stride_head, _ = q.stride()
+    a.o_stride_tok, a.o_stride_head, _ = out.stride()
+    a.kv.k_addr, a.kv.stride_head, a.kv.stride_block = desc.addr, desc.stride_head, desc.stride_block
+    a.kv.block_size, a.kv.num_blocks = desc.block_size, desc.num_blocks
+    bt_row = block_table.stride(0)
+    a.block_table_stride, a.block_table_width = bt_row, block_table.shape[1]
+    a.lens_dtype = _INDEX_CODES[seq_lens.dtype]
+    a.num_heads, a.num_kv_heads, a.head_dim = h, hkv, d
+    a.dtype, a.scale, a.keep_nan, a.window = _lib.dtype_code(q.dtype), scale, keep_nan, window or 0
+    a.lse_stride_head = s
+    with _lib.on_device(dev):
+        stream = _lib.stream_ptr(dev)
+        for first in range(0, s, _lib.DECODE_PAGED_MAX_SEQS):
+            n = a.num_seqs = min(s - first, _lib.DECODE_PAGED_MAX_SEQS)
+            a.q = q.data_ptr() + 2 * first * a.q_stride_tok
+            a.out = out.data_ptr() + 2 * first * a.o_stride_tok
+            a.kv.block_table = block_table.data_ptr() + 4 * first * bt_row
+            a.seq_lens = seq_lens.data_ptr() + first * seq_lens.element_size()
+            if starts is not None:
+                a.seq_starts = starts.data_ptr() + first * starts.element_size()
+            if lse is not None:
+                a.lse = lse.data_ptr() + 4 * first
+            # fp32 partials: stream-ordered scratch from torch's caching allocator
+            a.workspace_bytes = L.hcp_decode_fp4_workspace(n, h, hkv, d)
+            ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
+            a.workspace = ws.data_ptr()
+            _lib.check(L.hcp_decode_fp4(ctypes.addressof(a), stream), "hcp_decode_fp4")
     return (out, lse) if with_lse else out
 
 
