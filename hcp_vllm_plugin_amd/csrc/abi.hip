@@ -1175,7 +1175,8 @@ static int32_t paged_wgs(int32_t num_heads, int32_t num_kv_heads, int32_t per_cu
   return std::max(1, per_cu * kNumCus / (num_kv_heads * chunks));
 }
 constexpr int32_t kPagedPerCu = 1;  // a workgroup's chunk buffers take 128 KB of a CU's LDS
-constexpr int32_t kFp4PerCu = 2;    // chunks in registers: two waves to a SIMD
+// 4-bit chunks: two workgroups to a CU, four at 64 columns (256 or 128 registers)
+static int32_t fp4_per_cu(int32_t head_dim) { return head_dim <= 64 ? 4 : 2; }
 
 static size_t unplanned_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                   int32_t head_dim, int32_t per_cu) {
@@ -1194,7 +1195,7 @@ size_t hcp_decode_paged_workspace(int32_t num_seqs, int32_t num_heads, int32_t n
 
 size_t hcp_decode_fp4_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                 int32_t head_dim) {
-  return unplanned_workspace(num_seqs, num_heads, num_kv_heads, head_dim, kFp4PerCu);
+  return unplanned_workspace(num_seqs, num_heads, num_kv_heads, head_dim, fp4_per_cu(head_dim));
 }
 
 // A region of the 4-bit cache: what the kernels' 32-bit offsets and 16-byte
@@ -1249,7 +1250,7 @@ static int decode_unplanned(const hcp_decode_paged_args* a, bool fp4, const char
   if (a->block_table_width > ((int64_t{1} << 34) / kv.block_size) / a->num_seqs ||
       a->block_table_width * kv.block_size > INT32_MAX)
     return fail(HCP_EUNSUPPORTED, "%s: block table names too many keys", who);
-  const int32_t per_cu = fp4 ? kFp4PerCu : kPagedPerCu;
+  const int32_t per_cu = fp4 ? fp4_per_cu(a->head_dim) : kPagedPerCu;
   const size_t need =
       unplanned_workspace(a->num_seqs, a->num_heads, a->num_kv_heads, a->head_dim, per_cu);
   if (!a->workspace || a->workspace_bytes < need)

@@ -544,7 +544,7 @@ decode_paged_kernel(PagedDecParams p_) {
   const int chunk = static_cast<int>(item % p_.d.head_chunks);
   const int wg = static_cast<int>(item / p_.d.head_chunks);
   const int n = p_.num_seqs;
-  paged_shares<NT, kStart, 2, false>(p_, wg, sm_len, sm_all, sm_w, sm_cut,
+  paged_shares<NT, kStart, 2, 1, false>(p_, wg, sm_len, sm_all, sm_w, sm_cut,
                               [](int, int len) { return (len >> 5) + ((len & 31) != 0); });
   const int r0 = __builtin_amdgcn_readfirstlane(sm_cut[0]);
   const int o0 = __builtin_amdgcn_readfirstlane(sm_cut[1]);

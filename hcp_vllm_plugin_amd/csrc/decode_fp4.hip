@@ -6,9 +6,9 @@
 // d + d / 16 bytes where 16-bit values take 4 d, so the same HBM rate would ask for
 // 3.8 times the keys per second, and what a key costs in instructions counts:
 //  * the cache lies as the matrix operands do (fp4.h): a lane loads 32 columns of
-//    one key of K, or 8 columns of four keys of V, in 16 bytes straight into
-//    registers, a wave 1 KB in a row; one v_cvt_scalef32_pk makes two 16-bit
-//    operand values of a byte, exactly, its scale applied;
+//    one key of K, or 8 columns of four keys of V, in 16 bytes, a wave 1 KB in a
+//    row; one v_cvt_scalef32_pk makes two 16-bit operand values of a byte, exactly,
+//    its scale applied;
 //  * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32 as in decode_split_body:
 //    16 query heads are the columns, the contraction order of either product is
 //    free, so K's is the order of a lane's bytes and P stays in the registers S
@@ -16,29 +16,38 @@
 //  * the running maximum is raised, and O rescaled, only when a score is past it
 //    by 2^8 (fp32 sums and two 16-bit terms of P have room for that).
 // The 4 waves of a workgroup take the 32-key chunks of its share in turn (chunks
-// lie on multiples of 32 positions, so that 16 keys never cross a block), the next
-// chunk's loads in flight, and are combined through LDS; decode_reduce_kernel
+// lie on multiples of 32 positions, so that 16 keys never cross a block), each
+// through LDS of its own, where the next chunk lands while one is computed (held
+// in registers instead, two chunks take 212 of them at 128 columns and spill at
+// 256: 364 us for 32 x 4k-16k keys of 16 / 8 x 256, now 137; 14 / 2 x 64, 64 x
+// 16k-32k 64 -> 51 us).  The waves are combined through LDS; decode_reduce_kernel
 // merges a sequence's partials.
+//
+// Bound by HBM: 64 x 16k-32k keys of 28 / 4 x 128 (850 MB) take 148 us with the
+// merge, 5.7 TB/s; its loads alone, without the arithmetic, take 142, and the
+// 16-bit kernel reads blocks at 6.1 TB/s.  One sequence of 2000 keys: 11.4 us, the
+// chain of latencies (lengths, block ids, keys, combine, merge).
 #include "decode_share.h"
 
 namespace hcp {
 
-// What a wave holds of a chunk (32 keys: two tiles of 16).
+// A wave's tile (16 keys) in LDS: its codes, each lane's 16 bytes of a load next to
+// the other lanes', then its scales.
 template <int D>
-struct Fp4Chunk {
-  static constexpr int KW = D / 32;           // dwords of K per lane and tile
-  static constexpr int KS = D == 256 ? 2 : 1; // K scales per lane and tile
-  static constexpr int VP = D == 256 ? 2 : 1; // octets of V per lane and tile
-  uint32_t k[2][KW];
-  uint32_t ks[2][KS];
-  uint32_t v[2][VP][4];  // [key of the quad]
-  uint32_t vs[2];
+struct Fp4Tile {
+  static constexpr int NC = D / 64;             // loads of codes, 1 KB each
+  static constexpr int SC = 1024 * NC;          // where the scales begin
+  static constexpr int SW = D == 256 ? 32 : 16; // dwords of K (or V) scales
+  static constexpr int BYTES = SC + 256;
+  static constexpr int NI = NC + 1;             // loads
+  static constexpr int P = D == 256 ? 2 : 1;    // 16-byte pieces of K (or V) per lane
 };
 
+#define HCP_LDS_PTR(T) __attribute__((address_space(3))) T*
+
 template <typename T>
-__device__ __forceinline__ T ldnt(const char* p) {
-  return __builtin_nontemporal_load(
-      (const __attribute__((address_space(1))) T*)(reinterpret_cast<uintptr_t>(p)));
+__device__ __forceinline__ T lds_at(const HCP_LDS_PTR(char) p) {
+  return *reinterpret_cast<const HCP_LDS_PTR(T)>(p);
 }
 
 constexpr float kRaise = 8.f;  // how far (in powers of two) a score may pass the running maximum
@@ -46,11 +55,12 @@ constexpr float kRaise = 8.f;  // how far (in powers of two) a score may pass th
 template <int D, typename T, bool KEEP_NAN>
 __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_in, int chunk_in,
                                                int slot_out, int r, int first, int all,
-                                               int kb, int ke, float (*sm_o)[16][D + 4],
+                                               int kb, int ke, char (*bufE)[2 * Fp4Tile<D>::BYTES],
+                                               char (*bufO)[2 * Fp4Tile<D>::BYTES],
                                                float (*sm_m)[16], float (*sm_l)[16]) {
   using E = Elem<T>;
   using V8 = typename E::vec8;
-  using Chunk = Fp4Chunk<D>;
+  using Tile = Fp4Tile<D>;
   constexpr int QSTEPS = D / 32;
   constexpr int NU = D / 16;
   constexpr int W = 4;
@@ -78,63 +88,72 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
     }
   }
 
-  // Lane offsets in a tile's bytes.  A piece past the row's dv columns is
-  // fetched from the row's first instead: it meets zeros of Q, or lands in
-  // columns of O that are not stored.
-  const Fp4Region reg{dv, p.kv.block_size};
-  int koff[Chunk::KS], ksoff[Chunk::KS], voff[Chunk::VP];
-#pragma unroll
-  for (int i = 0; i < Chunk::KS; ++i) {
-    const int d0 = D / 4 * g4 + 32 * i;
-    const bool in = d0 < dv;
-    koff[i] = c16 * (dv / 2) + (in ? d0 / 2 : 0);
-    ksoff[i] = ((c16 >> 2) * (dv / 32) + (in ? d0 / 32 : 0)) * 4 + (c16 & 3);
-  }
-#pragma unroll
-  for (int i = 0; i < Chunk::VP; ++i) {
-    const int oct = NU * c16 / 8 + i;
-    voff[i] = (g4 * (dv / 8) + (oct < dv / 8 ? oct : 0)) * 16;
-  }
-  const int vgrp = NU * c16 / 32;
-  const int vsoff = (g4 * (dv / 32) + (vgrp < dv / 32 ? vgrp : 0)) * 4;
   const int bs = p.kv.block_size, bs_shift = 31 - __builtin_clz(bs);
-  const auto* bt = (const __attribute__((address_space(4))) int32_t*)(
-      p.kv.block_table + static_cast<uint64_t>(r) * p.bt_stride * 4);
+  const auto* bt = global_ptr(reinterpret_cast<const int32_t*>(
+      p.kv.block_table + static_cast<uint64_t>(r) * p.bt_stride * 4));
   const uint32_t id_max = static_cast<uint32_t>(p.kv.num_blocks) - 1;
   const char* head = reinterpret_cast<const char*>(p.kv.k_addr) + kvh * p.kv.stride_head;
 
-  auto load = [&](int x0, Chunk& ch) __attribute__((always_inline)) {
+  // Lane offsets in a region.  A piece past the row's dv columns is fetched from
+  // the row's first instead: it meets zeros of Q, or lands in columns of O that
+  // are not stored.
+  const int vb = bs * (dv / 2), ng = dv / 32;
+  int koff[Tile::P], voff[Tile::P];  // (D 64: one load, K in the lower lanes, V in the upper)
+#pragma unroll
+  for (int i = 0; i < Tile::P; ++i) {
+    const int l = lane & 31;
+    const int key = D == 64 ? l >> 1 : c16, d0 = D == 64 ? 32 * (l & 1) : D / 4 * g4 + 32 * i;
+    const int quad = D == 64 ? l >> 3 : g4, oct = D == 64 ? l & 7 : NU * c16 / 8 + i;
+    koff[i] = key * (dv / 2) + (d0 < dv ? d0 / 2 : 0);
+    voff[i] = vb + (quad * (dv / 8) + (oct < dv / 8 ? oct : 0)) * 16;
+    if (D == 64 && lane >= 32) koff[i] = voff[i];
+  }
+  const int si = lane & (Tile::SW - 1), sv = lane / Tile::SW & 1;
+  const int soff = bs * dv + sv * bs * ng + (si < 4 * ng ? si : 0) * 4;
+  const int region = static_cast<int>(Fp4Region{dv, bs}.bytes());
+
+  // Block ids of a chunk's tiles, in the two halves of the wave.
+  auto fetch_ids = [&](int x0) __attribute__((always_inline)) {
+    const int x = x0 + (lane & 32) / 2;
+    return static_cast<uint32_t>(bt[(x < all ? x : all - 1) >> bs_shift]);
+  };
+  // (buffer loads: behind global loads into LDS the compiler waits for every load
+  // before it uses one's result)
+  auto issue = [&](int x0, uint32_t ids, HCP_LDS_PTR(char) dst) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int x = x0 + 16 * t;
-      uint32_t id = bt[(x < all ? x : all - 1) >> bs_shift];
+      uint32_t id = __builtin_amdgcn_readlane(ids, 32 * t);
       id = id < id_max ? id : id_max;  // past the cache: its last block
-      const int off = x & (bs - 1);
-      const char* kc = head + id * p.kv.stride_block + off * (dv / 2);
-      const char* sc = head + id * p.kv.stride_block + bs * dv + off * (dv / 32);
-      const char* vc = kc + bs * (dv / 2);
+      const int off = (x0 + 16 * t) & (bs - 1);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(head + id * p.kv.stride_block), 0, region, 0x00020000);
+      auto load = [&](int at, int o, int so) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, reinterpret_cast<HCP_LDS_PTR(void)>(dst + t * Tile::BYTES + at), 16, o, so, 0, 2);
+      };
+      const int row = off * (dv / 2);
 #pragma unroll
-      for (int i = 0; i < Chunk::KS; ++i) {
-        if constexpr (D == 64) {
-          const u32x2 a = ldnt<u32x2>(kc + koff[0]);
-          ch.k[t][0] = a[0];
-          ch.k[t][1] = a[1];
-        } else {
-          const u32x4 a = ldnt<u32x4>(kc + koff[i]);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) ch.k[t][4 * i + w] = a[w];
-        }
-        ch.ks[t][i] = ldnt<uint8_t>(sc + ksoff[i]);
+      for (int i = 0; i < Tile::P; ++i) {
+        load(i * 1024, koff[i], row);
+        if constexpr (D > 64) load((Tile::P + i) * 1024, voff[i], row);
       }
-#pragma unroll
-      for (int i = 0; i < Chunk::VP; ++i) {
-        const u32x4 a = ldnt<u32x4>(vc + voff[i]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) ch.v[t][i][w] = a[w];
-      }
-      ch.vs[t] = ldnt<uint32_t>(sc + bs * (dv / 32) + vsoff);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, reinterpret_cast<HCP_LDS_PTR(void)>(dst + t * Tile::BYTES + Tile::SC), 4, soff,
+          off * ng, 0, 2);
     }
   };
+  // where in a tile a lane finds its K codes, K scale (a byte), V codes and V scales
+  // (a dword: four keys)
+  const int kc_at = D == 64 ? c16 * 32 + g4 * 8 : lane * 16;
+  const int vc_at = D == 64 ? 512 + g4 * 128 + (c16 >> 1) * 16 : Tile::P * 1024 + lane * 16;
+  int ks_at[Tile::P];
+#pragma unroll
+  for (int i = 0; i < Tile::P; ++i) {
+    const int g = D / 4 * g4 / 32 + i;
+    ks_at[i] = Tile::SC + ((c16 >> 2) * ng + (g < ng ? g : 0)) * 4 + (c16 & 3);
+  }
+  const int vgrp = NU * c16 / 32;
+  const int vs_at = Tile::SC + Tile::SW * 4 + (g4 * ng + (vgrp < ng ? vgrp : 0)) * 4;
 
   const float c = p.d.scale_log2;
   float m_run = -INFINITY, l_run = 0.f;
@@ -142,15 +161,30 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
 #pragma unroll
   for (int u = 0; u < NU; ++u) oacc[u] = f32x4{};
 
-  auto compute = [&](int x0, Chunk& ch) __attribute__((always_inline)) {
+  auto compute = [&](int x0, const HCP_LDS_PTR(char) src) __attribute__((always_inline)) {
     f32x4 s[2] = {f32x4{}, f32x4{}};
+    uint32_t vsw[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      const HCP_LDS_PTR(char) const tile = src + t * Tile::BYTES;
 #pragma unroll
-      for (int q = 0; q < QSTEPS; ++q)
-        s[t] = E::mfma16(as_vec8<V8>(fp4_values<T>(
-                             ch.k[t][q], __uint_as_float(ch.ks[t][Chunk::KS == 1 ? 0 : q / 4] << 23))),
-                         qf[q], s[t]);
+      for (int i = 0; i < Tile::P; ++i) {
+        const float ks =
+            __uint_as_float(static_cast<uint32_t>(lds_at<uint8_t>(tile + ks_at[i])) << 23);
+        if constexpr (D == 64) {
+          const u32x2 w = lds_at<u32x2>(tile + kc_at);
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            s[t] = E::mfma16(as_vec8<V8>(fp4_values<T>(w[q], ks)), qf[q], s[t]);
+        } else {
+          const u32x4 w = lds_at<u32x4>(tile + i * 1024 + kc_at);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            s[t] = E::mfma16(as_vec8<V8>(fp4_values<T>(w[q], ks)), qf[4 * i + q], s[t]);
+        }
+      }
+      vsw[t] = lds_at<uint32_t>(tile + vs_at);
+    }
     if (x0 < first || x0 + 32 > ke) {
       // keys outside the split: no weight, and a finite value whatever their
       // bytes say (0 times a NaN would stay one)
@@ -161,7 +195,7 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
           const int key = x0 + 16 * t + 4 * g4 + i;
           if (key < first || key >= ke) {
             s[t][i] = -INFINITY;
-            ch.vs[t] &= ~(0xffu << (8 * i));
+            vsw[t] &= ~(0xffu << (8 * i));
           }
         }
     }
@@ -199,13 +233,19 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
     float vs[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      vs[j] = __uint_as_float(((ch.vs[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
+      vs[j] = __uint_as_float(((vsw[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
+    u32x4 vw[2][Tile::P];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < Tile::P; ++i)
+        vw[t][i] = lds_at<u32x4>(src + t * Tile::BYTES + i * 1024 + vc_at);
     // columns 2 u and 2 u + 1 of 8 keys -> two operands
     auto pv = [&](auto sel, auto piece, int u) __attribute__((always_inline)) {
       uint32_t x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        uint32_t w = ch.v[j >> 2][decltype(piece)::value][j & 3];
+        uint32_t w = vw[j >> 2][decltype(piece)::value][j & 3];
         if constexpr (D == 64) w >>= 16 * (c16 & 1);
         x[j] = fp4_pair<T, decltype(sel)::value>(w, vs[j]);
       }
@@ -238,30 +278,47 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
     }
   };
 
-  // the wave's chunks: kb + 32 (wave, wave + W, ..)
+  // The wave's chunks, kb + 32 (wave, wave + W, ..): the block ids of the one after
+  // the next are fetched, the next one's bytes loaded, and when only those are
+  // outstanding the current one has landed.  (Loads without a branch around
+  // them, so that the compiler's waits are exact too: past the last chunk they
+  // repeat it.)
+  constexpr int ST = 32 * W;
   int x = kb + 32 * wave;
   if (x < ke) {
-    Chunk a, b;
-    load(x, a);
+    HCP_LDS_PTR(char) const be = (HCP_LDS_PTR(char))(bufE[wave]);
+    HCP_LDS_PTR(char) const bo = (HCP_LDS_PTR(char))(bufO[wave]);
+    const int last = x + (ke - 1 - x) / ST * ST;
+    auto upto = [&](int y) __attribute__((always_inline)) { return y < last ? y : last; };
+    uint32_t ia = fetch_ids(x), ib = fetch_ids(upto(x + ST));
+    __builtin_amdgcn_sched_barrier(0);
+    issue(x, ia, be);
     while (true) {
-      if (x + 32 * W >= ke) {
-        compute(x, a);
-        break;
-      }
-      load(x + 32 * W, b);
-      compute(x, a);
-      x += 32 * W;
-      if (x + 32 * W >= ke) {
-        compute(x, b);
-        break;
-      }
-      load(x + 32 * W, a);
-      compute(x, b);
-      x += 32 * W;
+      ia = fetch_ids(upto(x + 2 * ST));
+      // (ids before the loads: waiting for them must not wait for these)
+      __builtin_amdgcn_sched_barrier(0);
+      issue(upto(x + ST), ib, bo);
+      wait_vmcnt<2 * Tile::NI + 1>();
+      compute(x, be);
+      x += ST;
+      if (x > last) break;
+      ib = fetch_ids(upto(x + 2 * ST));
+      __builtin_amdgcn_sched_barrier(0);
+      issue(upto(x + ST), ia, be);
+      wait_vmcnt<2 * Tile::NI + 1>();
+      compute(x, bo);
+      x += ST;
+      if (x > last) break;
     }
   }
 
-  // ---- combine the W waves ----
+  // ---- combine the W waves, in the chunk buffers (two waves to each) ----
+  wait_vmcnt<0>();  // the last loads still write there
+  __syncthreads();
+  float (*const so_e)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(&bufE[0][0]);
+  float (*const so_o)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(&bufO[0][0]);
+  static_assert(sizeof(float) * 2 * 16 * (D + 4) <= W * 2 * Tile::BYTES, "combine staging");
+  float (*const mine)[D + 4] = wave < 2 ? so_e[wave] : so_o[wave - 2];
   float l_tot = l_run + __shfl_xor(l_run, 16);
   l_tot += __shfl_xor(l_tot, 32);
   if (g4 == 0) {
@@ -272,7 +329,7 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int u = 0; u < NU; u += 4)
-      *reinterpret_cast<f32x4*>(&sm_o[wave][c16][NU * (4 * g4 + i) + u]) =
+      *reinterpret_cast<f32x4*>(&mine[c16][NU * (4 * g4 + i) + u]) =
           f32x4{oacc[u][i], oacc[u + 1][i], oacc[u + 2][i], oacc[u + 3][i]};
   __syncthreads();
   for (int idx = tid; idx < G * D; idx += 64 * W) {
@@ -286,7 +343,7 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
     for (int w = 0; w < W; ++w) {
       const float sc = fast_exp2(sm_m[w][h] - Mu);
       L += sm_l[w][h] * sc;
-      O += sm_o[w][h][d] * sc;
+      O += (w < 2 ? so_e[w] : so_o[w - 2])[h][d] * sc;
     }
     const int64_t slot = static_cast<int64_t>(slot_out) * p.d.num_heads + h0 + h;
     const bool some = KEEP_NAN ? L != 0.f : L > 0.f;
@@ -295,13 +352,15 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   }
 }
 
-// The batch is cut as for decode_paged_kernel; a chunk costs a quarter of the
-// bytes, so a split's start counts for more of them, and a share is at least one
-// chunk for each wave.
+// The batch is cut as for decode_paged_kernel, a share at least one chunk for each
+// wave.  At 64 columns four workgroups fit a CU (64 x 16k-32k keys of 14 / 2 x 64:
+// 55 -> 51 us), but the second two pay only from two chunks for each wave on (16 x
+// 1k-8k: 12.3 us, 15.0 with all of them).
 template <int D, typename T, bool KEEP_NAN>
-__global__ __launch_bounds__(256, 2) void decode_fp4_kernel(PagedDecParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void decode_fp4_kernel(PagedDecParams p) {
   constexpr int W = 4;
-  __shared__ float sm_o[W][16][D + 4];
+  __shared__ __attribute__((aligned(1024))) char bufE[W][2 * Fp4Tile<D>::BYTES];
+  __shared__ __attribute__((aligned(1024))) char bufO[W][2 * Fp4Tile<D>::BYTES];
   __shared__ float sm_m[W][16], sm_l[W][16];
   __shared__ int sm_len[kDecMaxSeqs], sm_all[kDecMaxSeqs];  // keys seen, in the cache (-1: not run)
   __shared__ int sm_w[2][W];
@@ -314,9 +373,10 @@ __global__ __launch_bounds__(256, 2) void decode_fp4_kernel(PagedDecParams p) {
   const int chunk = static_cast<int>(item % p.d.head_chunks);
   const int wg = static_cast<int>(item / p.d.head_chunks);
   auto first_chunk = [](int all, int len) { return (all - len) & ~31; };
-  paged_shares<64 * W, 16, 4, true>(p, wg, sm_len, sm_all, sm_w, sm_cut, [&](int all, int len) {
-    return len > 0 ? (all - first_chunk(all, len) + 31) >> 5 : 0;
-  });
+  paged_shares<64 * W, 8, 4, D == 64 ? 2 : 1, true>(
+      p, wg, sm_len, sm_all, sm_w, sm_cut, [&](int all, int len) {
+        return len > 0 ? (all - first_chunk(all, len) + 31) >> 5 : 0;
+      });
   const int r0 = __builtin_amdgcn_readfirstlane(sm_cut[0]);
   const int o0 = __builtin_amdgcn_readfirstlane(sm_cut[1]);
   const int r1 = r0 < 0 ? -2 : __builtin_amdgcn_readfirstlane(sm_cut[2]);  // -1, -2: no share
@@ -334,7 +394,7 @@ __global__ __launch_bounds__(256, 2) void decode_fp4_kernel(PagedDecParams p) {
     }
     const int end = base + 32 * e;
     fp4_split_body<D, T, KEEP_NAN>(p, kvh, chunk, wg + r, r, all - len, all, base + 32 * b,
-                                   end < all ? end : all, sm_o, sm_m, sm_l);
+                                   end < all ? end : all, bufE, bufO, sm_m, sm_l);
     __syncthreads();  // this split has been combined out of the buffers
   }
   // the reduce goes by the slots alone: a sequence without keys says so

@@ -19,21 +19,35 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return x;
 }
 
-// Length r as the caller gives it (or, of `starts`, first key).
-__device__ __forceinline__ int64_t paged_len(const void* lens, bool wide, int r) {
-  return wide ? global_ptr(reinterpret_cast<const int64_t*>(lens))[r]
-              : global_ptr(reinterpret_cast<const int32_t*>(lens))[r];
+// Lengths (or first keys) r, r + 1, .. as the caller gives them, those past n the
+// last one's: all loads on their way at once, not one after the other.
+template <int N>
+__device__ __forceinline__ void paged_lens(const void* lens, bool wide, int r, int n,
+                                           int64_t (&x)[N]) {
+  if (wide) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      x[j] = global_ptr(reinterpret_cast<const int64_t*>(lens))[r + j < n ? r + j : n - 1];
+  } else {
+    int32_t y[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      y[j] = global_ptr(reinterpret_cast<const int32_t*>(lens))[r + j < n ? r + j : n - 1];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = y[j];
+  }
 }
 
 // Cuts the keys of all sequences, laid end to end in chunks of 32, into equal
 // shares, one for each of at most p.d.num_wgs workgroups, each of at least LEAST
-// chunks; every sequence counts for START chunks more, what its split costs to
-// start.  count(all, len): the chunks of a sequence with `all` keys in the cache,
-// the last `len` of them seen.  A workgroup of NT threads gets its share in
-// sm_cut: first sequence (-1: none) and first chunk of it, last sequence and the
-// end in its chunks; sm_len / sm_all [kDecMaxSeqs] get the keys of every sequence
-// (sm_all -1: HCP_LEN_NOT_RUN).  STARTS: p.starts counts.  Ends with a barrier.
-template <int NT, int START, int LEAST, bool STARTS, typename Count>
+// chunks (twice that past a LATE-th of the workgroups); every sequence counts for
+// START chunks more, what its split costs to start.  count(all, len): the chunks of
+// a sequence with `all` keys in the cache, the last `len` of them seen.  A
+// workgroup of NT threads gets its share in sm_cut: first sequence (-1: none) and
+// first chunk of it, last sequence and the end in its chunks; sm_len / sm_all
+// [kDecMaxSeqs] get the keys of every sequence (sm_all -1: HCP_LEN_NOT_RUN).
+// STARTS: p.starts counts.  Ends with a barrier.
+template <int NT, int START, int LEAST, int LATE, bool STARTS, typename Count>
 __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, int* sm_len,
                                              int* sm_all, int (*sm_w)[NT / 64], int* sm_cut,
                                              Count count) {
@@ -43,16 +57,21 @@ __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, i
   // ---- prefix sums over the sequences: chunks, sequences with keys ----
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c[EPT], cs = 0, zs = 0;
+  int64_t lens[EPT], from[EPT];
+  paged_lens(p_.lens, p_.lens_wide, tid * EPT, n, lens);
+  if constexpr (STARTS) {
+    if (p_.starts != nullptr) paged_lens(p_.starts, p_.lens_wide, tid * EPT, n, from);
+  }
 #pragma unroll
   for (int j = 0; j < EPT; ++j) {
     const int r = tid * EPT + j;
-    const int64_t given = r < n ? paged_len(p_.lens, p_.lens_wide, r) : 0;
+    const int64_t given = r < n ? lens[j] : 0;
     const int all =  // keys that the sequence's query sees; max_len < 2^31
         static_cast<int>(given < 0 ? 0 : given < p_.max_len ? given : p_.max_len);
     int seen = all;
     if constexpr (STARTS) {
       if (p_.starts != nullptr && r < n) {
-        const int64_t s = paged_len(p_.starts, p_.lens_wide, r);
+        const int64_t s = from[j];
         seen = s <= 0 ? all : s < all ? all - static_cast<int>(s) : 0;
       }
     }
@@ -84,8 +103,12 @@ __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, i
     some += sm_w[1][w];
   }
   // ---- this workgroup's share ----
-  const unsigned most = static_cast<unsigned>(p_.d.num_wgs), half = (total + LEAST - 1) / LEAST;
-  const unsigned wgs = most < half ? most : half;
+  unsigned wgs = static_cast<unsigned>(p_.d.num_wgs);
+  {
+    const unsigned least = (total + LEAST - 1) / LEAST, twice = total / (2 * LEAST);
+    const unsigned few = wgs / LATE < least ? wgs / LATE : least, many = few > twice ? few : twice;
+    wgs = wgs < many ? wgs : many;
+  }
   if (static_cast<unsigned>(wg) < wgs) {
     const unsigned share = total / wgs;
     const unsigned start = share < START ? share : START;
