@@ -74,7 +74,8 @@ def check_slots(slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> torch.Ten
     """``slot_mapping`` as the kernels read it."""
     if slot_mapping.dtype not in _INDEX_CODES or slot_mapping.dim() != 1:
         raise ValueError("slot_mapping must be int32 or int64, of one dimension")
-    if not kv_cache.is_cuda or slot_mapping.device != kv_cache.device:
+    index = kv_cache.get_device()
+    if index < 0 or slot_mapping.get_device() != index:
         raise ValueError("slot_mapping must be on the cache's GPU")
     return slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
 
@@ -89,19 +90,20 @@ def _write_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
         raise ValueError(f"{n} slots for {shape[0]} key rows")
     if shape[1] != hkv or shape[2] != d:
         raise ValueError("key/value heads or head_dim do not match the cache")
-    if dt not in (torch.float16, torch.bfloat16) or value.dtype != dt:
+    if (dt != torch.bfloat16 and dt != torch.float16) or value.dtype != dt:
         raise ValueError("key/value must both be float16 or bfloat16")
-    ks, vs = key.stride(), value.stride()
-    if ks[2] != 1 or vs[2] != 1:
+    (k_tok, k_head, k_col), (v_tok, v_head, v_col) = key.stride(), value.stride()
+    if k_col != 1 or v_col != 1:
         raise ValueError("key/value head_dim must be contiguous")
     slots = check_slots(slot_mapping, kv_cache)
-    if key.device != dev or value.device != dev:
+    index = dev.index
+    if key.get_device() != index or value.get_device() != index:
         raise ValueError("key/value must be on the cache's GPU")
     if n == 0:
         return
     with _lib.on_device(dev):
         rc = _lib.lib().hcp_fp4_write(
-            key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], slots.data_ptr(),
+            key.data_ptr(), k_tok, k_head, value.data_ptr(), v_tok, v_head, slots.data_ptr(),
             _INDEX_CODES[slots.dtype], n, hkv, ctypes.addressof(desc), _lib.dtype_code(dt),
             _lib.stream_ptr(dev))
     _lib.check(rc, "hcp_fp4_write")
@@ -112,7 +114,7 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     """K and V ``[n, Hkv, D]`` that a 4-bit cache stands for at ``slot_mapping``,
     in the 16-bit ``dtype`` they were written in (exactly: a code's value has two
     significant bits).  A slot that is negative or past the cache reads as zeros."""
-    if dtype not in (torch.float16, torch.bfloat16):
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise ValueError("dtype must be float16 or bfloat16")
     desc, hkv, d = fp4_desc(kv_cache)
     slots, dev = check_slots(slot_mapping, kv_cache), kv_cache.device

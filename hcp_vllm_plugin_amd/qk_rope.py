@@ -24,17 +24,28 @@ __all__ = ["qk_norm_rope"]
 _INDEX = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
 
+_TYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
 def _rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype,
-          device: torch.device) -> tuple[int, int]:
-    """Token and head stride of ``t``, which must have the kernel's rows."""
+          index: int) -> tuple[int, int, int]:
+    """Address, token and head stride of ``t``, which must have the kernel's rows."""
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, not {shape}")
-    if t.dtype != dtype or t.device != device:
+    if t.dtype != dtype or t.get_device() != index:
         raise ValueError(f"{name} must be of query's dtype and device")
-    tok, head, col = t.stride()
-    if col != 1 or (t.data_ptr() | 2 * tok | 2 * head) & 15:
+    (tok, head, col), at = t.stride(), t.data_ptr()
+    if col != 1 or (at | 2 * tok | 2 * head) & 15:
         raise ValueError(f"{name}: 16-byte aligned rows with contiguous head_dim")
-    return tok, head
+    return at, tok, head
+
+
+def _weight(t: torch.Tensor, d: int, dtype: torch.dtype, index: int) -> tuple[int, torch.dtype]:
+    at, wd = t.data_ptr(), t.dtype
+    if t.shape != (d,) or not t.is_contiguous() or at & 15 or t.get_device() != index or \
+            (wd != dtype and wd != torch.float32):
+        raise ValueError("weights must be [head_dim], float32 or of query's dtype, on its device")
+    return at, wd
 
 
 def qk_norm_rope(
@@ -69,88 +80,80 @@ def qk_norm_rope(
     into the cache at ``slot_mapping[t]`` (tokens past its length and negative
     slots are not written); the key then comes back only where ``key_out`` asks
     for it.  ``query_out`` / ``key_out`` may be query and key themselves."""
-    dt, dev = query.dtype, query.device
-    if dt not in (torch.float16, torch.bfloat16) or dev.type != "cuda" or query.dim() != 3 or \
-            key.dim() != 3:
+    dt, index = query.dtype, query.get_device()
+    code = _TYPES.get(dt)
+    if code is None or index < 0 or query.dim() != 3 or key.dim() != 3:
         raise ValueError("query and key must be float16/bfloat16 [T, heads, D] on the GPU")
     t, h, d = query.shape
     hkv = key.shape[1]
-    a = _lib.QkRopeArgs()
-    a.q_stride_tok, a.q_stride_head = _rows("query", query, (t, h, d), dt, dev)
-    a.k_stride_tok, a.k_stride_head = _rows("key", key, (t, hkv, d), dt, dev)
-    if positions.dtype not in _INDEX or positions.shape != (t,) or positions.device != dev or \
+    kv_shape = (t, hkv, d)
+    q, q_tok, q_head = _rows("query", query, (t, h, d), dt, index)
+    k, k_tok, k_head = _rows("key", key, kv_shape, dt, index)
+    pos_code = _INDEX.get(positions.dtype)
+    if pos_code is None or positions.shape != (t,) or positions.get_device() != index or \
             not positions.is_contiguous():
         raise ValueError("positions must be contiguous int32/int64 [T] on query's device")
     tab = cos_sin_cache
-    if tab.dim() != 2 or tab.device != dev or tab.dtype not in (torch.float32, dt):
+    wide_table = tab.dtype == torch.float32
+    if tab.dim() != 2 or tab.get_device() != index or not (wide_table or tab.dtype == dt):
         raise ValueError("cos_sin_cache must be [max_positions, rot], float32 or query's dtype, on "
                          "query's device")
-    most, rot = tab.shape
+    (most, rot), (tab_row, col), tab_at = tab.shape, tab.stride(), tab.data_ptr()
     if rot:
-        row, col = tab.stride()
         if rot % 16 or rot > d or most == 0:
             raise ValueError("rot must be a multiple of 16 up to head_dim, and the table not empty")
-        if col != 1 or tab.data_ptr() % 16 or row % 8:
+        if col != 1 or tab_at & 15 or tab_row & 7:
             raise ValueError("cos_sin_cache: 16-byte aligned rows")
-        a.cos_sin, a.table_stride, a.max_positions = tab.data_ptr(), row, most
-    wide = None
-    for w in (q_weight, k_weight):
-        if w is None:
-            continue
-        if w.shape != (d,) or w.stride(0) != 1 or w.device != dev or w.data_ptr() % 16 or \
-                w.dtype not in (torch.float32, dt) or w.dtype != (wide or w.dtype):
-            raise ValueError("weights must be [head_dim] and of one dtype, float32 or query's, on "
-                             "query's device")
-        wide = w.dtype
-    a.slot_dtype = _lib.DTYPE_I64
+    else:
+        tab_at = tab_row = 0
+    wq = wk = 0
+    w_type = dt
+    if q_weight is not None:
+        wq, w_type = _weight(q_weight, d, dt, index)
+    if k_weight is not None:
+        wk, wt = _weight(k_weight, d, dt, index)
+        if wq and wt != w_type:
+            raise ValueError("q_weight and k_weight must be of one dtype")
+        w_type = wt
+    v = v_tok = v_head = slots_at = num_slots = cache = fp4 = kind = 0
+    slot_code = pos_code
     if kv_cache is None:
         if value is not None or slot_mapping is not None:
             raise ValueError("value and slot_mapping go with a kv_cache")
         if key_out is None:
-            key_out = torch.empty((t, hkv, d), dtype=dt, device=dev)
+            key_out = torch.empty(kv_shape, dtype=dt, device=query.device)
     else:
         if value is None or slot_mapping is None:
             raise ValueError("a cache write needs value and slot_mapping")
-        a.v_stride_tok, a.v_stride_head = _rows("value", value, (t, hkv, d), dt, dev)
-        a.v = value.data_ptr()
+        v, v_tok, v_head = _rows("value", value, kv_shape, dt, index)
         slots = check_slots(slot_mapping, kv_cache)
-        if kv_cache.device != dev:
+        if kv_cache.get_device() != index:
             raise ValueError("kv_cache must be on query's device")
-        if slots.shape[0] > t:
-            raise ValueError(f"{slots.shape[0]} slots for {t} tokens")
-        a.slot_mapping, a.num_slots, a.slot_dtype = slots.data_ptr(), slots.shape[0], \
-            _INDEX[slots.dtype]
+        slots_at, num_slots, slot_code = slots.data_ptr(), slots.shape[0], _INDEX[slots.dtype]
+        if num_slots > t:
+            raise ValueError(f"{num_slots} slots for {t} tokens")
         if kv_cache.dtype == torch.uint8:
             desc, c_hkv, c_d = fp4_desc(kv_cache)
-            a.cache_kind, a.fp4 = 2, ctypes.addressof(desc)
+            kind, fp4 = 2, ctypes.addressof(desc)
         else:
             if kv_cache.dtype != dt:
                 raise ValueError("kv_cache must be of query's dtype, or a 4-bit cache (uint8)")
-            desc, a.cache, c_hkv, c_d = _cache_desc(kv_cache)
-            a.cache_kind = 1
+            desc, cache, c_hkv, c_d = _cache_desc(kv_cache)
+            kind = 1
         if c_hkv != hkv or c_d != d:
             raise ValueError("key heads or head_dim do not match the cache")
     if query_out is None:
-        query_out = torch.empty((t, h, d), dtype=dt, device=dev)
-        a.qo_stride_tok, a.qo_stride_head = h * d, d
+        query_out = torch.empty((t, h, d), dtype=dt, device=query.device)
+        qo, qo_tok, qo_head = query_out.data_ptr(), h * d, d
     else:
-        a.qo_stride_tok, a.qo_stride_head = _rows("query_out", query_out, (t, h, d), dt, dev)
+        qo, qo_tok, qo_head = _rows("query_out", query_out, (t, h, d), dt, index)
+    ko = ko_tok = ko_head = 0
     if key_out is not None:
-        a.ko_stride_tok, a.ko_stride_head = _rows("key_out", key_out, (t, hkv, d), dt, dev)
-        a.k_out = key_out.data_ptr()
-    a.q, a.k, a.q_out = query.data_ptr(), key.data_ptr(), query_out.data_ptr()
-    if q_weight is not None:
-        a.q_weight = q_weight.data_ptr()
-    if k_weight is not None:
-        a.k_weight = k_weight.data_ptr()
-    a.positions, a.pos_dtype = positions.data_ptr(), _INDEX[positions.dtype]
-    a.num_tokens, a.eps, a.interleaved = t, eps, bool(interleaved)
-    a.num_heads, a.num_kv_heads, a.head_dim, a.rot = h, hkv, d, rot
-    a.dtype = a.weight_dtype = _lib.dtype_code(dt)
-    if wide == torch.float32:
-        a.weight_dtype = _lib.DTYPE_F32
-    a.table_dtype = _lib.DTYPE_F32 if tab.dtype == torch.float32 else a.dtype
-    with _lib.on_device(dev):
-        rc = _lib.lib().hcp_qk_norm_rope(ctypes.addressof(a), _lib.stream_ptr(dev))
-    _lib.check(rc, "hcp_qk_norm_rope")
+        ko, ko_tok, ko_head = _rows("key_out", key_out, kv_shape, dt, index)
+    _lib.launch(_lib.lib().hcp_qk_norm_rope, _lib.pack_qk_rope(
+        q, q_tok, q_head, k, k_tok, k_head, v, v_tok, v_head, qo, qo_tok, qo_head, ko, ko_tok,
+        ko_head, wq, wk, positions.data_ptr(), tab_at, tab_row, most, slots_at, num_slots, cache,
+        fp4, t, eps, h, hkv, d, rot, code, code if w_type == dt else _lib.DTYPE_F32,
+        _lib.DTYPE_F32 if wide_table else code, pos_code, slot_code, bool(interleaved), kind, 0),
+        index, "hcp_qk_norm_rope")
     return query_out, key_out

@@ -10,7 +10,6 @@ launch and without waiting for the device.
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
@@ -46,10 +45,9 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
 
     ``positions`` and ``slot_mapping`` have ``num_tokens`` rows: the new tokens,
     then (padding) position 0 and slot -1.  Lengths below 0 count as 0."""
-    n = ctx_lens.shape[0] if ctx_lens.dim() == 1 else -1
-    dev = block_table.device
-    if ctx_lens.dtype not in _INDEX or new_lens.dtype not in _INDEX or ctx_lens.shape != (n,) or \
-            new_lens.shape != (n,):
+    index, ints_of = block_table.get_device(), _INDEX.get
+    ctx_code, new_code, (n, *more) = ints_of(ctx_lens.dtype), ints_of(new_lens.dtype), ctx_lens.shape
+    if more or ctx_code is None or new_code is None or new_lens.shape != (n,):
         raise ValueError("ctx_lens and new_lens must be int32/int64 of one dimension and length")
     if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 of two dimensions")
@@ -58,30 +56,21 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
         raise ValueError("block_table must have contiguous rows, one for each request")
     if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be contiguous int32 of one dimension")
-    if dev.type != "cuda" or ctx_lens.device != dev or new_lens.device != dev or \
-            free_blocks.device != dev:
+    if index < 0 or ctx_lens.get_device() != index or new_lens.get_device() != index or \
+            free_blocks.get_device() != index:
         raise ValueError("all tensors must be on one GPU")
     if block_size <= 0 or block_size & (block_size - 1):
         raise ValueError("block_size must be a power of two")
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
-    ints = torch.empty(2 * n + 2, dtype=torch.int32, device=dev)
-    wide = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
-    a = _lib.StepTablesArgs()
-    a.ctx_lens, a.ctx_stride, a.ctx_dtype = ctx_lens.data_ptr(), ctx_lens.stride(0), \
-        _INDEX[ctx_lens.dtype]
-    a.new_lens, a.new_stride, a.new_dtype = new_lens.data_ptr(), new_lens.stride(0), \
-        _INDEX[new_lens.dtype]
-    a.block_table, a.table_stride, a.table_width = block_table.data_ptr(), row, width
-    a.free_blocks, a.num_free = free_blocks.data_ptr(), free_blocks.shape[0]
-    base = ints.data_ptr()
-    a.query_start_loc, a.seq_lens, a.blocks_used = base, base + 4 * (n + 1), base + 4 * (2 * n + 1)
-    a.positions = base = wide.data_ptr()
-    a.slot_mapping = base + 8 * num_tokens
-    a.num_tokens, a.num_seqs, a.block_size = num_tokens, n, block_size
-    with _lib.on_device(dev):
-        rc = _lib.lib().hcp_step_tables(ctypes.addressof(a), _lib.stream_ptr(dev))
-    _lib.check(rc, "hcp_step_tables")
+    ints = torch.empty(2 * n + 2, dtype=torch.int32, device=block_table.device)
+    wide = torch.empty((2, num_tokens), dtype=torch.int64, device=block_table.device)
+    at, wide_at = ints.data_ptr(), wide.data_ptr()
+    _lib.launch(_lib.lib().hcp_step_tables, _lib.pack_step_tables(
+        ctx_lens.data_ptr(), new_lens.data_ptr(), ctx_lens.stride(0), new_lens.stride(0),
+        block_table.data_ptr(), row, width, free_blocks.data_ptr(), free_blocks.shape[0],
+        num_tokens, at, at + 4 * (n + 1), at + 4 * (2 * n + 1), wide_at, wide_at + 8 * num_tokens,
+        ctx_code, new_code, n, block_size), index, "hcp_step_tables")
     starts, lens, used = ints.split_with_sizes((n + 1, n, 1))
     positions, slots = wide.unbind(0)
     return StepTables(starts, lens, positions, slots, used)

@@ -952,7 +952,8 @@ def decode_fp4(
     read on the device when the call executes.  A query that sees no key gets
     out 0 and LSE -inf; a length past its table row counts as the row's keys.
     ``keep_nan``: as ``DecodeBatch.run``.  Returns out (and lse float32 ``[H, S]``)."""
-    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16) or q.stride(2) != 1:
+    dt, index = q.dtype, q.get_device()
+    if q.dim() != 3 or (dt != torch.bfloat16 and dt != torch.float16) or q.stride(2) != 1:
         raise ValueError("q must be float16/bfloat16 [S, H, D] with contiguous head_dim")
     desc, hkv, dim = fp4_desc(kv_cache)
     s, h, d = q.shape
@@ -960,55 +961,48 @@ def decode_fp4(
         raise ValueError("kv_cache must be a 4-bit cache of q's head_dim, its heads dividing q's")
     if window is not None and window <= 0:
         raise ValueError("window must be a positive number of keys")
-    dev = q.device
-    for name, t in (("seq_lens", seq_lens), ("starts", starts)):
-        if t is not None and (t.dtype not in _INDEX_CODES or t.shape != (s,) or t.device != dev
-                              or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous int32/int64 [S] on q's GPU")
-    if starts is not None and starts.dtype != seq_lens.dtype:
-        raise ValueError("starts must be of seq_lens' dtype")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < s or \
-            block_table.stride(1) != 1 or block_table.device != dev:
-        raise ValueError("block_table must be int32 with contiguous rows, one for each query, on q's "
-                         "GPU")
-    if not q.is_cuda or kv_cache.device != dev:
+    lens_code = _INDEX_CODES.get(seq_lens.dtype)
+    if lens_code is None or seq_lens.shape != (s,) or not seq_lens.is_contiguous() or \
+            seq_lens.get_device() != index:
+        raise ValueError("seq_lens must be contiguous int32/int64 [S] on q's GPU")
+    if starts is not None and (starts.dtype != seq_lens.dtype or starts.shape != (s,)
+                               or not starts.is_contiguous() or starts.get_device() != index):
+        raise ValueError("starts must be as seq_lens")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+            block_table.get_device() != index:
+        raise ValueError("block_table must be int32 of two dimensions on q's GPU")
+    (rows, width), (bt_row, bt_col) = block_table.shape, block_table.stride()
+    if rows < s or (width > 1 and bt_col != 1):
+        raise ValueError("block_table must have contiguous rows, one for each query")
+    if index < 0 or kv_cache.get_device() != index:
         raise ValueError("all tensors must be on one GPU")
-    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+    q_at, (q_tok, q_head, _) = q.data_ptr(), q.stride()
+    if (q_at | 2 * q_tok | 2 * q_head) & 15:
         q = q.contiguous()
+        q_at, (q_tok, q_head, _) = q.data_ptr(), q.stride()
     if out is None:
-        out = torch.empty((s, h, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
+        out = torch.empty((s, h, d), dtype=dt, device=q.device)
+    elif out.shape != q.shape or out.dtype != dt or out.stride(2) != 1 or \
+            out.get_device() != index:
         raise ValueError("out must be as q, with contiguous head_dim")
-    lse = torch.empty((h, s), dtype=torch.float32, device=dev) if with_lse else None
-    L = _lib.lib()
-    a = _lib.DecodePagedArgs()
-    a.q_stride_tok, a.q_stride_head, _ = q.stride()
-    a.o_stride_tok, a.o_stride_head, _ = out.stride()
-    a.kv.k_addr, a.kv.stride_head, a.kv.stride_block = desc.addr, desc.stride_head, desc.stride_block
-    a.kv.block_size, a.kv.num_blocks = desc.block_size, desc.num_blocks
-    bt_row = block_table.stride(0)
-    a.block_table_stride, a.block_table_width = bt_row, block_table.shape[1]
-    a.lens_dtype = _INDEX_CODES[seq_lens.dtype]
-    a.num_heads, a.num_kv_heads, a.head_dim = h, hkv, d
-    a.dtype, a.scale, a.keep_nan, a.window = _lib.dtype_code(q.dtype), scale, keep_nan, window or 0
-    a.lse_stride_head = s
-    with _lib.on_device(dev):
-        stream = _lib.stream_ptr(dev)
-        for first in range(0, s, _lib.DECODE_PAGED_MAX_SEQS):
-            n = a.num_seqs = min(s - first, _lib.DECODE_PAGED_MAX_SEQS)
-            a.q = q.data_ptr() + 2 * first * a.q_stride_tok
-            a.out = out.data_ptr() + 2 * first * a.o_stride_tok
-            a.kv.block_table = block_table.data_ptr() + 4 * first * bt_row
-            a.seq_lens = seq_lens.data_ptr() + first * seq_lens.element_size()
-            if starts is not None:
-                a.seq_starts = starts.data_ptr() + first * starts.element_size()
-            if lse is not None:
-                a.lse = lse.data_ptr() + 4 * first
-            # fp32 partials: stream-ordered scratch from torch's caching allocator
-            a.workspace_bytes = L.hcp_decode_fp4_workspace(n, h, hkv, d)
-            ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
-            a.workspace = ws.data_ptr()
-            _lib.check(L.hcp_decode_fp4(ctypes.addressof(a), stream), "hcp_decode_fp4")
+    lse = torch.empty((h, s), dtype=torch.float32, device=q.device) if with_lse else None
+    out_at, (o_tok, o_head, _), lse_at = out.data_ptr(), out.stride(), \
+        lse.data_ptr() if with_lse else 0
+    bt_at, lens_at, starts_at = block_table.data_ptr(), seq_lens.data_ptr(), \
+        0 if starts is None else starts.data_ptr()
+    L, wide = _lib.lib(), 8 if lens_code == _lib.DTYPE_I64 else 4
+    for r in range(0, s, _lib.DECODE_PAGED_MAX_SEQS):
+        n = min(s - r, _lib.DECODE_PAGED_MAX_SEQS)
+        # fp32 partials: stream-ordered scratch from torch's caching allocator
+        size = L.hcp_decode_fp4_workspace(n, h, hkv, d)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _lib.launch(L.hcp_decode_fp4, _lib.pack_decode_paged(
+            q_at + 2 * r * q_tok, q_tok, q_head, desc.addr, 0, bt_at + 4 * r * bt_row, 0,
+            desc.stride_head, desc.stride_block, 0, 0, desc.block_size, desc.num_blocks, bt_row,
+            width, lens_at + wide * r, ws.data_ptr(), size, out_at + 2 * r * o_tok, o_tok, o_head,
+            lse_at and lse_at + 4 * r, s, lens_code, n, window or 0, h, hkv, d,
+            _lib.DTYPE_BF16 if dt == torch.bfloat16 else _lib.DTYPE_F16, keep_nan, scale,
+            starts_at and starts_at + wide * r), index, "hcp_decode_fp4")
     return (out, lse) if with_lse else out
 
 
