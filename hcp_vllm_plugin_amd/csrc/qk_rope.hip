@@ -9,10 +9,12 @@
 // rounded from 32 bits to 16.  A key on its way into the 4-bit cache is computed in
 // 64 bits up to there: next to a border between two codes a difference in the last place is a
 // whole step of the code, and so the cache does not depend on the order in which
-// something is summed (the pass waits on memory either way).
+// something is summed.
 //
 // HBM-bound: 4 d bytes for a query row, 4 d (16-bit cache) or 2 d + 17 d / 32 for a
-// key or value row.  A lane holds 16 columns of a row, the eight of a pair's first
+// key or value row; 8192 tokens of 28 / 4 x 128 (155 MB) 33 us, 4.7 TB/s, where a
+// large copy runs at 4.9; 4096 of 64 / 8 x 128 into the 4-bit cache (155 MB) 36 us;
+// one token 3.8 us.  A lane holds 16 columns of a row, the eight of a pair's first
 // sides and the eight of their second sides, so that nothing is exchanged but the
 // sum of squares, over the 8 lanes of a row at d = 128; it keeps its 8 cosines and
 // sines for all heads of its token (read again for every head they would be twice
@@ -106,7 +108,7 @@ __device__ __forceinline__ void rope_row(const RopeParams& p, const RopeLane& l,
 // The same in 64 bits, four columns at a time, each widened where it is used: all
 // sixteen at once, with weights and angles held widened across the wave's rows,
 // take 167 registers where these take 126, and leave three waves on a SIMD (4096
-// tokens at 64 / 8 heads x 128: 52 us with the read back, now 42).
+// tokens at 64 / 8 heads x 128: 52 us with the read back, then 42).
 template <typename T>
 __device__ __forceinline__ void rope_row_wide(const RopeParams& p, const RopeLane& l, bool norm,
                                               const float (&wa)[8], const float (&wb)[8],
@@ -245,17 +247,20 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(RopeParams p) {
                        (t * p.v_stride_tok + h * p.v_stride_head) * 2
                  : reinterpret_cast<const char*>(p.k) +
                        (t * p.k_stride_tok + h * p.k_stride_head) * 2, a, b);
-    u32x4 ka = a, kb = b;
-    if constexpr (CACHE == kRopeCacheFp4)
-      rope_row_wide<T>(p, l, p.k_weight != nullptr, wa, wb, lpr, ka, kb);
-    else
-      rope_row<T>(p, l, p.k_weight != nullptr, wa, wb, lpr, ka, kb);
-    if (!is_v) {
-      a = ka;
-      b = kb;
-      if (in && p.k_out != nullptr)
-        put(reinterpret_cast<char*>(p.k_out) +
-                (t * p.ko_stride_tok + h * p.ko_stride_head) * 2, a, b);
+    // (the 64-bit arithmetic not for a job of values alone: 42.6 -> 40.7 us there)
+    if (CACHE != kRopeCacheFp4 || j * rows < p.num_kv_heads) {
+      u32x4 ka = a, kb = b;
+      if constexpr (CACHE == kRopeCacheFp4)
+        rope_row_wide<T>(p, l, p.k_weight != nullptr, wa, wb, lpr, ka, kb);
+      else
+        rope_row<T>(p, l, p.k_weight != nullptr, wa, wb, lpr, ka, kb);
+      if (!is_v) {
+        a = ka;
+        b = kb;
+        if (in && p.k_out != nullptr)
+          put(reinterpret_cast<char*>(p.k_out) +
+                  (t * p.ko_stride_tok + h * p.ko_stride_head) * 2, a, b);
+      }
     }
     if constexpr (CACHE == kRopeCache16) {
       if (in && write)
