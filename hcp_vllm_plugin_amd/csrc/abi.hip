@@ -1210,7 +1210,7 @@ static int check_fp4(uint64_t addr, int64_t stride_block, int64_t stride_head, i
                 "two from 16 to 65536)", who, block_size);
   if (num_blocks < 0 || num_blocks > INT32_MAX)
     return fail(HCP_EINVAL, "%s: bad num_blocks", who);
-  if (!addr || (addr & 15) || stride_block % 16 || stride_head % 16)
+  if ((!addr && num_blocks) || (addr & 15) || stride_block % 16 || stride_head % 16)
     return fail(HCP_EINVAL, "%s: the cache must be 16-byte aligned, strides too", who);
   return HCP_OK;
 }
@@ -1246,9 +1246,9 @@ static int decode_unplanned(const hcp_decode_paged_args* a, bool fp4, const char
       rc = fail(HCP_EUNSUPPORTED, "%s: seq_starts need a 4-bit cache", who);
   }
   if (rc) return rc;
-  // the kernel sums chunks of 32 keys in 32 bits
+  // the kernels sum chunks of 32 keys in 32 bits, and look 256 keys ahead over the 4-bit cache
   if (a->block_table_width > ((int64_t{1} << 34) / kv.block_size) / a->num_seqs ||
-      a->block_table_width * kv.block_size > INT32_MAX)
+      a->block_table_width * kv.block_size > INT32_MAX - (fp4 ? 512 : 0))
     return fail(HCP_EUNSUPPORTED, "%s: block table names too many keys", who);
   const int32_t per_cu = fp4 ? fp4_per_cu(a->head_dim) : kPagedPerCu;
   const size_t need =
@@ -1506,6 +1506,8 @@ static int32_t shift_of(int32_t x) {
 
 static bool index_dtype(int32_t d) { return d == HCP_DTYPE_I32 || d == HCP_DTYPE_I64; }
 
+constexpr int64_t kMostThreads = (int64_t{1} << 32) - 256;  // of a launch
+
 // What hcp_fp4_write and hcp_fp4_read share.
 static int fp4_params(hcp::Fp4Params& p, const void* slots, int32_t slot_dtype, int64_t num_tokens,
                       int32_t num_kv_heads, const hcp_fp4_cache* cache, int32_t dtype,
@@ -1520,8 +1522,8 @@ static int fp4_params(hcp::Fp4Params& p, const void* slots, int32_t slot_dtype, 
                            c.head_dim, who);
   if (rc) return rc;
   if (num_tokens > 0 && !slots) return fail(HCP_EINVAL, "%s: null pointer", who);
-  // one thread per eight columns, 256 to a workgroup: the grid stays within 32 bits
-  if (num_tokens > (int64_t{1} << 31) / (num_kv_heads * (c.head_dim / 8)) * 128)
+  // one thread per eight columns: a launch's threads are counted in 32 bits
+  if (num_tokens > kMostThreads / num_kv_heads / (c.head_dim / 8))
     return fail(HCP_EINVAL, "%s: too many rows", who);
   p.slots = slots;
   p.slots_wide = slot_dtype == HCP_DTYPE_I64;
@@ -1596,7 +1598,7 @@ int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries, const i
   if (!aligned8(entries) || !aligned8(out_start) || !aligned16(k_out) || !aligned16(v_out) ||
       !aligned8(entries_out))
     return fail(HCP_EINVAL, "%s: misaligned pointer", who);
-  if (max_len > (int64_t{1} << 31) / (num_kv_heads * (c.head_dim / 8)) * 128)
+  if (max_len > kMostThreads / num_kv_heads / (c.head_dim / 8))
     return fail(HCP_EINVAL, "%s: too many rows", who);
   hcp::Fp4GatherParams p{};
   p.entries = entries;
@@ -1636,8 +1638,8 @@ int hcp_qk_norm_rope(const hcp_qk_rope_args* a, void* stream) {
     return fail(HCP_EUNSUPPORTED, "%s: index dtype (int32 or int64)", who);
   if (a->cache_kind < 0 || a->cache_kind > 2)
     return fail(HCP_EINVAL, "%s: cache_kind %d", who, a->cache_kind);
-  if (a->num_tokens < 0 || a->num_tokens > INT32_MAX || a->num_slots < 0 ||
-      a->num_slots > a->num_tokens)
+  if (a->num_tokens < 0 || a->num_tokens > kMostThreads / 64 || a->num_slots < 0 ||
+      a->num_slots > a->num_tokens)  // (a wave for a token)
     return fail(HCP_EINVAL, "%s: bad num_tokens / num_slots", who);
   if (!(a->eps >= 0) || !std::isfinite(a->eps))
     return fail(HCP_EINVAL, "%s: eps must be finite and >= 0", who);

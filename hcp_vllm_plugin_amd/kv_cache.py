@@ -133,7 +133,7 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Te
                       slot_mapping: torch.Tensor) -> None:
     """Write ``key``/``value`` ``[N, Hkv, D]`` rows ``[0, n)``, ``n =
     slot_mapping.numel()``, into ``kv_cache`` at ``slot_mapping``; into a 4-bit
-    cache (uint8) as its codes."""
+    cache (uint8) as its codes.  Slots inside the cache are distinct."""
     if kv_cache.dtype == torch.uint8:
         return _write_fp4(key, value, kv_cache, slot_mapping)
     _, desc_addr, hkv, d = _cache_desc(kv_cache)

@@ -78,7 +78,7 @@ def qk_norm_rope(
 
     With ``value``, ``kv_cache`` and ``slot_mapping``, key and value of token t go
     into the cache at ``slot_mapping[t]`` (tokens past its length and negative
-    slots are not written); the key then comes back only where ``key_out`` asks
+    slots are not written, the others are distinct); the key then comes back only where ``key_out`` asks
     for it.  ``query_out`` / ``key_out`` may be query and key themselves."""
     dt, index = query.dtype, query.get_device()
     code = _TYPES.get(dt)

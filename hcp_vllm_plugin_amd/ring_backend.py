@@ -1307,6 +1307,12 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
         addresses, the entries; over a 4-bit cache a list of launches, each with
         keys that fit the scratch they are expanded into."""
         if pc.layout == "fp4":
+            w = self.sliding_window
+            if w is not None:  # keys before every query's window are not expanded
+                skip = np.clip(ent["causal_offset"] - w + 1, 0, ent["len"])
+                ent["start"] += skip
+                ent["len"] -= skip
+                ent["causal_offset"] -= skip
             most = _FP4_SCRATCH // (4 * self.num_kv_heads * self.head_size)
             launches, first, keys = [], 0, 0
             for i, n in enumerate([*ent["len"].tolist(), most + 1]):
@@ -1379,7 +1385,9 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
         """Launches of the batch's requests ``rows`` (query rows ``qs``, ``keys``
         keys each, the first seen ``starts``): [(first, end of a run of query rows,
         or their indices and None, launch)], each of as many as one takes."""
-        most = _lib.DECODE_PAGED_MAX_SEQS
+        # (a launch's keys are counted in 32-key chunks, in 32 bits)
+        named = max(1, block_table.shape[1] * pc.block_size)
+        most = max(1, min(_lib.DECODE_PAGED_MAX_SEQS, (1 << 34) // named))
         words = [np.ascontiguousarray(x, dtype=np.int64) for x in (rows, qs, keys, starts)
                  if x is not None]
         dev, _ = _upload(words, query.device)
@@ -1421,25 +1429,42 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
         ends = [min(sum(int(kv[0].shape[0]) for kv in s), tk) if s else 0
                 for s, tk in zip(staged, seq_lens)]
         starts = [0 if end >= tk else end for end, tk in zip(ends, seq_lens)]
-        key = (*self._layout_key("fp4_rows", pc), _lib.stream_ptr(query.device), tuple(starts))
-        plans = step.fast.get(key)
-        if plans is None:
+        kvs, of = [], []  # chunks that some query sees, and whose
+        for r, (chunks, start) in enumerate(zip(staged, starts)):
+            if start:
+                kvs += [kv for kv in chunks if kv[0].shape[0] > 0]
+                of += [r] * (len(kvs) - len(of))
+        lens = [int(k.shape[0]) for k, _ in kvs]
+        # planned for a step's first layer, the others bring their chunks' addresses
+        key = (*self._layout_key("fp4_rows", pc), _lib.stream_ptr(query.device), tuple(starts),
+               tuple(of), tuple(lens))
+        plan = step.fast.get(key)
+        if plan is None:
             if max(seq_lens) > block_table.shape[1] * pc.block_size:
                 raise ValueError("segment extends past the block-table row")
             if min(seq_lens) < 0:
                 raise ValueError("negative segment start/length")
             rows = np.arange(n)
-            plans = step.fast[key] = self._plan_fp4_rows(query, rows, rows, seq_lens, block_table,
-                                                         pc, starts)
+            plan = step.fast[key] = {"batch": None, "rows": self._plan_fp4_rows(
+                query, rows, rows, seq_lens, block_table, pc, starts)}
         lse = torch.empty((self.num_heads, n), dtype=torch.float32, device=query.device)
-        self._run_fp4_rows(plans, query, out, pc, False, lse)
+        self._run_fp4_rows(plan["rows"], query, out, pc, False, lse)
         _count("decode")
-        segs = [[segment_contiguous(k, v) for k, v in s if k.shape[0] > 0] if 0 < end < tk else []
-                for s, end, tk in zip(staged, ends, seq_lens)]
-        if any(segs):
-            DecodeBatch(segs, self.num_heads, self.num_kv_heads, self.head_size,
-                        query.device).run(query, out, None, self.scale, acc=(out, lse))
-            _count("decode")
+        if not kvs:
+            return
+        words, batch = _chunk_words(kvs), plan["batch"]
+        if batch is None:
+            ent = np.zeros(len(kvs), dtype=ENTRY_DTYPE)
+            ent["q_start"], ent["q_len"], ent["len"] = of, 1, lens
+            for i, f in enumerate(("k_addr", "v_addr", "stride_tok", "stride_head")):
+                ent[f] = words[:, i]
+            batch = plan["batch"] = DecodeBatch.from_entries(
+                ent, self.num_heads, self.num_kv_heads, self.head_size, query.device, keep=kvs,
+                entry_seq=np.asarray(of, dtype=np.int32), num_seqs=n)
+        else:
+            batch = batch.rebind_chunks(words, kvs)
+        batch.run(query, out, None, self.scale, acc=(out, lse))
+        _count("decode")
 
     def _local_launch(self, query, plan: _Plan, step, pc):
         """The launch of a plan's local entries, shared by the layers that plan

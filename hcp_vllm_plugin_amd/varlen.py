@@ -957,7 +957,7 @@ def decode_fp4(
         raise ValueError("q must be float16/bfloat16 [S, H, D] with contiguous head_dim")
     desc, hkv, dim = fp4_desc(kv_cache)
     s, h, d = q.shape
-    if d != dim or h % hkv:
+    if d != dim or not hkv or h % hkv:
         raise ValueError("kv_cache must be a 4-bit cache of q's head_dim, its heads dividing q's")
     if window is not None and window <= 0:
         raise ValueError("window must be a positive number of keys")
@@ -991,8 +991,10 @@ def decode_fp4(
     bt_at, lens_at, starts_at = block_table.data_ptr(), seq_lens.data_ptr(), \
         0 if starts is None else starts.data_ptr()
     L, wide = _lib.lib(), 8 if lens_code == _lib.DTYPE_I64 else 4
-    for r in range(0, s, _lib.DECODE_PAGED_MAX_SEQS):
-        n = min(s - r, _lib.DECODE_PAGED_MAX_SEQS)
+    # (a launch's keys are counted in 32-key chunks, in 32 bits)
+    most = max(1, min(_lib.DECODE_PAGED_MAX_SEQS, (1 << 34) // max(1, width * desc.block_size)))
+    for r in range(0, s, most):
+        n = min(s - r, most)
         # fp32 partials: stream-ordered scratch from torch's caching allocator
         size = L.hcp_decode_fp4_workspace(n, h, hkv, d)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
@@ -1000,7 +1002,7 @@ def decode_fp4(
             q_at + 2 * r * q_tok, q_tok, q_head, desc.addr, 0, bt_at + 4 * r * bt_row, 0,
             desc.stride_head, desc.stride_block, 0, 0, desc.block_size, desc.num_blocks, bt_row,
             width, lens_at + wide * r, ws.data_ptr(), size, out_at + 2 * r * o_tok, o_tok, o_head,
-            lse_at and lse_at + 4 * r, s, lens_code, n, window or 0, h, hkv, d,
+            lse_at and lse_at + 4 * r, s, lens_code, n, min(window or 0, 0x7fffffff), h, hkv, d,
             _lib.DTYPE_BF16 if dt == torch.bfloat16 else _lib.DTYPE_F16, keep_nan, scale,
             starts_at and starts_at + wide * r), index, "hcp_decode_fp4")
     return (out, lse) if with_lse else out

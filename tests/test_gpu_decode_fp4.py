@@ -89,7 +89,7 @@ def test_few_sequences(dev, lens, h, hkv, d):
     assert torch.equal(again, got[0])
 
 
-@pytest.mark.parametrize("window", [1, 2, 16, 31, 33, 100, 5000])
+@pytest.mark.parametrize("window", [1, 2, 16, 31, 33, 100, 5000, 1 << 40])
 @pytest.mark.parametrize("with_starts", [False, True])
 def test_window_and_starts(dev, window, with_starts):
     gen = torch.Generator().manual_seed(window)

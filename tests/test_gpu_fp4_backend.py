@@ -92,7 +92,7 @@ class Step:
                 k, v, pk, pv = kvs[r]
                 qr = q[a:a + n]
                 first, see = tk - n, torch.arange(tk)[None] <= tk - n + torch.arange(n)[:, None]
-                if self.window:
+                if self.window:  # (of the local keys; a staged prefix is seen whole)
                     see &= torch.arange(tk)[None] > tk - n - self.window + torch.arange(n)[:, None]
                 if peer:
                     # queries past the prefix see it whole, and the local keys behind it
@@ -140,8 +140,23 @@ def test_without_peers(dev, h, hkv, d, dtype, window, reqs):
     [(90, 180, 128), (1, 250, 64), (20, 20, 0)],      # across a prefix's end; mixed
 ])
 def test_with_staged_peers(dev, h, hkv, d, dtype, reqs):
-    s = Step(dev, reqs, h, hkv, d, dtype, seed=d + 1, layers=2)
+    s = Step(dev, reqs, h, hkv, d, dtype, seed=d + 1, layers=3)
     s.check(s.run())
+
+
+def test_two_chunks_and_a_window_behind_peers(dev):
+    """A prefix of two chunks; a window that ends inside the local keys."""
+    for window in (None, 30):
+        s = Step(dev, [(1, 400, 130), (1, 90, 0), (1, 260, 64)], 28, 4, 128, torch.bfloat16,
+                 window=window, seed=9, layers=2)
+        first = int(s.meta.block_table[0, 0])
+        for layer, _, kvs, _ in s.layers:
+            pk, pv = kvs[0][2].to(dev), kvs[0][3].to(dev)
+            rb.stage_peer_kv("a", layer.layer_name, pk[:50], pv[:50])
+            rb.stage_peer_kv("b", layer.layer_name, pk[50:], pv[50:])
+        rb.map_request_peer(first, ["a", "b"])
+        s.check(s.run())
+        rb.clear_peer_kv()
 
 
 def test_decode_rows_apart(dev, monkeypatch):

@@ -127,9 +127,11 @@ def test_c_writes_and_reads_refuse(L):
         assert b"hcp_fp4_write" in L.hcp_last_error()
     ok[8] = 0
     assert L.hcp_fp4_write(*ok) == _lib.HCP_OK  # nothing to write
-    ok[8], d.num_blocks = 5, 0
+    ok[8], d.num_blocks, d.addr = 5, 0, 0
     assert L.hcp_fp4_write(*ok) == _lib.HCP_OK  # nowhere to write
-    d.num_blocks = 10
+    d.num_blocks, d.addr = 10, 0x1000
+    ok[8] = (1 << 32) // (4 * 16)  # threads past 32 bits
+    assert L.hcp_fp4_write(*ok) == _lib.HCP_EINVAL
     ok = [4096, _lib.DTYPE_I64, 5, 4, at, _lib.DTYPE_BF16, 4096, 4096, None]
     for i, x in ((0, None), (2, -1), (3, 0), (4, None), (6, None), (7, 4104)):
         args = list(ok)
@@ -167,7 +169,8 @@ def test_c_decode_refuses(L):
             ("num_heads", 27, _lib.HCP_EINVAL), ("dtype", _lib.DTYPE_F32, _lib.HCP_EUNSUPPORTED),
             ("num_seqs", -1, _lib.HCP_EINVAL), ("num_seqs", 1025, _lib.HCP_EUNSUPPORTED),
             ("window", -1, _lib.HCP_EINVAL), ("block_table_width", 0, _lib.HCP_EINVAL),
-            ("block_table_width", 1 << 28, _lib.HCP_EUNSUPPORTED), ("q", 0, _lib.HCP_EINVAL),
+            ("block_table_width", 1 << 28, _lib.HCP_EUNSUPPORTED),
+            ("block_table_width", (1 << 27) - 20, _lib.HCP_EUNSUPPORTED), ("q", 0, _lib.HCP_EINVAL),
             ("q", 0x10008, _lib.HCP_EINVAL), ("q_stride_tok", 100, _lib.HCP_EINVAL),
             ("scale", 0.0, _lib.HCP_EINVAL), ("lens_dtype", 7, _lib.HCP_EUNSUPPORTED),
             ("workspace_bytes", need - 1, _lib.HCP_EWORKSPACE), ("workspace", 8, _lib.HCP_EINVAL)):
@@ -210,6 +213,7 @@ def test_c_rope_refuses(L):
             ({"weight_dtype": _lib.DTYPE_F16}, _lib.HCP_EUNSUPPORTED),
             ({"pos_dtype": 2}, _lib.HCP_EUNSUPPORTED), ({"cache_kind": 3}, _lib.HCP_EINVAL),
             ({"num_tokens": -1}, _lib.HCP_EINVAL), ({"num_slots": 6}, _lib.HCP_EINVAL),
+            ({"num_tokens": 1 << 26}, _lib.HCP_EINVAL),
             ({"eps": -1.0}, _lib.HCP_EINVAL), ({"eps": float("nan")}, _lib.HCP_EINVAL),
             ({"q": 0}, _lib.HCP_EINVAL), ({"q_out": 0x10004}, _lib.HCP_EINVAL),
             ({"positions": 0}, _lib.HCP_EINVAL), ({"max_positions": 0}, _lib.HCP_EINVAL),
