@@ -23,10 +23,10 @@
 // 16k-32k 64 -> 51 us).  The waves are combined through LDS; decode_reduce_kernel
 // merges a sequence's partials.
 //
-// Bound by HBM: 64 x 16k-32k keys of 28 / 4 x 128 (850 MB) take 148 us with the
-// merge, 5.7 TB/s; its loads alone, without the arithmetic, take 142, and the
-// 16-bit kernel reads blocks at 6.1 TB/s.  One sequence of 2000 keys: 11.4 us, the
-// chain of latencies (lengths, block ids, keys, combine, merge).
+// Bound by HBM: 64 x 16k-32k keys of 28 / 4 x 128 (850 MB) take 143 us with the
+// merge, 6.0 TB/s; its loads alone, without the arithmetic, 95% of that; the 16-bit
+// kernel reads blocks at 6.1 TB/s.  One sequence of 2000 keys: 11.4 us, the chain of
+// latencies (lengths, block ids, keys, combine, merge).
 #include "decode_share.h"
 
 namespace hcp {

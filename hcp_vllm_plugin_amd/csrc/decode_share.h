@@ -106,7 +106,8 @@ __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, i
   unsigned wgs = static_cast<unsigned>(p_.d.num_wgs);
   {
     const unsigned least = (total + LEAST - 1) / LEAST, twice = total / (2 * LEAST);
-    const unsigned few = wgs / LATE < least ? wgs / LATE : least, many = few > twice ? few : twice;
+    const unsigned early = (wgs + LATE - 1) / LATE;
+    const unsigned few = early < least ? early : least, many = few > twice ? few : twice;
     wgs = wgs < many ? wgs : many;
   }
   if (static_cast<unsigned>(wg) < wgs) {

@@ -77,6 +77,16 @@ def test_ragged(dev, dtype, h, hkv, d, bs):
     check(got, q, kvs, scale_for(d), dtype)
 
 
+def test_more_heads_than_workgroups(dev):
+    """KV heads that leave one workgroup to each of them."""
+    gen = torch.Generator().manual_seed(13)
+    lens = [5, 70]
+    q, cache, bt, kvs = batch(gen, dev, lens, 700, 700, 64, 16, torch.bfloat16)
+    t = torch.tensor(lens, dtype=torch.int32, device=dev)
+    got = decode_fp4(q.to(dev), cache, bt.to(dev), t, scale_for(64), with_lse=True)
+    check(got, q, kvs, scale_for(64), torch.bfloat16)
+
+
 @pytest.mark.parametrize("lens", [[1], [2000], [9000], [20000, 3], [0], [0, 0, 5]])
 @pytest.mark.parametrize("h,hkv,d", [(28, 4, 128), (16, 8, 256), (14, 2, 64)])
 def test_few_sequences(dev, lens, h, hkv, d):
