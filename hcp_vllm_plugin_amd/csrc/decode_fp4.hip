@@ -13,8 +13,10 @@
 //    16 query heads are the columns, the contraction order of either product is
 //    free, so K's is the order of a lane's bytes and P stays in the registers S
 //    came in; V's keys are paired by one v_perm for two values;
-//  * the running maximum is raised, and O rescaled, only when a score is past it
-//    by 2^8 (fp32 sums and two 16-bit terms of P have room for that).
+//  * the running maximum is raised, and O rescaled, only when a weight is past 2^8
+//    (fp32 sums and two 16-bit terms of P have room for that), so that a chunk
+//    needs the maximum of its weights alone; their sum is a matrix product with
+//    ones.
 // The 4 waves of a workgroup take the 32-key chunks of its share in turn (chunks
 // lie on multiples of 32 positions, so that 16 keys never cross a block), each
 // through LDS of its own, where the next chunk lands while one is computed (held
@@ -23,10 +25,13 @@
 // 16k-32k 64 -> 51 us).  The waves are combined through LDS; decode_reduce_kernel
 // merges a sequence's partials.
 //
-// Bound by HBM: 64 x 16k-32k keys of 28 / 4 x 128 (850 MB) take 143 us with the
-// merge, 6.0 TB/s; its loads alone, without the arithmetic, 95% of that; the 16-bit
-// kernel reads blocks at 6.1 TB/s.  One sequence of 2000 keys: 11.4 us, the chain of
-// latencies (lengths, block ids, keys, combine, merge).
+// Bound by HBM: 64 x 16k-32k keys of 28 / 4 x 128 (850 MB) take 144 us with the
+// merge, 5.9 TB/s (146 on the same card with the scores' maximum, the sum and the
+// scales in more instructions); its loads alone, without the arithmetic, 94% of
+// that; the 16-bit kernel reads blocks at 6.1 TB/s.  At 64 columns a chunk has as
+// many instructions for half the bytes: 256 x 32k keys of 14 / 2 x 64 (1.13 GB) take
+// 230 us (237 before), 200 by the loads alone.  One sequence of 2000 keys: 11.4 us,
+// the chain of latencies (lengths, block ids, keys, combine, merge).
 #include "decode_share.h"
 
 namespace hcp {
@@ -50,7 +55,40 @@ __device__ __forceinline__ T lds_at(const HCP_LDS_PTR(char) p) {
   return *reinterpret_cast<const HCP_LDS_PTR(T)>(p);
 }
 
-constexpr float kRaise = 8.f;  // how far (in powers of two) a score may pass the running maximum
+constexpr float kRaise = 256.f;  // exp of how far a score may pass the running maximum
+
+// Two weights (0 to kRaise, or NaN) in two 16-bit terms: hi near the weight, lo
+// what is left of it, 2^-17 of it or less (fp16: to 2^-24 at least).  (two_terms
+// of common.h keeps both terms positive for the products with an infinity; the
+// 4-bit cache holds none.)
+template <typename T>
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo);
+template <>
+__device__ __forceinline__ void split_weights<__bf16>(float a, float b, uint32_t& hi,
+                                                      uint32_t& lo) {
+  hi = pack2<__bf16>(a, b);
+  lo = pack2<__bf16>(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ void split_weights<_Float16>(float a, float b, uint32_t& hi,
+                                                        uint32_t& lo) {
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  lo = __builtin_bit_cast(
+      uint32_t, __builtin_amdgcn_cvt_pkrtz(
+                    a - Elem<_Float16>::to_float(static_cast<uint16_t>(hi & 0xffffu)),
+                    b - Elem<_Float16>::to_float(static_cast<uint16_t>(hi >> 16))));
+}
+
+// Byte J of a dword of scales as a float, in one instruction.
+template <int J>
+__device__ __forceinline__ float fp4_scale_of(uint32_t w) {
+  uint32_t r;
+  asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD "
+      "src1_sel:BYTE_%3"
+      : "=v"(r)
+      : "v"(23), "v"(w), "n"(J));
+  return __uint_as_float(r);
+}
 
 template <int D, typename T, bool KEEP_NAN>
 __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_in, int chunk_in,
@@ -89,7 +127,7 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   }
 
   const int bs = p.kv.block_size, bs_shift = 31 - __builtin_clz(bs);
-  const auto* bt = global_ptr(reinterpret_cast<const int32_t*>(
+  const auto* bt = global_ptr(reinterpret_cast<const char*>(
       p.kv.block_table + static_cast<uint64_t>(r) * p.bt_stride * 4));
   const uint32_t id_max = static_cast<uint32_t>(p.kv.num_blocks) - 1;
   const char* head = reinterpret_cast<const char*>(p.kv.k_addr) + kvh * p.kv.stride_head;
@@ -115,7 +153,8 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   // Block ids of a chunk's tiles, in the two halves of the wave.
   auto fetch_ids = [&](int x0) __attribute__((always_inline)) {
     const int x = x0 + (lane & 32) / 2;
-    return static_cast<uint32_t>(bt[(x < all ? x : all - 1) >> bs_shift]);
+    const uint32_t at = static_cast<uint32_t>(x < all ? x : all - 1) >> bs_shift << 2;
+    return *global_ptr(reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(bt) + at));
   };
   // (buffer loads: behind global loads into LDS the compiler waits for every load
   // before it uses one's result)
@@ -156,7 +195,14 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   const int vs_at = Tile::SC + Tile::SW * 4 + (g4 * ng + (vgrp < ng ? vgrp : 0)) * 4;
 
   const float c = p.d.scale_log2;
-  float m_run = -INFINITY, l_run = 0.f;
+  // -(running maximum), 0 before the first; the weight past which it is raised; the
+  // sum of the weights as rounded (a matrix product with ones, in every row)
+  float neg_m = 0.f, limit = -1.f;
+  f32x4 lacc = f32x4{};
+  const V8 ones = as_vec8<V8>(__is_same(T, __bf16)
+                                  ? u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
+                                  : u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u});
+  const uint32_t half = c16 & 1 ? 0x07060302u : 0x05040100u;
   f32x4 oacc[NU];
 #pragma unroll
   for (int u = 0; u < NU; ++u) oacc[u] = f32x4{};
@@ -199,55 +245,76 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
           }
         }
     }
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c;
-    if (__builtin_amdgcn_ballot_w64(mx > m_run + kRaise) != 0) {
+    float w[2][4];
+    auto weights = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[t][i] = fast_exp2(__builtin_fmaf(s[t][i], c, neg_m));
+    };
+    weights();
+    const float top = fmaxf(fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[0][2], w[0][3])),
+                            fmaxf(fmaxf(w[1][0], w[1][1]), fmaxf(w[1][2], w[1][3])));
+    if (__builtin_amdgcn_ballot_w64(top > limit) != 0) {
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c;
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(m_run, mx);
-      const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
-      m_run = m_new;
-      l_run *= alpha;
+      const float m_old = limit < 0.f ? -INFINITY : -neg_m;
+      const float m_new = fmaxf(m_old, mx);
+      neg_m = m_new == -INFINITY ? 0.f : -m_new;
+      limit = m_new == -INFINITY ? -1.f : kRaise;
+      const float alpha = fast_exp2(m_old + neg_m);
+      lacc *= alpha;
 #pragma unroll
       for (int u = 0; u < NU; ++u) oacc[u] *= alpha;
+      weights();
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
     u32x4 pw, rw;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = fast_exp2(__builtin_fmaf(s[t][i], c, -m_use));
-        l_run += s[t][i];
-      }
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // P in two 16-bit terms, as in decode_split_body
         uint32_t hi, lo;
-        two_terms<T>(s[t][2 * i], s[t][2 * i + 1], hi, lo);
+        split_weights<T>(w[t][2 * i], w[t][2 * i + 1], hi, lo);
         pw[2 * t + i] = hi;
         rw[2 * t + i] = lo;
       }
-    }
     const V8 pf = as_vec8<V8>(pw), rf = as_vec8<V8>(rw);
+    lacc = E::mfma16(ones, pf, lacc);
+    lacc = E::mfma16(ones, rf, lacc);
     float vs[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      vs[j] = __uint_as_float(((vsw[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
+    for (int t = 0; t < 2; ++t) {
+      vs[4 * t] = fp4_scale_of<0>(vsw[t]);
+      vs[4 * t + 1] = fp4_scale_of<1>(vsw[t]);
+      vs[4 * t + 2] = fp4_scale_of<2>(vsw[t]);
+      vs[4 * t + 3] = fp4_scale_of<3>(vsw[t]);
+    }
     u32x4 vw[2][Tile::P];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < Tile::P; ++i)
         vw[t][i] = lds_at<u32x4>(src + t * Tile::BYTES + i * 1024 + vc_at);
+    if constexpr (D == 64) {
+      // a lane's two of the four bytes, of two keys in one dword
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          vw[t][0][j] = __builtin_amdgcn_perm(vw[t][0][2 * j + 1], vw[t][0][2 * j], half);
+    }
     // columns 2 u and 2 u + 1 of 8 keys -> two operands
     auto pv = [&](auto sel, auto piece, int u) __attribute__((always_inline)) {
       uint32_t x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t w = vw[j >> 2][decltype(piece)::value][j & 3];
-        if constexpr (D == 64) w >>= 16 * (c16 & 1);
-        x[j] = fp4_pair<T, decltype(sel)::value>(w, vs[j]);
+      for (int j = 0; j < 8; j += 2) {
+        constexpr int S = decltype(sel)::value;
+        const u32x4 v = vw[j >> 2][decltype(piece)::value];
+        const int at = D == 64 ? (j & 3) >> 1 : j & 3;
+        x[j] = fp4_pair<T, S>(v[at], vs[j]);
+        x[j + 1] = fp4_pair<T, D == 64 ? S + 2 : S>(v[D == 64 ? at : at + 1], vs[j + 1]);
       }
       u32x4 a, b;
 #pragma unroll
@@ -319,11 +386,9 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   float (*const so_o)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(&bufO[0][0]);
   static_assert(sizeof(float) * 2 * 16 * (D + 4) <= W * 2 * Tile::BYTES, "combine staging");
   float (*const mine)[D + 4] = wave < 2 ? so_e[wave] : so_o[wave - 2];
-  float l_tot = l_run + __shfl_xor(l_run, 16);
-  l_tot += __shfl_xor(l_tot, 32);
   if (g4 == 0) {
-    sm_m[wave][c16] = m_run;
-    sm_l[wave][c16] = l_tot;
+    sm_m[wave][c16] = limit < 0.f ? -INFINITY : -neg_m;
+    sm_l[wave][c16] = lacc[0];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
