@@ -1579,11 +1579,11 @@ int hcp_fp4_read(const void* slot_mapping, int32_t slot_dtype, int64_t num_token
 }
 
 int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries, const int64_t* out_start,
-                   int64_t max_len, int32_t num_kv_heads, const hcp_fp4_cache* cache,
+                   int64_t num_rows, int32_t num_kv_heads, const hcp_fp4_cache* cache,
                    int32_t dtype, void* k_out, void* v_out, hcp_varlen_entry* entries_out,
                    void* stream) {
   const char* who = "hcp_fp4_gather";
-  if (num_entries < 0 || max_len < 0 || num_kv_heads <= 0)
+  if (num_entries < 0 || num_rows < 0 || num_kv_heads <= 0)
     return fail(HCP_EINVAL, "%s: bad sizes", who);
   if (!dtype16(dtype)) return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, dtype);
   if (!cache) return fail(HCP_EINVAL, "%s: null cache descriptor", who);
@@ -1592,18 +1592,18 @@ int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries, const i
                            c.head_dim, who);
   if (rc) return rc;
   if (num_entries > 65535) return fail(HCP_EINVAL, "%s: more than 65535 entries", who);
-  if (num_entries == 0 || (max_len == 0 && !entries_out)) return HCP_OK;
+  if (num_entries == 0 || (num_rows == 0 && !entries_out)) return HCP_OK;
   if (c.num_blocks == 0) return fail(HCP_EINVAL, "%s: a cache without blocks", who);
   if (!entries || !out_start || !k_out || !v_out) return fail(HCP_EINVAL, "%s: null pointer", who);
   if (!aligned8(entries) || !aligned8(out_start) || !aligned16(k_out) || !aligned16(v_out) ||
       !aligned8(entries_out))
     return fail(HCP_EINVAL, "%s: misaligned pointer", who);
-  if (max_len > kMostThreads / num_kv_heads / (c.head_dim / 8))
+  if (num_rows > kMostThreads / num_kv_heads / (c.head_dim / 8))
     return fail(HCP_EINVAL, "%s: too many rows", who);
   hcp::Fp4GatherParams p{};
   p.entries = entries;
   p.out_start = out_start;
-  p.max_len = max_len;
+  p.num_rows = num_rows;
   p.num_entries = num_entries;
   p.num_kv_heads = num_kv_heads;
   p.opr_shift = shift_of(c.head_dim / 8);

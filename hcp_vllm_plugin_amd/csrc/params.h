@@ -238,7 +238,7 @@ struct Fp4Params {
 struct Fp4GatherParams {
   const hcp_varlen_entry* entries;
   const int64_t* out_start;
-  int64_t max_len;
+  int64_t num_rows;
   int32_t num_entries, num_kv_heads;
   int32_t opr_shift;
   const char* cache;

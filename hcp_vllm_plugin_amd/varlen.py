@@ -432,7 +432,7 @@ class VarlenLaunch:
             out_start = np.zeros(self.num_entries, dtype=np.int64)
             out_start[1:] = np.cumsum(lens)[:-1]
             self._fp4 = {"hkv": fp4.num_kv_heads, "dim": fp4.head_dim, "total": int(lens.sum()),
-                         "max_len": int(lens.max()), "block_size": fp4.block_size,
+                         "block_size": fp4.block_size,
                          "num_blocks": fp4.num_blocks, "stride_head": fp4.stride_head,
                          "stride_block": fp4.stride_block}
             arr = host.copy()
@@ -549,7 +549,7 @@ class VarlenLaunch:
         desc = _lib.Fp4CacheDesc(cache_addr, f["stride_block"], f["stride_head"], f["num_blocks"],
                                  f["block_size"], d)
         rc = _lib.lib().hcp_fp4_gather(
-            f["paged_ptr"], self.num_entries, f["start_ptr"], f["max_len"], hkv,
+            f["paged_ptr"], self.num_entries, f["start_ptr"], f["total"], hkv,
             ctypes.addressof(desc), _lib.dtype_code(q.dtype), base, base + side, base + 2 * side,
             stream)
         _lib.check(rc, "hcp_fp4_gather")

@@ -727,13 +727,15 @@ int hcp_fp4_read(const void* slot_mapping, int32_t slot_dtype, int64_t num_token
 /*
  * hcp_gather_paged_kv out of a 4-bit cache: entry e's keys [kv.start, kv.start +
  * kv.len), through its kv.block_table alone (the other fields of kv are not read;
- * an entry without one is skipped), become rows out_start[e] .. of k_out / v_out.
+ * an entry without one is skipped), become rows out_start[e] .. of k_out / v_out
+ * [num_rows, Hkv, head_dim].  The entries' rows lie in their order: out_start
+ * [num_entries] begins at 0 and does not fall.
  * A block id past the cache reads its last block.  entries_out [num_entries]
  * (DEVICE, may be NULL) gets the entries with kv the contiguous segment of k_out /
  * v_out that they now have, for hcp_varlen_launch to read behind this call.
  */
 int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries,
-                   const int64_t* out_start, int64_t max_len, int32_t num_kv_heads,
+                   const int64_t* out_start, int64_t num_rows, int32_t num_kv_heads,
                    const hcp_fp4_cache* cache, int32_t dtype, void* k_out, void* v_out,
                    hcp_varlen_entry* entries_out, void* stream);
 

@@ -1,10 +1,15 @@
 """GPU: K and V into the 4-bit cache and back (``reshape_and_cache``, ``gather_kv``),
 byte for byte against the format in plain operations."""
 
+import ctypes
+
+import numpy as np
 import pytest
 import torch
 
+from hcp_vllm_plugin_amd import _lib
 from hcp_vllm_plugin_amd.kv_cache import fp4_cache_shape, gather_kv, reshape_and_cache
+from hcp_vllm_plugin_amd.varlen import ENTRY_DTYPE, fp4_desc
 from tests import _fp4_util as f4
 from tests._util import randn
 
@@ -121,3 +126,52 @@ def test_far_blocks(dev):
     kk, vv = gather_kv(cache, slots.to(dev), torch.float16)
     assert torch.equal(kk.cpu().double(), f4.stand_for(k))
     assert torch.equal(vv.cpu().double(), f4.stand_for(v))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hkv,bs,lens", [
+    (128, 4, 16, [37]), (64, 2, 32, [0, 1, 0, 0, 700, 33, 0]), (96, 3, 16, [5] * 70 + [900, 0, 2]),
+    (256, 1, 16, [1] * 4300), (32, 1, 64, [300, 0, 0])])
+def test_gather_of_ragged_entries(dev, dtype, d, hkv, bs, lens):
+    """Entries' keys one after another (``hcp_fp4_gather``): what gather_kv reads at
+    their slots, from any first key on; an entry without a block table, and rows past
+    the last one's, stay as they were."""
+    gen = torch.Generator().manual_seed(d + len(lens))
+    n, start = len(lens), [(7 * i) % 41 for i in range(len(lens))]
+    width = max((s + x + bs - 1) // bs for s, x in zip(start, lens))
+    nb = 400
+    cache = torch.randint(104, 140, fp4_cache_shape(nb, hkv, bs, d), generator=gen,
+                          dtype=torch.uint8).to(dev)
+    table = torch.randint(0, nb, (n, width), generator=gen, dtype=torch.int32)
+    table_dev = table.to(dev)
+    ent = np.zeros(n, dtype=ENTRY_DTYPE)
+    ent["q_len"], ent["start"], ent["len"] = 3, start, lens
+    ent["block_table"] = table_dev.data_ptr() + 4 * width * np.arange(n)
+    skipped = n // 2 if n > 1 else -1
+    if skipped >= 0:
+        ent["block_table"][skipped] = 0
+    at = np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
+    total, more = int(at[-1]), 3
+    ent_dev = torch.from_numpy(ent.view(np.uint8).copy()).to(dev)
+    at_dev = torch.from_numpy(at[:-1].copy()).to(dev)
+    kv = torch.full((2, total + more, hkv, d), 5.0, dtype=dtype, device=dev)
+    made = torch.zeros_like(ent_dev)
+    desc, _, _ = fp4_desc(cache)
+    _lib.check(_lib.lib().hcp_fp4_gather(
+        ent_dev.data_ptr(), n, at_dev.data_ptr(), total, hkv, ctypes.addressof(desc),
+        _lib.dtype_code(dtype), kv[0].data_ptr(), kv[1].data_ptr(), made.data_ptr(),
+        _lib.stream_ptr(dev)), "hcp_fp4_gather")
+    slots = torch.full((total + more,), -1, dtype=torch.int64)
+    for r, (s, x) in enumerate(zip(start, lens)):
+        pos = torch.arange(s, s + x)
+        if r != skipped:
+            slots[at[r]:at[r] + x] = table[r][pos // bs].long() * bs + pos % bs
+    k, v = gather_kv(cache, slots.to(dev), dtype)
+    named = (slots >= 0).to(dev)[:, None, None]
+    for got, want in ((kv[0], k), (kv[1], v)):
+        assert torch.equal(got, torch.where(named, want, 5.0))
+    out = made.cpu().numpy().view(ENTRY_DTYPE)
+    for f, x in (("start", at[:-1]), ("len", lens), ("q_len", 3), ("block_table", 0),
+                 ("stride_tok", hkv * d), ("stride_head", d), ("k_addr", kv[0].data_ptr()),
+                 ("v_addr", kv[1].data_ptr())):
+        assert (out[f] == x).all(), f
