@@ -55,28 +55,23 @@ __device__ __forceinline__ T lds_at(const HCP_LDS_PTR(char) p) {
   return *reinterpret_cast<const HCP_LDS_PTR(T)>(p);
 }
 
-constexpr float kRaise = 256.f;  // exp of how far a score may pass the running maximum
+// How far (in powers of two) a score may pass the running maximum, and what the
+// maximum's own weight is: fp16's terms have 2^-24 for their last place, so that
+// weights begin 2^7 higher, the largest at 2^15 of its 65504.
+constexpr float kRaise = 8.f;
+template <typename T>
+constexpr float kLift = __is_same(T, __bf16) ? 0.f : 7.f;
 
-// Two weights (0 to kRaise, or NaN) in two 16-bit terms: hi near the weight, lo
-// what is left of it, 2^-17 of it or less (fp16: to 2^-24 at least).  (two_terms
-// of common.h keeps both terms positive for the products with an infinity; the
+// Two weights (or NaN) in two 16-bit terms: hi the weight rounded, lo what is left of
+// it, rounded: 2^-17 of it (fp16 2^-22, and 2^-25 at least).  Both to the nearest:
+// cut off, many small weights next to a large one would add up to less than they are.
+// (two_terms of common.h keeps both terms positive for products with an infinity; the
 // 4-bit cache holds none.)
 template <typename T>
-__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo);
-template <>
-__device__ __forceinline__ void split_weights<__bf16>(float a, float b, uint32_t& hi,
-                                                      uint32_t& lo) {
-  hi = pack2<__bf16>(a, b);
-  lo = pack2<__bf16>(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ void split_weights<_Float16>(float a, float b, uint32_t& hi,
-                                                        uint32_t& lo) {
-  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-  lo = __builtin_bit_cast(
-      uint32_t, __builtin_amdgcn_cvt_pkrtz(
-                    a - Elem<_Float16>::to_float(static_cast<uint16_t>(hi & 0xffffu)),
-                    b - Elem<_Float16>::to_float(static_cast<uint16_t>(hi >> 16))));
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(a, b);
+  lo = pack2<T>(a - Elem<T>::to_float(static_cast<uint16_t>(hi & 0xffffu)),
+                b - Elem<T>::to_float(static_cast<uint16_t>(hi >> 16)));
 }
 
 // Byte J of a dword of scales as a float, in one instruction.
@@ -195,9 +190,10 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   const int vs_at = Tile::SC + Tile::SW * 4 + (g4 * ng + (vgrp < ng ? vgrp : 0)) * 4;
 
   const float c = p.d.scale_log2;
-  // -(running maximum), 0 before the first; the weight past which it is raised; the
+  // -(running maximum, kLift below), 0 before the first; the weight past which it is raised; the
   // sum of the weights as rounded (a matrix product with ones, in every row)
   float neg_m = 0.f, limit = -1.f;
+  const float most = __builtin_exp2f(kRaise + kLift<T>);
   f32x4 lacc = f32x4{};
   const V8 ones = as_vec8<V8>(__is_same(T, __bf16)
                                   ? u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
@@ -261,9 +257,9 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float m_old = limit < 0.f ? -INFINITY : -neg_m;
-      const float m_new = fmaxf(m_old, mx);
+      const float m_new = fmaxf(m_old, mx - kLift<T>);
       neg_m = m_new == -INFINITY ? 0.f : -m_new;
-      limit = m_new == -INFINITY ? -1.f : kRaise;
+      limit = m_new == -INFINITY ? -1.f : most;
       const float alpha = fast_exp2(m_old + neg_m);
       lacc *= alpha;
 #pragma unroll

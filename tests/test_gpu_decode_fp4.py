@@ -243,3 +243,51 @@ def test_two_streams(dev):
             outs.append(decode_fp4(qd, cache, btd, t, scale_for(128)))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def _placed(dev, k, v, dtype, kv=None):
+    """One sequence with these keys and values: (cache, table, what they (or kv) stand
+    for in it)."""
+    n, hkv, d = k.shape
+    nb = -(-n // 16) + 1
+    cache = torch.zeros(fp4_cache_shape(nb, hkv, 16, d), dtype=torch.uint8, device=dev)
+    reshape_and_cache(k.to(dev), v.to(dev), cache, torch.arange(n, device=dev))
+    k, v = kv or (k, v)
+    return cache, torch.arange(nb, dtype=torch.int32)[None], (f4.stand_for(k), f4.stand_for(v))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_small_weights(dev, dtype):
+    """A key in the first 32 of each wave far above 32764 others, 2^-14 of it each:
+    together they weigh half as much, so a bias of their weights shows.  (As many KV
+    heads, with the same keys, as leave a workgroup to each.)"""
+    gen, n, heads = torch.Generator().manual_seed(17), 32768, 1024
+    k = (torch.randn(n, 1, 32, generator=gen) * 0.05).to(dtype)
+    v = (1 + 0.1 * torch.randn(n, 1, 32, generator=gen)).to(dtype)
+    k[5:128:32], v[5:128:32] = 0.375, -1.0
+    q = torch.ones(1, heads, 32, dtype=dtype)
+    cache, bt, (ks, vs) = _placed(dev, k.to(dev).expand(n, heads, 32),
+                                  v.to(dev).expand(n, heads, 32), dtype, (k, v))
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    out, lse = decode_fp4(q.to(dev), cache, bt.to(dev), lens, 0.81, with_lse=True)
+    assert (out == out[:, :1]).all() and (lse == lse[:1]).all()
+    check((out[:, :1], lse[:1]), q[:, :1], [(ks, vs)], 0.81, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("slope", [0.01, 0.04, -0.04, 0.3, 3.0])
+def test_scores_that_rise_and_fall(dev, dtype, d, slope):
+    """Scores (of half of the query heads) that climb by ``slope`` a key, past the
+    maximum so far by less or by more than it is let stand, or fall."""
+    gen = torch.Generator().manual_seed(d)
+    n = 900
+    k = randn(gen, (n, 2, d), dtype) * 0.1
+    k[:, :, :32] = (slope * torch.arange(n) / 32)[:, None, None].to(dtype)
+    v = randn(gen, (n, 2, d), dtype)
+    q = randn(gen, (1, 8, d), dtype)
+    q[:, ::2, :32] = 1.0
+    cache, bt, kv = _placed(dev, k.to(dtype), v, dtype)
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    got = decode_fp4(q.to(dev), cache, bt.to(dev), lens, 1.0, with_lse=True)
+    check(got, q, [kv], 1.0, dtype)
