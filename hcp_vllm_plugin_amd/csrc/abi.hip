@@ -1749,6 +1749,8 @@ int hcp_step_tables(const hcp_step_tables_args* a, void* stream) {
   // (the kernel sums table entries in 32 bits)
   if (a->table_width >= (int64_t{1} << 32) / HCP_STEP_MAX_SEQS || a->num_tokens > INT32_MAX)
     return fail(HCP_EUNSUPPORTED, "%s: too many tokens or table entries", who);
+  if (a->num_seqs > 1 && a->table_stride < a->table_width)
+    return fail(HCP_EINVAL, "%s: the rows of the block table overlap", who);
   if (!a->query_start_loc || !a->blocks_used ||
       (a->num_seqs > 0 && (!a->ctx_lens || !a->new_lens || !a->seq_lens)) ||
       (a->num_seqs > 0 && a->table_width > 0 && !a->block_table) ||

@@ -40,6 +40,15 @@ def _rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype,
     return at, tok, head
 
 
+def _out_rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype,
+              index: int) -> tuple[int, int, int]:
+    """``_rows`` of a tensor that is written: its rows are apart."""
+    at, tok, head = _rows(name, t, shape, dtype, index)
+    if (shape[0] > 1 and not tok) or (shape[1] > 1 and not head):
+        raise ValueError(f"{name}: rows on top of each other")
+    return at, tok, head
+
+
 def _weight(t: torch.Tensor, d: int, dtype: torch.dtype, index: int) -> tuple[int, torch.dtype]:
     at, wd = t.data_ptr(), t.dtype
     if t.shape != (d,) or not t.is_contiguous() or at & 15 or t.get_device() != index or \
@@ -120,8 +129,6 @@ def qk_norm_rope(
     if kv_cache is None:
         if value is not None or slot_mapping is not None:
             raise ValueError("value and slot_mapping go with a kv_cache")
-        if key_out is None:
-            key_out = torch.empty(kv_shape, dtype=dt, device=query.device)
     else:
         if value is None or slot_mapping is None:
             raise ValueError("a cache write needs value and slot_mapping")
@@ -146,10 +153,13 @@ def qk_norm_rope(
         query_out = torch.empty((t, h, d), dtype=dt, device=query.device)
         qo, qo_tok, qo_head = query_out.data_ptr(), h * d, d
     else:
-        qo, qo_tok, qo_head = _rows("query_out", query_out, (t, h, d), dt, index)
+        qo, qo_tok, qo_head = _out_rows("query_out", query_out, (t, h, d), dt, index)
     ko = ko_tok = ko_head = 0
-    if key_out is not None:
-        ko, ko_tok, ko_head = _rows("key_out", key_out, kv_shape, dt, index)
+    if key_out is None and not kind:
+        key_out = torch.empty(kv_shape, dtype=dt, device=query.device)
+        ko, ko_tok, ko_head = key_out.data_ptr(), hkv * d, d
+    elif key_out is not None:
+        ko, ko_tok, ko_head = _out_rows("key_out", key_out, kv_shape, dt, index)
     _lib.launch(_lib.lib().hcp_qk_norm_rope, _lib.pack_qk_rope(
         q, q_tok, q_head, k, k_tok, k_head, v, v_tok, v_head, qo, qo_tok, qo_head, ko, ko_tok,
         ko_head, wq, wk, positions.data_ptr(), tab_at, tab_row, most, slots_at, num_slots, cache,

@@ -52,7 +52,7 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 of two dimensions")
     (rows, width), (row, col) = block_table.shape, block_table.stride()
-    if rows < n or (width > 1 and col != 1):
+    if rows < n or (width > 1 and col != 1) or (n > 1 and row < width):
         raise ValueError("block_table must have contiguous rows, one for each request")
     if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be contiguous int32 of one dimension")

@@ -983,8 +983,9 @@ def decode_fp4(
     if out is None:
         out = torch.empty((s, h, d), dtype=dt, device=q.device)
     elif out.shape != q.shape or out.dtype != dt or out.stride(2) != 1 or \
-            out.get_device() != index:
-        raise ValueError("out must be as q, with contiguous head_dim")
+            out.get_device() != index or (s > 1 and not out.stride(0)) or \
+            (h > 1 and not out.stride(1)):
+        raise ValueError("out must be as q, with contiguous head_dim and its rows apart")
     lse = torch.empty((h, s), dtype=torch.float32, device=q.device) if with_lse else None
     out_at, (o_tok, o_head, _), lse_at = out.data_ptr(), out.stride(), \
         lse.data_ptr() if with_lse else 0

@@ -807,7 +807,8 @@ int hcp_qk_norm_rope(const hcp_qk_rope_args* args, void* stream);
  * requests' order; its new tokens are at positions ctx .. ctx + new - 1.
  *   ctx_lens, new_lens   DEVICE [num_seqs], HCP_DTYPE_I32 or I64; counted as 0
  *                        below 0 and as 2^30 past that
- *   block_table          DEVICE int32, num_seqs rows of table_width ids; updated
+ *   block_table          DEVICE int32, num_seqs rows of table_width ids, table_stride
+ *                        (>= table_width) apart; updated
  *   free_blocks          DEVICE int32 [num_free]
  *   query_start_loc [num_seqs + 1], seq_lens [num_seqs], blocks_used [1]  DEVICE int32
  *   positions, slot_mapping [num_tokens]  DEVICE int64; rows past the new tokens get

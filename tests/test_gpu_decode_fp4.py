@@ -291,3 +291,12 @@ def test_scores_that_rise_and_fall(dev, dtype, d, slope):
     lens = torch.tensor([n], dtype=torch.int32, device=dev)
     got = decode_fp4(q.to(dev), cache, bt.to(dev), lens, 1.0, with_lse=True)
     check(got, q, [kv], 1.0, dtype)
+
+
+def test_rows_of_out_on_top_of_each_other_are_refused(dev):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=dev)
+    cache = torch.zeros(fp4_cache_shape(2, 2, 16, 64), dtype=torch.uint8, device=dev)
+    bt, lens = torch.zeros(2, 1, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int64, device=dev)
+    for out in (q[:1].expand(2, 4, 64), q[:, :1].expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="out"):
+            decode_fp4(q, cache, bt, lens, 0.1, out=out)

@@ -194,3 +194,14 @@ def test_captured_and_replayed(dev):
         eq, _ = qk_norm_rope(q, k, pos, table, **kw)
         torch.cuda.synchronize()
         assert torch.equal(gq, eq) and torch.equal(first, cache) and first.any()
+
+
+def test_outputs_on_top_of_each_other_are_refused(dev):
+    q, k = (torch.zeros(3, h, 64, dtype=torch.bfloat16, device=dev) for h in (4, 2))
+    pos, table = torch.zeros(3, dtype=torch.int64, device=dev), torch.zeros(4, 64, device=dev)
+    for kw in ({"query_out": q[:1].expand(3, 4, 64)}, {"query_out": q[:, :1].expand(3, 4, 64)},
+               {"key_out": k[:1].expand(3, 2, 64)}, {"key_out": k[:, :1].expand(3, 2, 64)}):
+        with pytest.raises(ValueError, match="on top"):
+            qk_norm_rope(q, k, pos, table, **kw)
+    one = qk_norm_rope(q[:1], k[:1], pos[:1], table, query_out=q[:1], key_out=k[:1])
+    assert one[0].shape == (1, 4, 64)

@@ -298,3 +298,17 @@ def test_python_refuses():
         HcpRingAttentionImpl(4, 80, 0.1, 2, kv_cache_dtype="fp4")
     with pytest.raises(NotImplementedError):
         HcpRingAttentionImpl(4, 64, 0.1, 2, kv_cache_dtype="fp8")
+
+
+def test_overlapping_table_rows_are_refused(L):
+    lens, free = torch.tensor([3, 4]), torch.zeros(2, dtype=torch.int32)
+    for bt in (torch.zeros(1, 3, dtype=torch.int32).expand(2, 3),
+               torch.zeros(8, dtype=torch.int32).as_strided((2, 3), (2, 1))):
+        with pytest.raises(ValueError, match="rows"):
+            build_step_tables(lens, lens, bt, free, 16, 4)
+    a = _lib.StepTablesArgs()
+    for f in ("ctx_lens", "new_lens", "block_table", "query_start_loc", "seq_lens", "blocks_used"):
+        setattr(a, f, 0x10000)
+    a.table_stride, a.table_width, a.num_seqs, a.block_size = 7, 8, 2, 16
+    a.ctx_dtype = a.new_dtype = _lib.DTYPE_I32
+    assert L.hcp_step_tables(ctypes.addressof(a), None) == _lib.HCP_EINVAL
