@@ -359,6 +359,7 @@ def packer(cls):
 pack_qk_rope = packer(QkRopeArgs)
 pack_step_tables = packer(StepTablesArgs)
 pack_decode_paged = packer(DecodePagedArgs)
+pack_fp4_cache = packer(Fp4CacheDesc)
 
 # include/hcp_mi355x.h HCP_DECODE_PAGED_MAX_SEQS
 DECODE_PAGED_MAX_SEQS = 1024
@@ -551,6 +552,12 @@ class SplitLimits(NamedTuple):
     max_workspace: int
 
 
+@functools.lru_cache(maxsize=1024)
+def decode_fp4_workspace(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """``hcp_decode_fp4_workspace``, asked once for a size."""
+    return lib().hcp_decode_fp4_workspace(num_seqs, num_heads, num_kv_heads, head_dim)
+
+
 @functools.lru_cache(maxsize=None)  # one entry per head_dim
 def split_limits(head_dim: int) -> SplitLimits:
     if not 0 < head_dim <= 256:  # refused by the launch: nothing to cut
@@ -601,13 +608,13 @@ def on_device(device: torch.device):
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def launch(entry, args: bytes, index: int, what: str) -> None:
-    """One entry point with its packed arguments on torch's current stream of GPU
-    ``index``, errors raised."""
+def launch(entry, index: int, what: str, *args) -> None:
+    """One entry point with its arguments (a packed block, or each) on torch's
+    current stream of GPU ``index``, errors raised."""
     if index == _get_device() and _raw_stream is not None:
-        rc = entry(args, _raw_stream(index))
+        rc = entry(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = entry(args, torch.cuda.current_stream(index).cuda_stream)
+            rc = entry(*args, torch.cuda.current_stream(index).cuda_stream)
     if rc < 0:
         check(rc, what)

@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .varlen import PagedCache, fp4_desc
+from .varlen import PagedCache, fp4_fields
 
 __all__ = ["reshape_and_cache", "fp4_cache_shape", "gather_kv"]
 
@@ -68,6 +68,7 @@ def fp4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int,
 
 
 _INDEX_CODES = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
+_TYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
 def check_slots(slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> torch.Tensor:
@@ -82,31 +83,28 @@ def check_slots(slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> torch.Ten
 
 def _write_fp4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
                slot_mapping: torch.Tensor) -> None:
-    desc, hkv, d = fp4_desc(kv_cache)
-    n, shape, dt, dev = slot_mapping.shape[0], key.shape, key.dtype, kv_cache.device
+    cache, hkv, d = fp4_fields(kv_cache)
+    n, shape, dt, index = slot_mapping.shape[0], key.shape, key.dtype, kv_cache.get_device()
     if shape != value.shape or len(shape) != 3:
         raise ValueError("key/value must be [N, Hkv, D] of one shape")
     if shape[0] < n:
         raise ValueError(f"{n} slots for {shape[0]} key rows")
     if shape[1] != hkv or shape[2] != d:
         raise ValueError("key/value heads or head_dim do not match the cache")
-    if (dt != torch.bfloat16 and dt != torch.float16) or value.dtype != dt:
+    code = _TYPES.get(dt)
+    if code is None or value.dtype != dt:
         raise ValueError("key/value must both be float16 or bfloat16")
     (k_tok, k_head, k_col), (v_tok, v_head, v_col) = key.stride(), value.stride()
     if k_col != 1 or v_col != 1:
         raise ValueError("key/value head_dim must be contiguous")
     slots = check_slots(slot_mapping, kv_cache)
-    index = dev.index
     if key.get_device() != index or value.get_device() != index:
         raise ValueError("key/value must be on the cache's GPU")
     if n == 0:
         return
-    with _lib.on_device(dev):
-        rc = _lib.lib().hcp_fp4_write(
-            key.data_ptr(), k_tok, k_head, value.data_ptr(), v_tok, v_head, slots.data_ptr(),
-            _INDEX_CODES[slots.dtype], n, hkv, ctypes.addressof(desc), _lib.dtype_code(dt),
-            _lib.stream_ptr(dev))
-    _lib.check(rc, "hcp_fp4_write")
+    _lib.launch(_lib.lib().hcp_fp4_write, index, "hcp_fp4_write", key.data_ptr(), k_tok, k_head,
+                value.data_ptr(), v_tok, v_head, slots.data_ptr(), _INDEX_CODES[slots.dtype], n,
+                hkv, _lib.pack_fp4_cache(*cache), code)
 
 
 def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -114,18 +112,17 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     """K and V ``[n, Hkv, D]`` that a 4-bit cache stands for at ``slot_mapping``,
     in the 16-bit ``dtype`` they were written in (exactly: a code's value has two
     significant bits).  A slot that is negative or past the cache reads as zeros."""
-    if dtype != torch.bfloat16 and dtype != torch.float16:
+    code = _TYPES.get(dtype)
+    if code is None:
         raise ValueError("dtype must be float16 or bfloat16")
-    desc, hkv, d = fp4_desc(kv_cache)
-    slots, dev = check_slots(slot_mapping, kv_cache), kv_cache.device
-    n = slots.shape[0]
-    kv = torch.empty((2, n, hkv, d), dtype=dtype, device=dev)
+    cache, hkv, d = fp4_fields(kv_cache)
+    slots = check_slots(slot_mapping, kv_cache)
+    n, index = slots.shape[0], slots.get_device()
+    kv = torch.empty(2, n, hkv, d, dtype=dtype, device=kv_cache.device)
     base = kv.data_ptr()
-    with _lib.on_device(dev):
-        rc = _lib.lib().hcp_fp4_read(
-            slots.data_ptr(), _INDEX_CODES[slots.dtype], n, hkv, ctypes.addressof(desc),
-            _lib.dtype_code(dtype), base, base + 2 * n * hkv * d, _lib.stream_ptr(dev))
-    _lib.check(rc, "hcp_fp4_read")
+    _lib.launch(_lib.lib().hcp_fp4_read, index, "hcp_fp4_read", slots.data_ptr(),
+                _INDEX_CODES[slots.dtype], n, hkv, _lib.pack_fp4_cache(*cache), code, base,
+                base + 2 * n * hkv * d)
     return kv.unbind(0)
 
 

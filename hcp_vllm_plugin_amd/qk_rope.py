@@ -150,20 +150,19 @@ def qk_norm_rope(
         if c_hkv != hkv or c_d != d:
             raise ValueError("key heads or head_dim do not match the cache")
     if query_out is None:
-        query_out = torch.empty((t, h, d), dtype=dt, device=query.device)
+        query_out = torch.empty(t, h, d, dtype=dt, device=query.device)
         qo, qo_tok, qo_head = query_out.data_ptr(), h * d, d
     else:
         qo, qo_tok, qo_head = _out_rows("query_out", query_out, (t, h, d), dt, index)
     ko = ko_tok = ko_head = 0
     if key_out is None and not kind:
-        key_out = torch.empty(kv_shape, dtype=dt, device=query.device)
+        key_out = torch.empty(t, hkv, d, dtype=dt, device=query.device)
         ko, ko_tok, ko_head = key_out.data_ptr(), hkv * d, d
     elif key_out is not None:
         ko, ko_tok, ko_head = _out_rows("key_out", key_out, kv_shape, dt, index)
-    _lib.launch(_lib.lib().hcp_qk_norm_rope, _lib.pack_qk_rope(
+    _lib.launch(_lib.lib().hcp_qk_norm_rope, index, "hcp_qk_norm_rope", _lib.pack_qk_rope(
         q, q_tok, q_head, k, k_tok, k_head, v, v_tok, v_head, qo, qo_tok, qo_head, ko, ko_tok,
         ko_head, wq, wk, positions.data_ptr(), tab_at, tab_row, most, slots_at, num_slots, cache,
         fp4, t, eps, h, hkv, d, rot, code, code if w_type == dt else _lib.DTYPE_F32,
-        _lib.DTYPE_F32 if wide_table else code, pos_code, slot_code, bool(interleaved), kind, 0),
-        index, "hcp_qk_norm_rope")
+        _lib.DTYPE_F32 if wide_table else code, pos_code, slot_code, bool(interleaved), kind, 0))
     return query_out, key_out

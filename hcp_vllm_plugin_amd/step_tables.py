@@ -64,13 +64,13 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
     ints = torch.empty(2 * n + 2, dtype=torch.int32, device=block_table.device)
-    wide = torch.empty((2, num_tokens), dtype=torch.int64, device=block_table.device)
+    wide = torch.empty(2, num_tokens, dtype=torch.int64, device=block_table.device)
     at, wide_at = ints.data_ptr(), wide.data_ptr()
-    _lib.launch(_lib.lib().hcp_step_tables, _lib.pack_step_tables(
+    _lib.launch(_lib.lib().hcp_step_tables, index, "hcp_step_tables", _lib.pack_step_tables(
         ctx_lens.data_ptr(), new_lens.data_ptr(), ctx_lens.stride(0), new_lens.stride(0),
         block_table.data_ptr(), row, width, free_blocks.data_ptr(), free_blocks.shape[0],
         num_tokens, at, at + 4 * (n + 1), at + 4 * (2 * n + 1), wide_at, wide_at + 8 * num_tokens,
-        ctx_code, new_code, n, block_size), index, "hcp_step_tables")
+        ctx_code, new_code, n, block_size))
     starts, lens, used = ints.split_with_sizes((n + 1, n, 1))
     positions, slots = wide.unbind(0)
     return StepTables(starts, lens, positions, slots, used)

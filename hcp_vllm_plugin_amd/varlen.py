@@ -97,8 +97,8 @@ class PagedCache:
         raise ValueError(f"unrecognised paged cache shape {tuple(cache.shape)}")
 
 
-def fp4_desc(cache: torch.Tensor) -> tuple["_lib.Fp4CacheDesc", int, int]:
-    """(descriptor, KV heads, head_dim) of a 4-bit cache."""
+def fp4_fields(cache: torch.Tensor) -> tuple[tuple, int, int]:
+    """(the fields of ``_lib.Fp4CacheDesc``, KV heads, head_dim) of a 4-bit cache."""
     shape, stride = cache.shape, cache.stride()
     if cache.dtype != torch.uint8 or len(shape) != 4 or shape[3] == 0 or shape[3] % 34 or \
             stride[3] != 1 or stride[2] != shape[3]:
@@ -106,7 +106,13 @@ def fp4_desc(cache: torch.Tensor) -> tuple["_lib.Fp4CacheDesc", int, int]:
                          "block and head contiguous")
     nb, hkv, bs, row = shape
     d = row // 17 * 16
-    return _lib.Fp4CacheDesc(cache.data_ptr(), stride[0], stride[1], nb, bs, d), hkv, d
+    return (cache.data_ptr(), stride[0], stride[1], nb, bs, d), hkv, d
+
+
+def fp4_desc(cache: torch.Tensor) -> tuple["_lib.Fp4CacheDesc", int, int]:
+    """(descriptor, KV heads, head_dim) of a 4-bit cache."""
+    fields, hkv, d = fp4_fields(cache)
+    return _lib.Fp4CacheDesc(*fields), hkv, d
 
 
 def segment_contiguous(k: torch.Tensor, v: torch.Tensor, start: int = 0,
@@ -885,9 +891,8 @@ class PagedDecode:
         a.lens_dtype = _lib.DTYPE_I64 if seq_lens.dtype == torch.int64 else _lib.DTYPE_I32
         a.num_seqs, a.window = n, int(window or 0)
         a.num_heads, a.num_kv_heads, a.head_dim = num_heads, pc.num_kv_heads, pc.head_dim
-        L = _lib.lib()
         self._fp4 = pc.layout == "fp4"
-        size = L.hcp_decode_fp4_workspace if self._fp4 else L.hcp_decode_paged_workspace
+        size = _lib.decode_fp4_workspace if self._fp4 else _lib.lib().hcp_decode_paged_workspace
         a.workspace_bytes = size(n, num_heads, pc.num_kv_heads, pc.head_dim)
         if starts is not None:
             if starts.dtype != seq_lens.dtype or starts.shape != seq_lens.shape or \
@@ -955,7 +960,7 @@ def decode_fp4(
     dt, index = q.dtype, q.get_device()
     if q.dim() != 3 or (dt != torch.bfloat16 and dt != torch.float16) or q.stride(2) != 1:
         raise ValueError("q must be float16/bfloat16 [S, H, D] with contiguous head_dim")
-    desc, hkv, dim = fp4_desc(kv_cache)
+    (cache_at, c_block, c_head, blocks, bs, dim), hkv, _ = fp4_fields(kv_cache)
     s, h, d = q.shape
     if d != dim or not hkv or h % hkv:
         raise ValueError("kv_cache must be a 4-bit cache of q's head_dim, its heads dividing q's")
@@ -981,31 +986,31 @@ def decode_fp4(
         q = q.contiguous()
         q_at, (q_tok, q_head, _) = q.data_ptr(), q.stride()
     if out is None:
-        out = torch.empty((s, h, d), dtype=dt, device=q.device)
+        out = torch.empty(s, h, d, dtype=dt, device=q.device)
     elif out.shape != q.shape or out.dtype != dt or out.stride(2) != 1 or \
             out.get_device() != index or (s > 1 and not out.stride(0)) or \
             (h > 1 and not out.stride(1)):
         raise ValueError("out must be as q, with contiguous head_dim and its rows apart")
-    lse = torch.empty((h, s), dtype=torch.float32, device=q.device) if with_lse else None
+    lse = torch.empty(h, s, dtype=torch.float32, device=q.device) if with_lse else None
     out_at, (o_tok, o_head, _), lse_at = out.data_ptr(), out.stride(), \
         lse.data_ptr() if with_lse else 0
     bt_at, lens_at, starts_at = block_table.data_ptr(), seq_lens.data_ptr(), \
         0 if starts is None else starts.data_ptr()
-    L, wide = _lib.lib(), 8 if lens_code == _lib.DTYPE_I64 else 4
+    wide = 8 if lens_code == _lib.DTYPE_I64 else 4
     # (a launch's keys are counted in 32-key chunks, in 32 bits)
-    most = max(1, min(_lib.DECODE_PAGED_MAX_SEQS, (1 << 34) // max(1, width * desc.block_size)))
+    most = max(1, min(_lib.DECODE_PAGED_MAX_SEQS, (1 << 34) // max(1, width * bs)))
     for r in range(0, s, most):
         n = min(s - r, most)
         # fp32 partials: stream-ordered scratch from torch's caching allocator
-        size = L.hcp_decode_fp4_workspace(n, h, hkv, d)
+        size = _lib.decode_fp4_workspace(n, h, hkv, d)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _lib.launch(L.hcp_decode_fp4, _lib.pack_decode_paged(
-            q_at + 2 * r * q_tok, q_tok, q_head, desc.addr, 0, bt_at + 4 * r * bt_row, 0,
-            desc.stride_head, desc.stride_block, 0, 0, desc.block_size, desc.num_blocks, bt_row,
-            width, lens_at + wide * r, ws.data_ptr(), size, out_at + 2 * r * o_tok, o_tok, o_head,
-            lse_at and lse_at + 4 * r, s, lens_code, n, min(window or 0, 0x7fffffff), h, hkv, d,
+        _lib.launch(_lib.lib().hcp_decode_fp4, index, "hcp_decode_fp4", _lib.pack_decode_paged(
+            q_at + 2 * r * q_tok, q_tok, q_head, cache_at, 0, bt_at + 4 * r * bt_row, 0, c_head,
+            c_block, 0, 0, bs, blocks, bt_row, width, lens_at + wide * r, ws.data_ptr(), size,
+            out_at + 2 * r * o_tok, o_tok, o_head, lse_at and lse_at + 4 * r, s, lens_code, n,
+            min(window or 0, 0x7fffffff), h, hkv, d,
             _lib.DTYPE_BF16 if dt == torch.bfloat16 else _lib.DTYPE_F16, keep_nan, scale,
-            starts_at and starts_at + wide * r), index, "hcp_decode_fp4")
+            starts_at and starts_at + wide * r))
     return (out, lse) if with_lse else out
 
 
