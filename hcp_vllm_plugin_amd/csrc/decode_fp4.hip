@@ -21,7 +21,7 @@
 // lie on multiples of 32 positions, so that 16 keys never cross a block), each
 // through LDS of its own, where the next chunk lands while one is computed (held
 // in registers instead, two chunks take 212 of them at 128 columns and spill at
-// 256: 364 us for 32 x 4k-16k keys of 16 / 8 x 256, now 137; 14 / 2 x 64, 64 x
+// 256: 364 us for 32 x 4k-16k keys of 16 / 8 x 256, then 137; 14 / 2 x 64, 64 x
 // 16k-32k 64 -> 51 us).  The waves are combined through LDS; decode_reduce_kernel
 // merges a sequence's partials.
 //
@@ -132,11 +132,39 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
   // are not stored.
   const int vb = bs * (dv / 2), ng = dv / 32;
   int koff[Tile::P], voff[Tile::P];  // (D 64: one load, K in the lower lanes, V in the upper)
+  // where in a tile a lane finds its K codes, K scale (a byte), V codes and V scales
+  // (a dword: four keys)
+  int kc_at[Tile::P], vc_at[Tile::P];
 #pragma unroll
   for (int i = 0; i < Tile::P; ++i) {
-    const int l = lane & 31;
-    const int key = D == 64 ? l >> 1 : c16, d0 = D == 64 ? 32 * (l & 1) : D / 4 * g4 + 32 * i;
-    const int quad = D == 64 ? l >> 3 : g4, oct = D == 64 ? l & 7 : NU * c16 / 8 + i;
+    int key = c16, d0 = D / 4 * g4, quad = g4, oct = NU * c16 / 8;
+    kc_at[i] = lane * 16;
+    vc_at[i] = Tile::P * 1024 + lane * 16;
+    if constexpr (D == 64) {
+      const int l = lane & 31;
+      key = l >> 1;
+      d0 = 32 * (l & 1);
+      quad = l >> 3;
+      oct = l & 7;
+      kc_at[i] = c16 * 32 + g4 * 8;
+      vc_at[i] = 512 + g4 * 128 + (c16 >> 1) * 16;
+    } else if constexpr (D == 256) {
+      // A lane takes two pieces in a row of either, but what a load fetches lies in a
+      // row too: keys 8 i .. of K, quads 2 i and 2 i + 1 of V, four lanes the 64 bytes
+      // of four pieces (with every other piece of 2 KB in a load, 64 x 16k keys of
+      // 16 / 8 heads took 418 us, now 368).  The order of the four in LDS spreads the
+      // reads of 16 lanes over all banks for V, over half of them for K (over all of
+      // them, K's 64 bytes in another order: 369).
+      const int q = lane >> 2, r = lane & 3, e = c16 >> 1;
+      key = 8 * i + (q >> 1);
+      d0 = 128 * (q & 1) + 32 * (r ^ (key >> 1 & 3));
+      quad = 2 * i + (q >> 3);
+      oct = 4 * (q & 7) + (r ^ (q >> 2 & 1));
+      kc_at[i] = (c16 >> 3) * 1024 + ((c16 & 7) * 2 + (g4 >> 1)) * 64 +
+                 ((2 * (g4 & 1) + i) ^ (c16 >> 1 & 3)) * 16;
+      vc_at[i] = 2048 + (g4 >> 1) * 1024 + ((g4 & 1) * 8 + e) * 64 +
+                 ((2 * (c16 & 1) + i) ^ (e >> 2)) * 16;
+    }
     koff[i] = key * (dv / 2) + (d0 < dv ? d0 / 2 : 0);
     voff[i] = vb + (quad * (dv / 8) + (oct < dv / 8 ? oct : 0)) * 16;
     if (D == 64 && lane >= 32) koff[i] = voff[i];
@@ -176,10 +204,6 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
           off * ng, 0, 2);
     }
   };
-  // where in a tile a lane finds its K codes, K scale (a byte), V codes and V scales
-  // (a dword: four keys)
-  const int kc_at = D == 64 ? c16 * 32 + g4 * 8 : lane * 16;
-  const int vc_at = D == 64 ? 512 + g4 * 128 + (c16 >> 1) * 16 : Tile::P * 1024 + lane * 16;
   int ks_at[Tile::P];
 #pragma unroll
   for (int i = 0; i < Tile::P; ++i) {
@@ -214,12 +238,12 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
         const float ks =
             __uint_as_float(static_cast<uint32_t>(lds_at<uint8_t>(tile + ks_at[i])) << 23);
         if constexpr (D == 64) {
-          const u32x2 w = lds_at<u32x2>(tile + kc_at);
+          const u32x2 w = lds_at<u32x2>(tile + kc_at[0]);
 #pragma unroll
           for (int q = 0; q < 2; ++q)
             s[t] = E::mfma16(as_vec8<V8>(fp4_values<T>(w[q], ks)), qf[q], s[t]);
         } else {
-          const u32x4 w = lds_at<u32x4>(tile + i * 1024 + kc_at);
+          const u32x4 w = lds_at<u32x4>(tile + kc_at[i]);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             s[t] = E::mfma16(as_vec8<V8>(fp4_values<T>(w[q], ks)), qf[4 * i + q], s[t]);
@@ -292,7 +316,7 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < Tile::P; ++i)
-        vw[t][i] = lds_at<u32x4>(src + t * Tile::BYTES + i * 1024 + vc_at);
+        vw[t][i] = lds_at<u32x4>(src + t * Tile::BYTES + vc_at[i]);
     if constexpr (D == 64) {
       // a lane's two of the four bytes, of two keys in one dword
 #pragma unroll
