@@ -608,6 +608,18 @@ def on_device(device: torch.device):
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
+                     torch.cuda.is_current_stream_capturing)
+
+
+def capturing(index: int) -> bool:
+    """Whether torch's current stream of GPU ``index`` is being captured."""
+    if index == _get_device():
+        return _capturing()
+    with torch.cuda.device(index):
+        return _capturing()
+
+
 def launch(entry, index: int, what: str, *args) -> None:
     """One entry point with its arguments (a packed block, or each) on torch's
     current stream of GPU ``index``, errors raised."""

@@ -67,6 +67,7 @@ from .kv_cache import reshape_and_cache
 from .merge import merge_attn_states
 from .ring_attn import COPY_STATS, ring_attn_with_lse
 from .ring_decode import GrowthBuffer, growth_assignee, local_partial, ring_decode_step
+from .step_tables import written_unseen
 from .varlen import (
     _MIN_PAGED_BLOCK,
     ENTRY_DTYPE,
@@ -331,13 +332,27 @@ class _Step:
     table as contiguous int32, its lengths on the device as the host saw them
     (``lens``, None where the copy took the general path) and the plans made
     from them (``fast``).  A layer keeps the record it got, so another thread's
-    step can neither take the plans away under it nor be given them."""
+    step can neither take the plans away under it nor be given them.  ``names``:
+    the layers that have run, where that is what tells one step from the next."""
 
-    __slots__ = ("meta", "stamp", "host", "bt", "lens", "owner", "fast")
+    __slots__ = ("meta", "stamp", "host", "bt", "lens", "owner", "fast", "names")
 
     def __init__(self, meta, stamp, host, bt, lens, owner):
         self.meta, self.stamp, self.host, self.bt = meta, stamp, host, bt
-        self.lens, self.owner, self.fast = lens, owner, {}
+        self.lens, self.owner, self.fast, self.names = lens, owner, {}, set()
+
+    def serves(self, layer_name: str) -> bool:
+        """Whether this may still be the step of ``layer_name``'s call, the metadata
+        object and its stamp being the same: metadata that ``build_step_tables`` writes
+        with no trace on the host is another step's when a layer comes again."""
+        meta = self.meta
+        if not written_unseen(meta.query_start_loc, meta.seq_lens, meta.block_table) or \
+                _capturing():
+            return True
+        if not layer_name or layer_name in self.names:
+            return False
+        self.names.add(layer_name)
+        return True
 
     def lens_on(self, stream: int, device: torch.device, given: torch.Tensor):
         """The lengths for launches on ``stream`` that read them on the device,
@@ -378,7 +393,8 @@ def _meta_stamp(attn_metadata) -> tuple:
     tensor the forward reads.  A caller that keeps one metadata object and
     refills its tensors in place between steps through torch's in-place ops
     bumps the version counters, so the next step does not reuse the previous
-    step's host copy or plans.  (vLLM builds a new metadata object every
+    step's host copy or plans; ``build_step_tables`` bumps its table's, and what it
+    writes unseen is told by the layers (``_Step.serves``).  (vLLM builds a new metadata object every
     step; tensors made under inference mode keep no version counter, and a
     caller that refills such tensors in one reused object calls
     ``invalidate_step_cache`` between steps.)"""
@@ -402,12 +418,13 @@ def _host_metadata(attn_metadata):
     return st.host, st.bt
 
 
-def _step(attn_metadata, queue=None) -> _Step:
+def _step(attn_metadata, queue=None, layer_name: str = "") -> _Step:
     """This step's record.  ``queue``: called, when the metadata is not on the
     host yet, between queueing its copy and waiting for it."""
     stamp = _meta_stamp(attn_metadata)
     st = _STEP["step"]
-    if st is not None and st.meta is attn_metadata and st.stamp == stamp:
+    if st is not None and st.meta is attn_metadata and st.stamp == stamp and \
+            st.serves(layer_name):
         return st
     block_table = attn_metadata.block_table
     if block_table.dtype != torch.int32:
@@ -429,6 +446,7 @@ def _step(attn_metadata, queue=None) -> _Step:
                             fb.reshape(-1).to(torch.int64)]).tolist()
         host = (packed[:n + 1], packed[n + 1:2 * n + 1], packed[2 * n + 1:])
     st = _Step(attn_metadata, stamp, host, block_table, lens, owner)
+    st.names.add(layer_name)
     _STEP.update(step=st, fast=st.fast)
     return st
 
@@ -976,10 +994,10 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
                 not (DECODE_RING_MAP and _decode_ring_enabled()):
             ahead = _Ahead(self, query, out, attn_metadata, pc)
         # small metadata tensors: one host sync per step (see _step)
-        step = _step(attn_metadata, ahead)
+        layer_name = getattr(layer, "layer_name", "")
+        step = _step(attn_metadata, ahead, layer_name)
         (qsl, seq_lens, first_blocks), block_table = step.host, step.bt
         BATCH_STATS["max_reqs"] = max(BATCH_STATS["max_reqs"], len(seq_lens))
-        layer_name = getattr(layer, "layer_name", "")
         n = len(seq_lens)
         if len(first_blocks) < n and qsl[n] > qsl[len(first_blocks)]:
             raise ValueError("the block table has no row for a request")

@@ -20,6 +20,15 @@ __all__ = ["StepTables", "build_step_tables"]
 
 _INDEX = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
+# Storages that are written where no version counter tells: by every replay of a
+# captured call, or as a table made under inference mode.
+_UNSEEN: set[int] = set()
+
+
+def written_unseen(*tensors: torch.Tensor) -> bool:
+    """Whether ``build_step_tables`` writes one of these without a trace on the host."""
+    return bool(_UNSEEN) and any(t.untyped_storage().data_ptr() in _UNSEEN for t in tensors)
+
 
 class StepTables(NamedTuple):
     query_start_loc: torch.Tensor  # int32 [n + 1]
@@ -27,6 +36,16 @@ class StepTables(NamedTuple):
     positions: torch.Tensor        # int64 [num_tokens]
     slot_mapping: torch.Tensor     # int64 [num_tokens]
     blocks_used: torch.Tensor      # int32 [1]
+
+
+def _note_written(block_table: torch.Tensor, ints: torch.Tensor, index: int) -> None:
+    """Who caches what a table says goes by its version counter (``ring_backend._step``)."""
+    torch._C._increment_version((block_table,))  # (nothing under inference mode)
+    if _lib.capturing(index):
+        _UNSEEN.add(ints.untyped_storage().data_ptr())
+        _UNSEEN.add(block_table.untyped_storage().data_ptr())
+    elif block_table.is_inference():
+        _UNSEEN.add(block_table.untyped_storage().data_ptr())
 
 
 def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -44,7 +63,12 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     table row can name get slot -1 too, and take no block.
 
     ``positions`` and ``slot_mapping`` have ``num_tokens`` rows: the new tokens,
-    then (padding) position 0 and slot -1.  Lengths below 0 count as 0."""
+    then (padding) position 0 and slot -1.  Lengths below 0 count as 0.
+
+    A captured call writes the same tensors at every replay.  ``forward`` outside
+    the graph reads them anew for a new metadata object, or when a layer comes again
+    with a kept one; a caller whose next step begins with a layer that the last one
+    left out calls ``ring_backend.invalidate_step_cache`` in between."""
     index, ints_of = block_table.get_device(), _INDEX.get
     ctx_code, new_code, (n, *more) = ints_of(ctx_lens.dtype), ints_of(new_lens.dtype), ctx_lens.shape
     if more or ctx_code is None or new_code is None or new_lens.shape != (n,):
@@ -71,6 +95,7 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
         block_table.data_ptr(), row, width, free_blocks.data_ptr(), free_blocks.shape[0],
         num_tokens, at, at + 4 * (n + 1), at + 4 * (2 * n + 1), wide_at, wide_at + 8 * num_tokens,
         ctx_code, new_code, n, block_size))
+    _note_written(block_table, ints, index)
     starts, lens, used = ints.split_with_sizes((n + 1, n, 1))
     positions, slots = wide.unbind(0)
     return StepTables(starts, lens, positions, slots, used)

@@ -1,10 +1,13 @@
 """GPU: a step's block table, slots and positions (``build_step_tables``), equal to the
 same made on the host."""
 
+import types
+
 import pytest
 import torch
 
 from hcp_vllm_plugin_amd import build_step_tables
+from hcp_vllm_plugin_amd import ring_backend as rb
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +132,67 @@ def test_captured_and_replayed(dev):
         table.fill_(step)
         again = build_step_tables(ctx, new, table, free, 16, 256)
         assert all(torch.equal(a, b) for a, b in zip(first, (*again, table)))
+
+
+class _Forward:
+    """One request's attention over a 16-bit cache with the metadata object that its caller
+    keeps from step to step."""
+
+    def __init__(self, dev, rows, lens, starts, table):
+        gen = torch.Generator().manual_seed(3)
+        rb.invalidate_step_cache()
+        self.impl = rb.HcpRingAttentionImpl(4, 64, 0.125, 2)
+        self.layers = [types.SimpleNamespace(layer_name=f"layer{i}") for i in range(2)]
+        self.cache = torch.randn(8, 2, 16, 128, generator=gen).to(dev, torch.bfloat16)
+        self.q = torch.randn(rows, 4, 64, generator=gen).to(dev, torch.bfloat16)
+        self.meta = types.SimpleNamespace(num_actual_tokens=rows, query_start_loc=starts,
+                                          seq_lens=lens, block_table=table)
+
+    def run(self, meta=None):
+        return [self.impl.forward(layer, self.q, None, None, self.cache, meta or self.meta,
+                                  torch.zeros_like(self.q)) for layer in self.layers]
+
+    def check(self):
+        """The kept object's result is that of an object that no step has seen."""
+        got = self.run()
+        want = self.run(types.SimpleNamespace(**vars(self.meta)))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        rb.invalidate_step_cache()
+        assert all(torch.equal(a, b) for a, b in zip(got, self.run()))
+        return got
+
+
+@pytest.mark.parametrize("inference", [False, True])
+@pytest.mark.parametrize("new", [1, 4])
+def test_forward_sees_the_table_that_a_call_has_written(dev, inference, new):
+    """A table made anew (here after the first one had run out of blocks) under the same
+    metadata object, lengths and starts; the table a view that the forward copies."""
+    with torch.inference_mode(inference):
+        table = torch.zeros(2, 6, dtype=torch.int32, device=dev)[:, :2]
+        free = torch.tensor([5, 6], dtype=torch.int32, device=dev)
+        ctx, fresh = (torch.tensor([x, x], device=dev) for x in (16, new))
+        f = _Forward(dev, 2 * new, torch.tensor([16 + new] * 2, dtype=torch.int32, device=dev),
+                     torch.tensor([0, new, 2 * new], dtype=torch.int32, device=dev), table)
+        first = f.run()
+        build_step_tables(ctx, fresh, table, free, 16, 2 * new)
+        assert table[:, 1].tolist() == [5, 6]
+        second = f.check()
+        assert not torch.equal(first[0], second[0])
+
+
+def test_forward_sees_the_tables_of_a_replayed_graph(dev):
+    """The tables captured, the attention not: every replay writes the same tensors."""
+    ctx = torch.tensor([3], dtype=torch.int32, device=dev)
+    new = torch.tensor([1], dtype=torch.int32, device=dev)
+    table = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+    free = torch.tensor([2, 3, 4, 5], dtype=torch.int32, device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t = build_step_tables(ctx, new, table, free, 16, 4)
+    g.replay()
+    f, outs = _Forward(dev, 1, t.seq_lens, t.query_start_loc, table), []
+    for n in (3, 17, 40, 15):
+        ctx.fill_(n)
+        g.replay()
+        outs.append(f.check()[0])
+    assert not any(torch.equal(outs[0], o) for o in outs[1:])
