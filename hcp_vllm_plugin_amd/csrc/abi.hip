@@ -47,6 +47,25 @@ int check_heads(int32_t h, int32_t hkv, int32_t d, int32_t dtype, const char* wh
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 
+// A dimension of a tensor that a launch writes: how many, and how far apart.
+struct Dim {
+  int64_t n, stride;
+};
+// Whether runs of `row` elements at these strides lie apart, each dimension's steps
+// clear of all that the shorter ones span: two of a launch's waves write no byte twice.
+template <int N>
+bool rows_apart(int64_t row, Dim (&&dims)[N]) {
+  for (Dim& d : dims) d.stride = d.stride < 0 ? -d.stride : d.stride;
+  std::sort(dims, dims + N, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  __int128 span = row;
+  for (const Dim& d : dims) {
+    if (d.n <= 1) continue;
+    if (d.stride < span) return false;
+    span += static_cast<__int128>(d.stride) * (d.n - 1);
+  }
+  return true;
+}
+
 int check_segment(const hcp_kv_segment& s, int32_t hd, const char* who, int idx) {
   if (s.len < 0 || s.start < 0) return fail(HCP_EINVAL, "%s: entry %d: negative kv start/len", who, idx);
   if (s.len > 0 && (s.k_addr == 0 || s.v_addr == 0))
@@ -1236,6 +1255,9 @@ static int decode_unplanned(const hcp_decode_paged_args* a, bool fp4, const char
   hcp_kv_segment kv = a->kv;
   kv.start = 0;
   kv.len = 1;
+  if (fp4 && !rows_apart(a->head_dim, {{a->num_seqs, a->o_stride_tok},
+                                       {a->num_heads, a->o_stride_head}}))
+    return fail(HCP_EINVAL, "%s: rows of out on top of each other", who);
   if (fp4) {
     rc = check_fp4(kv.k_addr, kv.stride_block, kv.stride_head, kv.num_blocks, kv.block_size,
                    a->head_dim, who);
@@ -1655,6 +1677,11 @@ int hcp_qk_norm_rope(const hcp_qk_rope_args* a, void* stream) {
        a->qo_stride_tok | a->qo_stride_head | a->ko_stride_tok | a->ko_stride_head |
        a->table_stride) % 8)
     return fail(HCP_EINVAL, "%s: strides must be multiples of 8 elements", who);
+  if (!rows_apart(a->head_dim, {{a->num_tokens, a->qo_stride_tok},
+                                {a->num_heads, a->qo_stride_head}}) ||
+      (a->k_out && !rows_apart(a->head_dim, {{a->num_tokens, a->ko_stride_tok},
+                                             {a->num_kv_heads, a->ko_stride_head}})))
+    return fail(HCP_EINVAL, "%s: rows of q_out or k_out on top of each other", who);
   hcp::RopeParams p{};
   if (a->cache_kind) {
     if (!a->v || (a->num_slots && !a->slot_mapping))

@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .kv_cache import _cache_desc, check_slots
-from .varlen import fp4_desc
+from .varlen import fp4_desc, rows_apart
 
 __all__ = ["qk_norm_rope"]
 
@@ -44,7 +44,7 @@ def _out_rows(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype,
               index: int) -> tuple[int, int, int]:
     """``_rows`` of a tensor that is written: its rows are apart."""
     at, tok, head = _rows(name, t, shape, dtype, index)
-    if (shape[0] > 1 and not tok) or (shape[1] > 1 and not head):
+    if not rows_apart(t):
         raise ValueError(f"{name}: rows on top of each other")
     return at, tok, head
 

@@ -938,6 +938,15 @@ class PagedDecode:
 _INDEX_CODES = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
 
+def rows_apart(t: torch.Tensor) -> bool:
+    """Whether the rows of t ``[n, heads, D]`` (contiguous D) lie apart, one of its first
+    two dimensions clear of all that the other spans: a launch may write them."""
+    (n, h, d), (a, b, _) = t.shape, t.stride()
+    if n > 1 and h > 1:
+        return (b >= d and a >= (h - 1) * b + d) or (a >= d and b >= (n - 1) * a + d)
+    return (n <= 1 or a >= d) and (h <= 1 or b >= d)
+
+
 def decode_fp4(
     q: torch.Tensor,
     kv_cache: torch.Tensor,
@@ -988,8 +997,7 @@ def decode_fp4(
     if out is None:
         out = torch.empty(s, h, d, dtype=dt, device=q.device)
     elif out.shape != q.shape or out.dtype != dt or out.stride(2) != 1 or \
-            out.get_device() != index or (s > 1 and not out.stride(0)) or \
-            (h > 1 and not out.stride(1)):
+            out.get_device() != index or not rows_apart(out):
         raise ValueError("out must be as q, with contiguous head_dim and its rows apart")
     lse = torch.empty(h, s, dtype=torch.float32, device=q.device) if with_lse else None
     out_at, (o_tok, o_head, _), lse_at = out.data_ptr(), out.stride(), \

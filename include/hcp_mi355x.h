@@ -745,6 +745,7 @@ int hcp_fp4_gather(const hcp_varlen_entry* entries, int32_t num_entries,
  * hcp_fp4_cache; v_addr and stride_tok are not read.  A block id past the cache
  * reads its last block.  With seq_starts, sequence r sees keys seq_starts[r] ..
  * seq_lens[r] - 1 (of these the last `window`): the keys behind a staged prefix.
+ * The rows of out lie apart (strides that let them overlap are refused).
  */
 size_t hcp_decode_fp4_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
                                 int32_t head_dim);
@@ -763,7 +764,8 @@ int hcp_decode_fp4(const hcp_decode_paged_args* args, void* stream);
  *   cos_sin      DEVICE [max_positions, rot], `dtype` or F32 (table_dtype), rows
  *                table_stride elements apart
  *   weights      DEVICE [head_dim], `dtype` or F32 (weight_dtype), either may be NULL
- *   q_out, k_out may be q and k; k_out may be NULL
+ *   q_out, k_out may be q and k; k_out may be NULL.  Their rows lie apart (strides
+ *                that let them overlap are refused)
  *   cache_kind   0: none; 1: `cache`; 2: `fp4`.  The rotated key and the value of
  *                token t < num_slots go to slot_mapping[t], slots outside the
  *                cache skipped, as in hcp_reshape_and_cache

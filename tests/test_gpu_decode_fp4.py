@@ -300,3 +300,15 @@ def test_rows_of_out_on_top_of_each_other_are_refused(dev):
     for out in (q[:1].expand(2, 4, 64), q[:, :1].expand(2, 4, 64)):
         with pytest.raises(ValueError, match="out"):
             decode_fp4(q, cache, bt, lens, 0.1, out=out)
+
+
+def test_rows_of_out_that_share_bytes_in_part_are_refused(dev):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=dev)
+    cache = torch.zeros(fp4_cache_shape(2, 2, 16, 64), dtype=torch.uint8, device=dev)
+    bt, lens = torch.zeros(2, 1, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int64, device=dev)
+    room = torch.zeros(4096, dtype=torch.bfloat16, device=dev)
+    for strides in ((255, 64, 1), (256, 63, 1), (64, 127, 1)):
+        with pytest.raises(ValueError, match="out"):
+            decode_fp4(q, cache, bt, lens, 0.1, out=room.as_strided((2, 4, 64), strides))
+    heads_first = room.as_strided((2, 4, 64), (64, 128, 1))
+    assert decode_fp4(q, cache, bt, lens, 0.1, out=heads_first) is heads_first

@@ -205,3 +205,16 @@ def test_outputs_on_top_of_each_other_are_refused(dev):
             qk_norm_rope(q, k, pos, table, **kw)
     one = qk_norm_rope(q[:1], k[:1], pos[:1], table, query_out=q[:1], key_out=k[:1])
     assert one[0].shape == (1, 4, 64)
+
+
+def test_outputs_that_share_bytes_in_part_are_refused(dev):
+    q, k = (torch.zeros(3, h, 64, dtype=torch.bfloat16, device=dev) for h in (4, 2))
+    pos, table = torch.zeros(3, dtype=torch.int64, device=dev), torch.zeros(4, 64, device=dev)
+    room = torch.zeros(4096, dtype=torch.bfloat16, device=dev)
+    for kw in ({"query_out": room.as_strided((3, 4, 64), (248, 64, 1))},
+               {"query_out": room.as_strided((3, 4, 64), (64, 184, 1))},
+               {"key_out": room.as_strided((3, 2, 64), (128, 56, 1))}):
+        with pytest.raises(ValueError, match="on top"):
+            qk_norm_rope(q, k, pos, table, **kw)
+    heads_first = room.as_strided((3, 4, 64), (64, 192, 1))
+    assert qk_norm_rope(q, k, pos, table, query_out=heads_first)[0] is heads_first

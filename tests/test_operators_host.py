@@ -11,7 +11,7 @@ import torch
 from hcp_vllm_plugin_amd import _lib, build_step_tables, decode_fp4, qk_norm_rope
 from hcp_vllm_plugin_amd.kv_cache import fp4_cache_shape, gather_kv, reshape_and_cache
 from hcp_vllm_plugin_amd.ring_backend import HcpRingAttentionImpl
-from hcp_vllm_plugin_amd.varlen import PagedCache, segment_paged
+from hcp_vllm_plugin_amd.varlen import PagedCache, rows_apart, segment_paged
 from tests import _fp4_util as f4
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -312,3 +312,34 @@ def test_overlapping_table_rows_are_refused(L):
     a.table_stride, a.table_width, a.num_seqs, a.block_size = 7, 8, 2, 16
     a.ctx_dtype = a.new_dtype = _lib.DTYPE_I32
     assert L.hcp_step_tables(ctypes.addressof(a), None) == _lib.HCP_EINVAL
+
+
+def test_outputs_on_top_of_each_other_are_refused(L):
+    """Strides that let rows share bytes in part, not only strides of 0."""
+    for field in ("qo_stride_tok", "qo_stride_head", "ko_stride_tok", "ko_stride_head"):
+        for stride in (0, 64, 120, 504 if field.endswith("tok") else 632):
+            a = _rope_args()
+            setattr(a, field, stride)
+            assert L.hcp_qk_norm_rope(ctypes.addressof(a), None) == _lib.HCP_EINVAL, (field, stride)
+            assert b"on top" in L.hcp_last_error()
+    for field, stride in (("o_stride_tok", 0), ("o_stride_tok", 28 * 128 - 1), ("o_stride_head", 127),
+                          ("o_stride_head", 28 * 128 + 1)):
+        a = _decode_args()
+        setattr(a, field, stride)
+        assert L.hcp_decode_fp4(ctypes.addressof(a), None) == _lib.HCP_EINVAL, (field, stride)
+        assert b"on top" in L.hcp_last_error()
+
+
+@pytest.mark.parametrize("shape,strides,apart", [
+    ((3, 4, 64), (256, 64, 1), True), ((3, 4, 64), (64, 192, 1), True),  # tokens or heads outside
+    ((3, 4, 64), (1000, 64, 1), True), ((3, 4, 64), (255, 64, 1), False),
+    ((3, 4, 64), (256, 63, 1), False), ((3, 4, 64), (64, 191, 1), False),
+    ((3, 4, 64), (0, 64, 1), False), ((3, 4, 64), (256, 0, 1), False),
+    ((1, 4, 64), (0, 64, 1), True), ((1, 4, 64), (0, 63, 1), False),
+    ((3, 1, 64), (64, 0, 1), True), ((3, 1, 64), (63, 0, 1), False),
+    ((1, 1, 64), (0, 0, 1), True), ((0, 4, 64), (256, 64, 1), True)])
+def test_rows_apart(shape, strides, apart):
+    t = torch.zeros(4000).as_strided(shape, strides)
+    assert rows_apart(t) == apart
+    flat = torch.arange(4000).as_strided(shape, strides).flatten()
+    assert (flat.unique().numel() == flat.numel()) == apart
