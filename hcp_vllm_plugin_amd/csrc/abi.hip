@@ -1530,6 +1530,14 @@ static bool index_dtype(int32_t d) { return d == HCP_DTYPE_I32 || d == HCP_DTYPE
 
 constexpr int64_t kMostThreads = (int64_t{1} << 32) - 256;  // of a launch
 
+// A 4-bit cache that is written: the bytes of each block and head are its own.
+static int check_fp4_written(const hcp_fp4_cache& c, int32_t num_kv_heads, const char* who) {
+  if (!rows_apart(hcp::Fp4Region{c.head_dim, c.block_size}.bytes(),
+                  {{c.num_blocks, c.stride_block}, {num_kv_heads, c.stride_head}}))
+    return fail(HCP_EINVAL, "%s: blocks or heads of the cache on top of each other", who);
+  return HCP_OK;
+}
+
 // What hcp_fp4_write and hcp_fp4_read share.
 static int fp4_params(hcp::Fp4Params& p, const void* slots, int32_t slot_dtype, int64_t num_tokens,
                       int32_t num_kv_heads, const hcp_fp4_cache* cache, int32_t dtype,
@@ -1567,7 +1575,8 @@ int hcp_fp4_write(const void* key, int64_t k_stride_tok, int64_t k_stride_head, 
                   const hcp_fp4_cache* cache, int32_t dtype, void* stream) {
   const char* who = "hcp_fp4_write";
   hcp::Fp4Params p{};
-  const int rc = fp4_params(p, slot_mapping, slot_dtype, num_tokens, num_kv_heads, cache, dtype, who);
+  int rc = fp4_params(p, slot_mapping, slot_dtype, num_tokens, num_kv_heads, cache, dtype, who);
+  if (!rc) rc = check_fp4_written(*cache, num_kv_heads, who);
   if (rc) return rc;
   if (num_tokens == 0 || p.num_slots == 0) return HCP_OK;
   if (!key || !value) return fail(HCP_EINVAL, "%s: null pointer", who);
@@ -1707,6 +1716,11 @@ int hcp_qk_norm_rope(const hcp_qk_rope_args* a, void* stream) {
     if (c.num_blocks && (!c.k_addr || !c.v_addr || (c.k_addr & 15) || (c.v_addr & 15) ||
                          (c.stride_block | c.stride_head | c.stride_tok) % 8))
       return fail(HCP_EINVAL, "%s: the cache must be 16-byte aligned, strides too", who);
+    if (!rows_apart(a->head_dim, {{c.num_blocks, c.stride_block}, {a->num_kv_heads, c.stride_head},
+                                  {bs, c.stride_tok},
+                                  {2, static_cast<int64_t>(c.v_addr - c.k_addr) / 2}}) &&
+        c.num_blocks)
+      return fail(HCP_EINVAL, "%s: rows of the cache on top of each other", who);
     p.k_cache = reinterpret_cast<void*>(c.k_addr);
     p.v_cache = reinterpret_cast<void*>(c.v_addr);
     p.stride_block = c.stride_block;
@@ -1716,8 +1730,9 @@ int hcp_qk_norm_rope(const hcp_qk_rope_args* a, void* stream) {
   } else if (a->cache_kind == hcp::kRopeCacheFp4) {
     if (!a->fp4) return fail(HCP_EINVAL, "%s: null cache descriptor", who);
     const hcp_fp4_cache& c = *a->fp4;
-    const int rc = check_fp4(c.addr, c.stride_block, c.stride_head, c.num_blocks, c.block_size,
-                             c.head_dim, who);
+    int rc = check_fp4(c.addr, c.stride_block, c.stride_head, c.num_blocks, c.block_size,
+                       c.head_dim, who);
+    if (!rc) rc = check_fp4_written(c, a->num_kv_heads, who);
     if (rc) return rc;
     if (c.head_dim != a->head_dim)
       return fail(HCP_EINVAL, "%s: the cache's head_dim %d is not %d", who, c.head_dim, a->head_dim);

@@ -707,7 +707,8 @@ typedef struct hcp_fp4_cache {
 
 /*
  * hcp_reshape_and_cache into a 4-bit cache: the same rows, slots and skipped
- * slots.  `cache` is a HOST pointer.
+ * slots.  `cache` is a HOST pointer; blocks and heads whose bytes overlap are
+ * refused (in either order of the two: reading takes them).
  */
 int hcp_fp4_write(const void* key, int64_t k_stride_tok, int64_t k_stride_head,
                   const void* value, int64_t v_stride_tok, int64_t v_stride_head,
@@ -768,7 +769,8 @@ int hcp_decode_fp4(const hcp_decode_paged_args* args, void* stream);
  *                that let them overlap are refused)
  *   cache_kind   0: none; 1: `cache`; 2: `fp4`.  The rotated key and the value of
  *                token t < num_slots go to slot_mapping[t], slots outside the
- *                cache skipped, as in hcp_reshape_and_cache
+ *                cache skipped, as in hcp_reshape_and_cache; a cache whose rows
+ *                overlap is refused
  * head_dim a multiple of 8 up to 256, rot a multiple of 16 up to head_dim (0: no
  * rotation); 16-byte aligned rows.  `cache` and `fp4` are HOST pointers.
  */

@@ -175,3 +175,26 @@ def test_gather_of_ragged_entries(dev, dtype, d, hkv, bs, lens):
                  ("stride_tok", hkv * d), ("stride_head", d), ("k_addr", kv[0].data_ptr()),
                  ("v_addr", kv[1].data_ptr())):
         assert (out[f] == x).all(), f
+
+
+@pytest.mark.parametrize("order", [(0, 1), (1, 0)])
+def test_heads_or_blocks_outside(dev, order):
+    """Caches whose heads lie outside their blocks, or the other way round; one with a head for
+    all (its bytes shared) is read, not written."""
+    gen = torch.Generator().manual_seed(12)
+    nb, hkv, bs, d = 6, 3, 16, 64
+    k, v = (randn(gen, (40, hkv, d), torch.bfloat16) for _ in "kv")
+    slots = torch.randperm(nb * bs, generator=gen)[:40]
+    want = torch.zeros(fp4_cache_shape(nb, hkv, bs, d), dtype=torch.uint8)
+    f4.write(want, k, v, slots)
+    sizes = (nb, hkv)
+    cache = torch.zeros(sizes[order[0]], sizes[order[1]], bs, d + d // 16, dtype=torch.uint8,
+                        device=dev).permute(*order, 2, 3)
+    reshape_and_cache(k.to(dev), v.to(dev), cache, slots.to(dev))
+    assert torch.equal(cache.cpu(), want)
+    one = cache[:, :1].expand(nb, hkv, bs, d + d // 16)
+    kk, _ = gather_kv(one, slots.to(dev), torch.bfloat16)
+    assert torch.equal(kk[:, 2].cpu().double(), f4.stand_for(k[:, 0]))
+    with pytest.raises(RuntimeError, match="on top"):
+        reshape_and_cache(k.to(dev), v.to(dev), one, slots.to(dev))
+    assert torch.equal(cache.cpu(), want)

@@ -343,3 +343,37 @@ def test_rows_apart(shape, strides, apart):
     assert rows_apart(t) == apart
     flat = torch.arange(4000).as_strided(shape, strides).flatten()
     assert (flat.unique().numel() == flat.numel()) == apart
+
+
+def test_caches_on_top_of_themselves_are_not_written(L):
+    """Blocks or heads of a cache that share bytes, whichever of the two is the outer one;
+    reading them is no race."""
+    region = 16 * 136
+    for block, head, status in ((0, region, _lib.HCP_EINVAL), (4 * region, 0, _lib.HCP_EINVAL),
+                                (4 * region - 16, region, _lib.HCP_EINVAL),
+                                (4 * region, region - 16, _lib.HCP_EINVAL),
+                                (region, 10 * region - 16, _lib.HCP_EINVAL),
+                                (region - 16, 10 * region, _lib.HCP_EINVAL),
+                                (4 * region, region, None), (region, 10 * region, None)):
+        d = _cache_desc(stride_block=block, stride_head=head)
+        at = ctypes.addressof(d)
+        n = 5 if status is not None else 0  # (what is taken is not launched here)
+        want = _lib.HCP_OK if status is None else status
+        assert L.hcp_fp4_write(4096, 512, 128, 4096, 512, 128, 4096, _lib.DTYPE_I64, n, 4, at,
+                               _lib.DTYPE_BF16, None) == want, (block, head)
+        a = _rope_args()
+        a.cache_kind, a.fp4 = 2, at
+        if status is not None:
+            assert L.hcp_qk_norm_rope(ctypes.addressof(a), None) == want, (block, head)
+            assert b"on top" in L.hcp_last_error()
+        assert L.hcp_fp4_read(4096, _lib.DTYPE_I64, 0, 4, at, _lib.DTYPE_BF16, 4096, 4096,
+                              None) == _lib.HCP_OK
+    # 16-bit layouts, in elements: K and V of a row side by side, or blocks of either
+    for v, block, head, tok in ((256, 0, 4096, 256), (256, 16384, 0, 256), (256, 16384, 4096, 0),
+                                (256, 16384, 4096, 248), (256, 16384, 4088, 256), (0, 16384, 4096, 256),
+                                (128, 16384, 4096, 256), (16384, 16384 - 8, 128, 512)):
+        a = _rope_args()
+        c = _lib.PagedCacheDesc(0x1000, 0x1000 + v, block, head, tok, 10, 16, 0)
+        a.cache_kind, a.cache = 1, ctypes.addressof(c)
+        assert L.hcp_qk_norm_rope(ctypes.addressof(a), None) == _lib.HCP_EINVAL, (v, block, head, tok)
+        assert b"on top" in L.hcp_last_error(), (v, block, head, tok)
