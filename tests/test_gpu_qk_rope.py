@@ -218,3 +218,35 @@ def test_outputs_that_share_bytes_in_part_are_refused(dev):
             qk_norm_rope(q, k, pos, table, **kw)
     heads_first = room.as_strided((3, 4, 64), (64, 192, 1))
     assert qk_norm_rope(q, k, pos, table, query_out=heads_first)[0] is heads_first
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("h,hkv,d,rot,bs,t", [
+    (14, 2, 64, 32, 16, 1), (2, 2, 32, 16, 16, 9), (6, 3, 96, 96, 16, 33), (16, 8, 256, 128, 64, 20),
+    # fewer waves than a token has jobs, then one: a wave goes from query jobs to several of
+    # keys and values, through the same LDS
+    (64, 8, 128, 128, 16, 700), (16, 8, 256, 256, 32, 700), (64, 8, 128, 64, 16, 2100),
+    (16, 8, 256, 256, 16, 2100), (5, 12, 96, 96, 16, 2100)])
+def test_into_the_4_bit_cache_at_length(dev, dtype, interleaved, h, hkv, d, rot, bs, t):
+    """Neighbours or halves paired, at every number of waves to a token: the cache holds the
+    formula's key, rounded to the type, then coded; bytes of no slot stay as they were."""
+    gen = torch.Generator().manual_seed(d + t + h)
+    q, k, v = _inputs(gen, t, h, hkv, d, dtype)
+    pos = torch.randint(0, 3000, (t,), generator=gen)
+    table = _table(3000, rot, torch.float32)
+    w = (1 + 0.2 * torch.randn(d, generator=gen)).to(dtype)
+    nb = -(-t // bs) + 3
+    slots = torch.randperm(nb * bs, generator=gen)[:t]
+    slots[t // 3] = -1 if t > 1 else slots[0]
+    cache = torch.randint(0, 256, fp4_cache_shape(nb, hkv, bs, d), generator=gen,
+                          dtype=torch.uint8)
+    key = _ref(k, w, pos, table, interleaved)[0].to(dtype)
+    want = cache.clone()
+    f4.write(want, key, v, slots)
+    got, hold = cache.to(dev), torch.empty_like(k, device=dev)
+    gq, _ = qk_norm_rope(q.to(dev), k.to(dev), pos.to(dev), table.to(dev), q_weight=w.to(dev),
+                         k_weight=w.to(dev), interleaved=interleaved, value=v.to(dev), kv_cache=got,
+                         slot_mapping=slots.to(dev), key_out=hold)
+    assert torch.equal(hold.cpu(), key) and torch.equal(got.cpu(), want)
+    _check(gq, _ref(q, w, pos, table, interleaved), dtype)
