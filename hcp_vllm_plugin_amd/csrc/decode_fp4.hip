@@ -25,13 +25,16 @@
 // 16k-32k 64 -> 51 us).  The waves are combined through LDS; decode_reduce_kernel
 // merges a sequence's partials.
 //
-// Bound by HBM: 64 x 16k-32k keys of 28 / 4 x 128 (850 MB) take 144 us with the
-// merge, 5.9 TB/s (146 on the same card with the scores' maximum, the sum and the
-// scales in more instructions); its loads alone, without the arithmetic, 94% of
-// that; the 16-bit kernel reads blocks at 6.1 TB/s.  At 64 columns a chunk has as
-// many instructions for half the bytes: 256 x 32k keys of 14 / 2 x 64 (1.13 GB) take
-// 230 us (237 before), 200 by the loads alone.  One sequence of 2000 keys: 11.4 us,
-// the chain of latencies (lengths, block ids, keys, combine, merge).
+// Bound by HBM, us of a pass with the merge: 64 x 16k-32k keys of 28 / 4 x 128 (851 MB)
+// 144-148, 5.9 TB/s (146 against 144 on one card with the scores' maximum, the sum and
+// the scales in more instructions); 256 x 16k of these heads (2.29 GB) 369, 6.2 TB/s; 64 x
+// 16k of 16 / 8 x 256 (2.28 GB) 355, 6.4 TB/s; the 16-bit kernel reads its blocks at 6.6.
+// On the same card the same launches with compute() left out 142, 358 and 344.  At
+// 64 columns a chunk has as many instructions for half the bytes, and a head's 1088
+// bytes of a 16-token block are eight and a half lines of which nine are fetched (1.22
+// GB of HBM for 1.14 GB): 256 x 32k keys of 14 / 2 x 64 take 210 us, 196 without
+// compute().  One sequence of 2000 keys: 8.3 us and 4.2 for the merge, the chain of
+// latencies (lengths, block ids, keys, combine, merge).
 #include "decode_share.h"
 
 namespace hcp {
@@ -152,7 +155,7 @@ __device__ __forceinline__ void fp4_split_body(const PagedDecParams& p, int kvh_
       // A lane takes two pieces in a row of either, but what a load fetches lies in a
       // row too: keys 8 i .. of K, quads 2 i and 2 i + 1 of V, four lanes the 64 bytes
       // of four pieces (with every other piece of 2 KB in a load, 64 x 16k keys of
-      // 16 / 8 heads took 418 us, now 368).  The order of the four in LDS spreads the
+      // 16 / 8 heads took 418 us on a card where these take 368).  The order of the four in LDS spreads the
       // reads of 16 lanes over all banks for V, over half of them for K (over all of
       // them, K's 64 bytes in another order: 369).
       const int q = lane >> 2, r = lane & 3, e = c16 >> 1;

@@ -12,13 +12,15 @@
 // something is summed.
 //
 // HBM-bound: 4 d bytes for a query row, 4 d (16-bit cache) or 2 d + 17 d / 32 for a
-// key or value row; 8192 tokens of 28 / 4 x 128 (155 MB) 33 us, 4.7 TB/s, where a
-// large copy runs at 4.9; 4096 of 64 / 8 x 128 into the 4-bit cache (155 MB) 36 us;
-// one token 3.8 us.  A lane holds 16 columns of a row, the eight of a pair's first
-// sides and the eight of their second sides, so that nothing is exchanged but the
-// sum of squares, over the 8 lanes of a row at d = 128; it keeps its 8 cosines and
-// sines for all heads of its token (read again for every head they would be twice
-// the row's own bytes).
+// key or value row; 8192 tokens of 28 / 4 x 128 (155 MB) 32.2 us, 4.8 TB/s, where a
+// large copy runs at 4.9; 4096 of 64 / 8 x 128 into the 4-bit cache (157 MB) 34.3 us;
+// one token 3.6 us.  Few KV heads leave their job's rows empty: 5003 tokens of 14 / 2 x
+// 64 without a cache, a wave's 16 rows taken by 14 query heads and then by 2 of keys, 7.8
+// us where their 21 MB would copy in 4.3.  A lane holds 16 columns of a row, the
+// eight of a pair's first sides and the eight of their second sides, so that nothing
+// is exchanged but the sum of squares, over the 8 lanes of a row at d = 128; it keeps
+// its 8 cosines and sines for all heads of its token (read again for every head they
+// would be twice the row's own bytes).
 #include "params.h"
 
 namespace hcp {

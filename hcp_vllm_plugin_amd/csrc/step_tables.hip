@@ -10,8 +10,8 @@
 // loaded at once; sums and cached lengths in LDS) and takes its share of the tokens
 // and of the new table entries, each of which finds its request by bisection; a
 // token in a new block takes its id from the free list, not from the table that
-// another workgroup may still be writing.  64 / 1000 / 4000 requests 4.0 / 5.5 / 12.4
-// us (with the lengths loaded one after the other 4.4 / 6.8 / 17.2).
+// another workgroup may still be writing.  64 / 1000 / 4000 requests 3.3 / 5.6 / 11.7
+// us (with the lengths loaded one after the other 0.4, 1.3 and 4.8 us more).
 #include "decode_share.h"
 #include "params.h"
 

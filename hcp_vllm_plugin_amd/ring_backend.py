@@ -876,7 +876,13 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
         16 / 8 x 256, 2 x 8192 (14) 98 / 90.  With 1024 staged keys each, 28 / 4 x
         128, 2 x 24576 (42) 145 / 164, 2 x 49152 (83) 201 / 171; 8 x 12000 (86) 221 /
         240, 8 x 16384 (115) 268 / 249; 32 x 8192 (244) 497 / 503, 32 x 16384 (462)
-        849 / 519."""
+        849 / 519.
+
+        Over a 4-bit cache the rows' keys are expanded too where they stay, and the
+        same 20 us are about where both take as long at 64 and 128 columns, but late at
+        256: 28 / 4 x 128, 16 x 512 (7) 83 / 96, 16 x 1536 (21) 94 / 93, 8 x 4096 (27) 110 /
+        93, 32 x 4096 (110) 315 / 96; 14 / 2 x 64, 8 x 1024 (2) 74 / 93, 32 x 4096 (30) 120
+        / 93; 16 / 8 x 256, 2 x 2048 (4) 91 / 93, 2 x 8192 (14) 131 / 95."""
         w = self.sliding_window
         keys = [tk if w is None else min(tk, w)
                 for r, tk in enumerate(seq_lens) if qsl[r + 1] - qsl[r] == 1]
@@ -888,7 +894,11 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
     def _plan(self, layer_name, qsl, seq_lens, block_table, first_blocks, pc, split):
         plan = _Plan()
         n = len(seq_lens)
-        # (a 4-bit cache's keys are expanded for the launch of the others anyway)
+        # (Over a 4-bit cache they stay: the decode launch of these rows takes segments,
+        # which that has not.  The prefill launch expands their keys as it does the
+        # others': 256 new tokens behind 1024 staged ones next to 16 rows of 1536 keys at
+        # 28 / 4 x 128 159 us a layer, next to 32 of 4096 382, of 16384 1228; over a 16-bit
+        # cache 144, 282 and 377.)
         apart = qsl != list(range(n + 1)) and pc.layout != "fp4" and \
             self._decode_rows_apart(qsl, seq_lens, True)
         ring_on = _decode_ring_enabled() and bool(DECODE_RING_MAP)
@@ -1438,7 +1448,12 @@ class HcpRingAttentionImpl(_ImplBase):  # type: ignore[misc,valid-type]
         """A pure decode batch with staged peers over a 4-bit cache: the local
         keys past each prefix (or, inside it, all of them: ring_backend.py:811-830)
         in the 4-bit decode, then the peers, which take that result as their
-        running accumulator."""
+        running accumulator.  It is of the model's type there, as the decode ring's
+        accumulator and the prefill's peer results are: half a step of the local
+        result, weighed by its share, next to the half step that the output takes.
+
+        us a layer (over a 16-bit cache, in one launch): 16 rows of 8192 keys, 4096 of
+        them staged, at 28 / 4 x 128 172 (98); 64 of 34000, 32768 staged, 780 (744)."""
         (_qsl, seq_lens, first_blocks), block_table = step.host, step.bt
         _check_base(pc)
         n = len(seq_lens)

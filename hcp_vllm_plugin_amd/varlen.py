@@ -965,7 +965,9 @@ def decode_fp4(
     ``block_table``, the last ``window`` of them; lengths and block ids are
     read on the device when the call executes.  A query that sees no key gets
     out 0 and LSE -inf; a length past its table row counts as the row's keys.
-    ``keep_nan``: as ``DecodeBatch.run``.  Returns out (and lse float32 ``[H, S]``)."""
+    A key written from an infinity or a NaN has NaN scores: the split of the keys that
+    holds it (which keys those are goes by the whole batch) is left out of its row, or
+    with ``keep_nan`` the row is NaN, as in ``DecodeBatch.run``.  Returns out (and lse float32 ``[H, S]``)."""
     dt, index = q.dtype, q.get_device()
     if q.dim() != 3 or (dt != torch.bfloat16 and dt != torch.float16) or q.stride(2) != 1:
         raise ValueError("q must be float16/bfloat16 [S, H, D] with contiguous head_dim")

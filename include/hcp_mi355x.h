@@ -112,6 +112,9 @@ typedef struct hcp_decode_split {
   int32_t slot;
 } hcp_decode_split;
 
+/* HCP_ABI_VERSION of the library.  A caller built against another version makes
+ * no other call: argument blocks grow at their ends from one to the next (with 12
+ * hcp_decode_paged_args by seq_starts), and an entry reads all of its own. */
 int hcp_abi_version(void);
 const char* hcp_last_error(void);
 
