@@ -394,9 +394,9 @@ def _meta_stamp(attn_metadata) -> tuple:
     refills its tensors in place between steps through torch's in-place ops
     bumps the version counters, so the next step does not reuse the previous
     step's host copy or plans; ``build_step_tables`` bumps its table's, and what it
-    writes unseen is told by the layers (``_Step.serves``).  (vLLM builds a new metadata object every
-    step; tensors made under inference mode keep no version counter, and a
-    caller that refills such tensors in one reused object calls
+    writes unseen is told by the layers (``_Step.serves``).  (vLLM builds a new
+    metadata object every step; tensors made under inference mode keep no version
+    counter, and a caller that refills such tensors in one reused object calls
     ``invalidate_step_cache`` between steps.)"""
     st = [id(attn_metadata)]
     for t in (attn_metadata.query_start_loc, attn_metadata.seq_lens, attn_metadata.block_table):

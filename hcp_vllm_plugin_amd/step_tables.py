@@ -65,10 +65,11 @@ def build_step_tables(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     ``positions`` and ``slot_mapping`` have ``num_tokens`` rows: the new tokens,
     then (padding) position 0 and slot -1.  Lengths below 0 count as 0.
 
-    A captured call writes the same tensors at every replay.  ``forward`` outside
-    the graph reads them anew for a new metadata object, or when a layer comes again
-    with a kept one; a caller whose next step begins with a layer that the last one
-    left out calls ``ring_backend.invalidate_step_cache`` in between."""
+    A captured call writes the same tensors at every replay, unseen by ``forward``
+    outside the graph, as is a table made under inference mode that any call writes.
+    ``forward`` reads these anew for a new metadata object, or when a layer comes
+    again with a kept one; a caller whose next step begins with a layer that the last
+    one left out calls ``ring_backend.invalidate_step_cache`` in between."""
     index, ints_of = block_table.get_device(), _INDEX.get
     ctx_code, new_code, (n, *more) = ints_of(ctx_lens.dtype), ints_of(new_lens.dtype), ctx_lens.shape
     if more or ctx_code is None or new_code is None or new_lens.shape != (n,):
