@@ -15,14 +15,18 @@ the work in hand-written gfx950 HIP kernels (``libhcp_mi355x.so``, C ABI in
   slots and positions from the requests' lengths), ``qk_norm_rope`` (head norms,
   rotation and cache write) and a KV cache in 4 bits (``kv_cache``, ``decode_fp4``,
   ``HcpRingAttentionImpl(kv_cache_dtype="fp4")``)
+* a decode step with drafted tokens: ``decode_drafts`` (their attention over a paged
+  cache) and ``verify_drafts`` (which of them stay), with ``rope_table`` for the
+  positions of long contexts
 
 Importing the package does not import vLLM; ``register()`` does.
 """
 
 from __future__ import annotations
 
+from .drafts import decode_drafts, verify_drafts
 from .merge import merge_attn_states, merge_pair
-from .qk_rope import qk_norm_rope
+from .qk_rope import qk_norm_rope, rope_table
 from .ring_attn import ring_attn_merged, ring_attn_with_lse
 from .step_tables import build_step_tables
 from .varlen import decode_fp4
@@ -36,6 +40,9 @@ __all__ = [
     "build_step_tables",
     "qk_norm_rope",
     "decode_fp4",
+    "rope_table",
+    "decode_drafts",
+    "verify_drafts",
     "BACKEND_PATH",
 ]
 

@@ -84,6 +84,11 @@ EXPORTED_SYMBOLS = (
     "hcp_decode_fp4",
     "hcp_qk_norm_rope",
     "hcp_step_tables",
+    "hcp_decode_drafts_workspace",
+    "hcp_decode_drafts",
+    "hcp_verify_workspace",
+    "hcp_verify_drafts",
+    "hcp_rope_table",
 )
 
 ABI_VERSION = 12
@@ -335,6 +340,71 @@ class StepTablesArgs(ctypes.Structure):
     ]
 
 
+class DecodeDraftsArgs(ctypes.Structure):
+    """``hcp_decode_drafts_args`` (include/hcp_mi355x.h)."""
+
+    _fields_ = [
+        ("decode", DecodePagedArgs),
+        ("row_starts", ctypes.c_uint64),
+        ("q_rows", ctypes.c_int64),
+        ("max_tokens", ctypes.c_int32),
+        ("fp4", ctypes.c_int32),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    """``hcp_verify_args`` (include/hcp_mi355x.h)."""
+
+    _fields_ = [
+        ("target", ctypes.c_uint64),
+        ("row_stride", ctypes.c_int64),
+        ("num_rows", ctypes.c_int64),
+        ("tokens", ctypes.c_uint64),
+        ("row_starts", ctypes.c_uint64),
+        ("uniform", ctypes.c_uint64),
+        ("uniform_stride", ctypes.c_int64),
+        ("draft_probs", ctypes.c_uint64),
+        ("q_stride_seq", ctypes.c_int64),
+        ("q_stride_row", ctypes.c_int64),
+        ("temperature", ctypes.c_uint64),
+        ("out", ctypes.c_uint64),
+        ("num_out", ctypes.c_uint64),
+        ("workspace", ctypes.c_uint64),
+        ("workspace_bytes", ctypes.c_uint64),
+        ("vocab", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("max_tokens", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("tokens_dtype", ctypes.c_int32),
+        ("starts_dtype", ctypes.c_int32),
+        ("probs", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class RopeTableArgs(ctypes.Structure):
+    """``hcp_rope_table_args`` (include/hcp_mi355x.h)."""
+
+    _fields_ = [
+        ("out", ctypes.c_uint64),
+        ("stride", ctypes.c_int64),
+        ("num_positions", ctypes.c_int64),
+        ("base", ctypes.c_double),
+        ("factor", ctypes.c_double),
+        ("original", ctypes.c_double),
+        ("low_freq", ctypes.c_double),
+        ("high_freq", ctypes.c_double),
+        ("beta_fast", ctypes.c_double),
+        ("beta_slow", ctypes.c_double),
+        ("attention_factor", ctypes.c_double),
+        ("divisors", ctypes.c_uint64),
+        ("rot", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scaling", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # include/hcp_mi355x.h HCP_STEP_MAX_SEQS
 STEP_MAX_SEQS = 4096
 
@@ -360,9 +430,15 @@ pack_qk_rope = packer(QkRopeArgs)
 pack_step_tables = packer(StepTablesArgs)
 pack_decode_paged = packer(DecodePagedArgs)
 pack_fp4_cache = packer(Fp4CacheDesc)
+pack_decode_drafts = packer(DecodeDraftsArgs)
+pack_verify = packer(VerifyArgs)
+pack_rope_table = packer(RopeTableArgs)
 
 # include/hcp_mi355x.h HCP_DECODE_PAGED_MAX_SEQS
 DECODE_PAGED_MAX_SEQS = 1024
+# include/hcp_mi355x.h HCP_DRAFTS_MAX_TOKENS, HCP_VERIFY_MAX_TOKENS
+DRAFTS_MAX_TOKENS = 64
+VERIFY_MAX_TOKENS = 64
 
 _lock = threading.Lock()
 _lib = None
@@ -480,6 +556,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.hcp_qk_norm_rope.argtypes = [_P, _P]
     lib.hcp_step_tables.restype = ctypes.c_int
     lib.hcp_step_tables.argtypes = [_P, _P]
+    lib.hcp_decode_drafts_workspace.restype = ctypes.c_size_t
+    lib.hcp_decode_drafts_workspace.argtypes = [_I32, _I32, _I32, _I32, _I32, _I32]
+    lib.hcp_decode_drafts.restype = ctypes.c_int
+    lib.hcp_decode_drafts.argtypes = [_P, _P]
+    lib.hcp_verify_workspace.restype = ctypes.c_size_t
+    lib.hcp_verify_workspace.argtypes = [_I32, _I32, _I32]
+    lib.hcp_verify_drafts.restype = ctypes.c_int
+    lib.hcp_verify_drafts.argtypes = [_P, _P]
+    lib.hcp_rope_table.restype = ctypes.c_int
+    lib.hcp_rope_table.argtypes = [_P, _P]
     lib.hcp_merge_attn_states.restype = ctypes.c_int
     lib.hcp_merge_attn_states.argtypes = [
         _P, _I64, _I64, _I32, _P, _I64,
@@ -556,6 +642,20 @@ class SplitLimits(NamedTuple):
 def decode_fp4_workspace(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
     """``hcp_decode_fp4_workspace``, asked once for a size."""
     return lib().hcp_decode_fp4_workspace(num_seqs, num_heads, num_kv_heads, head_dim)
+
+
+@functools.lru_cache(maxsize=1024)
+def decode_drafts_workspace(num_seqs: int, max_tokens: int, num_heads: int, num_kv_heads: int,
+                            head_dim: int, fp4: bool) -> int:
+    """``hcp_decode_drafts_workspace``, asked once for a size."""
+    return lib().hcp_decode_drafts_workspace(num_seqs, max_tokens, num_heads, num_kv_heads,
+                                             head_dim, fp4)
+
+
+@functools.lru_cache(maxsize=1024)
+def verify_workspace(num_seqs: int, max_tokens: int, vocab: int) -> int:
+    """``hcp_verify_workspace``, asked once for a size."""
+    return lib().hcp_verify_workspace(num_seqs, max_tokens, vocab)
 
 
 @functools.lru_cache(maxsize=None)  # one entry per head_dim

@@ -33,6 +33,10 @@ OBJECTS = [
     ("fp4_cache.hip", []),
     ("qk_rope.hip", []),
     ("step_tables.hip", []),
+    ("decode_drafts.hip", ["-DHCP_DRAFTS_FP4=0"]),
+    ("decode_drafts.hip", ["-DHCP_DRAFTS_FP4=1"]),
+    ("verify.hip", []),
+    ("rope_table.hip", []),
 ]
 
 HIPCC_FLAGS = [

@@ -1822,4 +1822,276 @@ int hcp_step_tables(const hcp_step_tables_args* a, void* stream) {
   return launch_status(hcp::launch_step_tables(p, static_cast<hipStream_t>(stream)), who);
 }
 
+// How a launch of hcp_decode_drafts is laid out: tiles of 16 rows to a workgroup,
+// chunks of so many, workgroups per KV head and chunk.
+struct DraftsPlan {
+  int32_t tiles, chunks, wgs;
+  size_t o_bytes, lse_bytes, bytes;  // of the partials, of their LSEs, of the workspace
+};
+static DraftsPlan plan_drafts(int32_t num_seqs, int32_t max_tokens, int32_t num_heads,
+                              int32_t num_kv_heads, int32_t head_dim, bool fp4) {
+  DraftsPlan d{};
+  const int32_t dw = hcp::padded_head_dim(head_dim), most = dw == 256 ? 2 : 4;
+  const int32_t all = (max_tokens * (num_heads / num_kv_heads) + 15) / 16;
+  d.chunks = (all + most - 1) / most;
+  d.tiles = (all + d.chunks - 1) / d.chunks;
+  d.wgs = std::max(1, hcp::drafts_per_cu(fp4, dw, d.tiles) * kNumCus / (num_kv_heads * d.chunks));
+  const size_t parts = static_cast<size_t>(num_seqs + d.wgs) * max_tokens * num_heads;
+  d.o_bytes = (parts * dw * sizeof(float) + 255) & ~static_cast<size_t>(255);
+  d.lse_bytes = (parts * sizeof(float) + 255) & ~static_cast<size_t>(255);
+  d.bytes = d.o_bytes + d.lse_bytes + 2 * sizeof(int32_t) * num_seqs;
+  return d;
+}
+
+static bool drafts_sizes(int32_t num_seqs, int32_t max_tokens, int32_t num_heads,
+                         int32_t num_kv_heads, int32_t head_dim) {
+  return num_seqs > 0 && num_seqs <= HCP_DECODE_PAGED_MAX_SEQS && max_tokens > 0 &&
+         max_tokens <= HCP_DRAFTS_MAX_TOKENS && num_heads > 0 && num_heads <= 1 << 16 &&
+         num_kv_heads > 0 && num_heads % num_kv_heads == 0 && head_dim > 0 && head_dim <= 256;
+}
+
+size_t hcp_decode_drafts_workspace(int32_t num_seqs, int32_t max_tokens, int32_t num_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, int32_t fp4) {
+  if (!drafts_sizes(num_seqs, max_tokens, num_heads, num_kv_heads, head_dim)) return 0;
+  return plan_drafts(num_seqs, max_tokens, num_heads, num_kv_heads, head_dim, fp4 != 0).bytes;
+}
+
+int hcp_decode_drafts(const hcp_decode_drafts_args* args, void* stream) {
+  const char* who = "hcp_decode_drafts";
+  if (!args) return fail(HCP_EINVAL, "%s: null arguments", who);
+  const hcp_decode_paged_args* a = &args->decode;
+  const bool fp4 = args->fp4 != 0;
+  int rc = check_heads(a->num_heads, a->num_kv_heads, a->head_dim, a->dtype, who);
+  if (rc) return rc;
+  if (a->num_seqs < 0 || a->window < 0 || a->block_table_width <= 0 || args->q_rows < 0 ||
+      args->max_tokens <= 0)
+    return fail(HCP_EINVAL, "%s: bad sizes", who);
+  if (a->num_seqs == 0 || args->q_rows == 0) return HCP_OK;
+  if (!drafts_sizes(a->num_seqs, args->max_tokens, a->num_heads, a->num_kv_heads, a->head_dim))
+    return fail(HCP_EUNSUPPORTED, "%s: more than %d sequences, %d tokens of one, or %d heads", who,
+                HCP_DECODE_PAGED_MAX_SEQS, HCP_DRAFTS_MAX_TOKENS, 1 << 16);
+  if (args->q_rows > INT32_MAX) return fail(HCP_EUNSUPPORTED, "%s: too many rows", who);
+  if (!a->q || !a->out || !a->seq_lens || !args->row_starts || !a->kv.block_table)
+    return fail(HCP_EINVAL, "%s: null pointer", who);
+  if (a->seq_starts) return fail(HCP_EUNSUPPORTED, "%s: seq_starts", who);
+  if (a->lens_dtype != HCP_DTYPE_I32 && a->lens_dtype != HCP_DTYPE_I64)
+    return fail(HCP_EUNSUPPORTED, "%s: seq_lens dtype %d (int32 or int64)", who, a->lens_dtype);
+  if (!aligned16(a->q) || (a->q_stride_tok | a->q_stride_head) % 8)
+    return fail(HCP_EINVAL, "%s: q not in 16-byte rows", who);
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale))
+    return fail(HCP_EINVAL, "%s: scale must be finite and > 0", who);
+  if (!rows_apart(a->head_dim, {{args->q_rows, a->o_stride_tok}, {a->num_heads, a->o_stride_head}}))
+    return fail(HCP_EINVAL, "%s: rows of out on top of each other", who);
+  if (a->lse && !rows_apart(args->q_rows, {{a->num_heads, a->lse_stride_head}}))
+    return fail(HCP_EINVAL, "%s: heads of lse on top of each other", who);
+  hcp_kv_segment kv = a->kv;
+  kv.start = 0;
+  kv.len = 1;
+  rc = fp4 ? check_fp4(kv.k_addr, kv.stride_block, kv.stride_head, kv.num_blocks, kv.block_size,
+                       a->head_dim, who)
+           : check_segment(kv, a->head_dim, who, 0);
+  if (rc) return rc;
+  if (kv.num_blocks <= 0) return fail(HCP_EINVAL, "%s: a cache without blocks", who);
+  // (16 rows of a block are one descriptor's)
+  if (!fp4 && (kv.stride_tok < 0 || kv.stride_tok >= int64_t{1} << 25))
+    return fail(HCP_EUNSUPPORTED, "%s: keys too far apart", who);
+  // the kernel sums chunks of 32 keys in 32 bits, and looks 256 keys ahead
+  if (a->block_table_width > ((int64_t{1} << 34) / kv.block_size) / a->num_seqs ||
+      a->block_table_width * kv.block_size > INT32_MAX - 1024)
+    return fail(HCP_EUNSUPPORTED, "%s: block table names too many keys", who);
+  const DraftsPlan d = plan_drafts(a->num_seqs, args->max_tokens, a->num_heads, a->num_kv_heads,
+                                   a->head_dim, fp4);
+  if (!a->workspace || a->workspace_bytes < d.bytes)
+    return fail(HCP_EWORKSPACE, "%s: workspace %zu bytes < %zu needed", who,
+                static_cast<size_t>(a->workspace_bytes), d.bytes);
+  if (!aligned16(a->workspace)) return fail(HCP_EINVAL, "%s: workspace not 16-byte aligned", who);
+  char* const ws = static_cast<char*>(a->workspace);
+  hcp::DraftParams p{};
+  hcp::DecParams& dp = p.p.d;
+  dp.q = a->q;
+  dp.q_stride_tok = a->q_stride_tok;
+  dp.q_stride_head = a->q_stride_head;
+  dp.num_wgs = d.wgs;
+  dp.ws_o = reinterpret_cast<float*>(ws);
+  dp.ws_lse = reinterpret_cast<float*>(ws + d.o_bytes);
+  dp.num_heads = a->num_heads;
+  dp.num_kv_heads = a->num_kv_heads;
+  dp.group = a->num_heads / a->num_kv_heads;
+  dp.head_chunks = d.chunks;
+  dp.head_dim = a->head_dim;
+  dp.scale_log2 = a->scale * hcp::kLog2e;
+  p.p.kv = kv;
+  p.p.lens = a->seq_lens;
+  p.p.lens_wide = a->lens_dtype == HCP_DTYPE_I64;
+  p.p.num_seqs = a->num_seqs;
+  p.p.bt_stride = a->block_table_stride;
+  p.p.max_len = a->block_table_width * kv.block_size;
+  p.p.seq_slots = reinterpret_cast<int32_t*>(ws + d.o_bytes + d.lse_bytes);
+  p.row_starts = args->row_starts;
+  p.q_rows = args->q_rows;
+  p.max_tokens = args->max_tokens;
+  p.window = std::min(a->window, 1 << 30);  // (positions less it stay in 32 bits)
+  p.num_slots = a->num_seqs + d.wgs;
+  const hcp::DraftOut o{a->out, a->o_stride_tok, a->o_stride_head, a->lse, a->lse_stride_head};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const hipError_t err = fp4 ? hcp::launch_drafts_fp4(p, d.tiles, a->dtype, st)
+                             : hcp::launch_drafts16(p, d.tiles, a->dtype, st);
+  return launch_status(err != hipSuccess ? err : hcp::launch_drafts_reduce(p, o, a->dtype, st), who);
+}
+
+struct VerifyPlan {
+  int32_t stat_slices, sum_slices;
+  size_t rows_at, sums_at, bytes;
+};
+static VerifyPlan plan_verify(int32_t num_seqs, int32_t max_tokens, int32_t vocab) {
+  VerifyPlan v{};
+  v.stat_slices = (vocab + hcp::kVerStatSlice - 1) / hcp::kVerStatSlice;
+  v.sum_slices = (vocab + hcp::kVerSumSlice - 1) / hcp::kVerSumSlice;
+  v.rows_at = sizeof(hcp::VerifyStat) * num_seqs * max_tokens * v.stat_slices;
+  v.sums_at = v.rows_at + sizeof(hcp::VerifyRow) * num_seqs;
+  v.bytes = v.sums_at + 2 * sizeof(double) * num_seqs * v.sum_slices;
+  return v;
+}
+static bool verify_sizes(int32_t num_seqs, int32_t max_tokens, int32_t vocab) {
+  return num_seqs > 0 && num_seqs <= 65536 && max_tokens > 0 &&
+         max_tokens <= HCP_VERIFY_MAX_TOKENS && vocab > 0 && vocab <= 1 << 22;
+}
+
+size_t hcp_verify_workspace(int32_t num_seqs, int32_t max_tokens, int32_t vocab) {
+  return verify_sizes(num_seqs, max_tokens, vocab) ? plan_verify(num_seqs, max_tokens, vocab).bytes
+                                                   : 0;
+}
+
+int hcp_verify_drafts(const hcp_verify_args* a, void* stream) {
+  const char* who = "hcp_verify_drafts";
+  if (!a) return fail(HCP_EINVAL, "%s: null arguments", who);
+  if (a->num_seqs < 0 || a->num_rows < 0 || a->vocab <= 0 || a->max_tokens <= 0)
+    return fail(HCP_EINVAL, "%s: bad sizes", who);
+  if (a->num_seqs == 0) return HCP_OK;
+  if (!verify_sizes(a->num_seqs, a->max_tokens, a->vocab))
+    return fail(HCP_EUNSUPPORTED, "%s: more than 65536 sequences, %d tokens of one, or 2^22 entries",
+                who, HCP_VERIFY_MAX_TOKENS);
+  if (!dtype16(a->dtype) && a->dtype != HCP_DTYPE_F32)
+    return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
+  if (!index_dtype(a->tokens_dtype) || !index_dtype(a->starts_dtype))
+    return fail(HCP_EUNSUPPORTED, "%s: tokens and row_starts must be int32 or int64", who);
+  if ((a->num_rows > 0 && (!a->target || !a->tokens)) || !a->row_starts || !a->uniform || !a->out ||
+      !a->num_out)
+    return fail(HCP_EINVAL, "%s: null pointer", who);
+  const VerifyPlan v = plan_verify(a->num_seqs, a->max_tokens, a->vocab);
+  if (static_cast<int64_t>(a->num_seqs) * a->max_tokens * v.stat_slices > INT32_MAX ||
+      static_cast<int64_t>(a->num_seqs) * v.sum_slices > INT32_MAX)
+    return fail(HCP_EUNSUPPORTED, "%s: too many rows", who);
+  if (!a->workspace || a->workspace_bytes < v.bytes)
+    return fail(HCP_EWORKSPACE, "%s: workspace %zu bytes < %zu needed", who,
+                static_cast<size_t>(a->workspace_bytes), v.bytes);
+  if (!aligned16(a->workspace)) return fail(HCP_EINVAL, "%s: workspace not 16-byte aligned", who);
+  char* const ws = static_cast<char*>(a->workspace);
+  hcp::VerifyParams p{};
+  p.target = a->target;
+  p.row_bytes = a->row_stride * (a->dtype == HCP_DTYPE_F32 ? 4 : 2);
+  p.num_rows = a->num_rows;
+  p.tokens = a->tokens;
+  p.tokens_wide = a->tokens_dtype == HCP_DTYPE_I64;
+  p.row_starts = a->row_starts;
+  p.starts_wide = a->starts_dtype == HCP_DTYPE_I64;
+  p.uniform = a->uniform;
+  p.uniform_stride = a->uniform_stride;
+  p.draft_probs = a->max_tokens > 1 ? a->draft_probs : nullptr;
+  p.q_stride_seq = a->q_stride_seq;
+  p.q_stride_row = a->q_stride_row;
+  p.temperature = a->temperature;
+  p.out = a->out;
+  p.num_out = a->num_out;
+  p.stats = reinterpret_cast<hcp::VerifyStat*>(ws);
+  p.rows = reinterpret_cast<hcp::VerifyRow*>(ws + v.rows_at);
+  p.sums = reinterpret_cast<double*>(ws + v.sums_at);
+  p.residuals = p.sums + static_cast<size_t>(a->num_seqs) * v.sum_slices;
+  p.vocab = a->vocab;
+  p.num_seqs = a->num_seqs;
+  p.max_tokens = a->max_tokens;
+  p.stat_slices = v.stat_slices;
+  p.sum_slices = v.sum_slices;
+  return launch_status(hcp::launch_verify(p, a->dtype, a->probs != 0,
+                                          static_cast<hipStream_t>(stream)), who);
+}
+
+int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
+  const char* who = "hcp_rope_table";
+  if (!a) return fail(HCP_EINVAL, "%s: null arguments", who);
+  if (a->rot <= 0 || a->rot > 2 * hcp::kRopeMaxFrequencies || a->rot % 16)
+    return fail(HCP_EUNSUPPORTED, "%s: rot %d (a multiple of 16 up to 256)", who, a->rot);
+  if (!dtype16(a->dtype) && a->dtype != HCP_DTYPE_F32)
+    return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
+  // (positions times frequencies stay exact to 2^-24 of a turn)
+  if (a->num_positions < 0 || a->num_positions > int64_t{1} << 28)
+    return fail(HCP_EINVAL, "%s: bad sizes", who);
+  const bool scaled = a->scaling != HCP_ROPE_SCALING_NONE;
+  if (a->scaling < 0 || a->scaling > HCP_ROPE_SCALING_DIVIDED)
+    return fail(HCP_EUNSUPPORTED, "%s: scaling %d", who, a->scaling);
+  if (!(a->base > 1.0) || !std::isfinite(a->base) || !std::isfinite(a->attention_factor))
+    return fail(HCP_EINVAL, "%s: base must be finite and above 1", who);
+  if (scaled && a->scaling != HCP_ROPE_SCALING_DIVIDED &&
+      (!(a->factor > 0.0) || !std::isfinite(a->factor)))
+    return fail(HCP_EINVAL, "%s: factor must be finite and above 0", who);
+  const bool fitted = a->scaling == HCP_ROPE_SCALING_LLAMA3 || a->scaling == HCP_ROPE_SCALING_YARN;
+  if (fitted && (!(a->original > 0.0) || !std::isfinite(a->original)))
+    return fail(HCP_EINVAL, "%s: original must be finite and above 0", who);
+  if (a->scaling == HCP_ROPE_SCALING_LLAMA3 && !(a->high_freq > a->low_freq && a->low_freq > 0.0))
+    return fail(HCP_EINVAL, "%s: high_freq must be above low_freq, and that above 0", who);
+  if (a->scaling == HCP_ROPE_SCALING_YARN && !(a->beta_fast >= a->beta_slow && a->beta_slow > 0.0))
+    return fail(HCP_EINVAL, "%s: beta_fast must not be below beta_slow, and that above 0", who);
+  if (a->scaling == HCP_ROPE_SCALING_DIVIDED && !a->divisors)
+    return fail(HCP_EINVAL, "%s: null divisors", who);
+  if (a->num_positions == 0) return HCP_OK;
+  const int64_t es = a->dtype == HCP_DTYPE_F32 ? 4 : 2;
+  if (!a->out || !aligned16(a->out) || a->stride * es % 16)
+    return fail(HCP_EINVAL, "%s: out not in 16-byte rows", who);
+  if (!rows_apart(a->rot, {{a->num_positions, a->stride}}))
+    return fail(HCP_EINVAL, "%s: rows of out on top of each other", who);
+  hcp::RopeTableParams p{};
+  p.out = a->out;
+  p.stride = a->stride;
+  p.num_positions = a->num_positions;
+  p.rot = a->rot;
+  p.factor = static_cast<float>(a->attention_factor);
+  constexpr double kTurn = 6.283185307179586;
+  // the dimension whose frequency turns beta times in `original` positions
+  auto dim = [&](double beta) {
+    return a->rot * std::log(a->original / (beta * kTurn)) / (2 * std::log(a->base));
+  };
+  double low = 0, high = 0;
+  if (a->scaling == HCP_ROPE_SCALING_YARN) {
+    low = std::max(std::floor(dim(a->beta_fast)), 0.0);
+    high = std::min(std::ceil(dim(a->beta_slow)), a->rot - 1.0);
+  }
+  for (int i = 0; i < a->rot / 2; ++i) {
+    double f = std::pow(a->base, -2.0 * i / a->rot);
+    switch (a->scaling) {
+      case HCP_ROPE_SCALING_LINEAR: f /= a->factor; break;
+      case HCP_ROPE_SCALING_LLAMA3: {
+        const double turns = a->original * f / kTurn;
+        const double keep = std::min(std::max((turns - a->low_freq) / (a->high_freq - a->low_freq),
+                                              0.0), 1.0);
+        f = keep * f + (1 - keep) * f / a->factor;
+        break;
+      }
+      case HCP_ROPE_SCALING_YARN: {
+        const double far = std::min(std::max((i - low) / std::max(high - low, 0.001), 0.0), 1.0);
+        f = f / a->factor * far + f * (1 - far);
+        break;
+      }
+      case HCP_ROPE_SCALING_DIVIDED: {
+        if (!(a->divisors[i] > 0.0) || !std::isfinite(a->divisors[i]))
+          return fail(HCP_EINVAL, "%s: divisors must be finite and above 0", who);
+        f /= a->divisors[i];
+        break;
+      }
+      default: break;
+    }
+    p.turns[i] = f / kTurn;
+  }
+  return launch_status(hcp::launch_rope_table(p, a->dtype, static_cast<hipStream_t>(stream)), who);
+}
+
 }  // extern "C"

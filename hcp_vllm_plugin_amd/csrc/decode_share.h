@@ -46,11 +46,18 @@ __device__ __forceinline__ void paged_lens(const void* lens, bool wide, int r, i
 // workgroup of NT threads gets its share in sm_cut: first sequence (-1: none) and
 // first chunk of it, last sequence and the end in its chunks; sm_len / sm_all
 // [kDecMaxSeqs] get the keys of every sequence (sm_all -1: HCP_LEN_NOT_RUN).
-// STARTS: p.starts counts.  Ends with a barrier.
-template <int NT, int START, int LEAST, int LATE, bool STARTS, typename Count>
+// STARTS: p.starts counts.  last(p, j, seen): how many of its `seen` keys the
+// thread's j-th sequence looks at, the last ones.  Ends with a barrier.
+struct LastWindow {
+  __device__ __forceinline__ int operator()(const PagedDecParams& p, int, int seen) const {
+    return p.window > 0 && seen > p.window ? p.window : seen;
+  }
+};
+template <int NT, int START, int LEAST, int LATE, bool STARTS, typename Count,
+          typename Last = LastWindow>
 __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, int* sm_len,
                                              int* sm_all, int (*sm_w)[NT / 64], int* sm_cut,
-                                             Count count) {
+                                             Count count, Last last = {}) {
   constexpr int EPT = kDecMaxSeqs / NT;  // sequences per thread of the prefix sum
   constexpr int W = NT / 64;
   const int n = p_.num_seqs;
@@ -75,7 +82,7 @@ __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, i
         seen = s <= 0 ? all : s < all ? all - static_cast<int>(s) : 0;
       }
     }
-    const int len = p_.window > 0 && seen > p_.window ? p_.window : seen;
+    const int len = last(p_, j, seen);
     if (r < n) {
       sm_all[r] = given == HCP_LEN_NOT_RUN ? -1 : all;
       sm_len[r] = len;

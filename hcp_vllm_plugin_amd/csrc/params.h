@@ -147,6 +147,72 @@ struct PagedDecParams {
                          // 0, -2: HCP_LEN_NOT_RUN)
 };
 
+// Decode of sequences with several query tokens each (decode_drafts.hip).
+struct DraftParams {
+  PagedDecParams p;        // p.window 0: the tokens' windows are `window`; p.d.head_chunks: of rows
+  const void* row_starts;  // [num_seqs + 1], as lens: the sequences' rows of q and out
+  int64_t q_rows;
+  int32_t max_tokens;      // query tokens of a sequence, at most
+  int32_t window;          // keys that a token sees (0: all up to its own)
+  int32_t num_slots;       // of the workspace, max_tokens * num_heads partials each
+};
+// Workgroups of a CU, by LDS and by the registers of RT tiles.
+__host__ __device__ constexpr int drafts_per_cu(bool fp4, int padded_dim, int tiles) {
+  return fp4 ? (padded_dim == 64 ? (tiles == 1 ? 4 : 2) : padded_dim == 128 ? 2 : tiles == 1 ? 2 : 1)
+             : (padded_dim == 64 && tiles <= 2 ? 2 : 1);
+}
+struct DraftOut {
+  void* out;
+  int64_t stride_tok, stride_head;
+  float* lse;
+  int64_t lse_stride_head;
+};
+
+constexpr int kRopeMaxFrequencies = 128;  // rot of 256
+struct RopeTableParams {
+  void* out;
+  int64_t stride, num_positions;
+  int32_t rot;
+  float factor;                       // of the cosines and sines
+  double turns[kRopeMaxFrequencies];  // frequencies over 2 pi
+};
+
+// Verification of drafted tokens (verify.hip).
+constexpr int kVerMaxTokens = HCP_VERIFY_MAX_TOKENS;
+constexpr int kVerStatSlice = 8192, kVerSumSlice = 2048;  // entries of a row to a workgroup
+struct VerifyStat {  // of a slice of a row
+  float top;
+  int32_t index;
+  double sum;
+};
+struct VerifyRow {  // what a sequence's last token is drawn from
+  int64_t row;      // of the target; -1: nothing to draw
+  double inverse;   // 1 / temperature
+  float top;
+  int32_t taken;    // drafts accepted
+  int32_t draft;    // the refused one, -1: none, or no token
+  int32_t refused;
+};
+struct VerifyParams {
+  const void* target;
+  int64_t row_bytes, num_rows;
+  const void* tokens;  // [num_rows]: the drafts, each in the row after the one that judges it
+  const void* row_starts;
+  const float* uniform;
+  int64_t uniform_stride;
+  const float* draft_probs;  // NULL: the drafts are certain
+  int64_t q_stride_seq, q_stride_row;
+  const float* temperature;  // NULL: 1
+  void* out;                 // [num_seqs, max_tokens], as tokens
+  int32_t* num_out;
+  VerifyStat* stats;  // [num_seqs][max_tokens][stat_slices]
+  VerifyRow* rows;    // [num_seqs]
+  double* sums;       // [num_seqs][sum_slices]
+  double* residuals;
+  int32_t vocab, num_seqs, max_tokens, stat_slices, sum_slices;
+  bool tokens_wide, starts_wide;
+};
+
 struct MergeParams {
   void* out;
   int64_t o_stride_tok, o_stride_head;
@@ -329,10 +395,16 @@ hipError_t launch_decode_reduce(const RedParams& rp, int num_wgs, int head_dim, 
                                 hipStream_t st);
 hipError_t launch_decode_fp4(const PagedDecParams& p, const RedParams& rp, int dtype,
                              hipStream_t st);
+// tiles: of 16 rows (query tokens times heads of a KV head) that a workgroup holds
+hipError_t launch_drafts16(const DraftParams& p, int tiles, int dtype, hipStream_t st);
+hipError_t launch_drafts_fp4(const DraftParams& p, int tiles, int dtype, hipStream_t st);
+hipError_t launch_drafts_reduce(const DraftParams& p, const DraftOut& o, int dtype, hipStream_t st);
 hipError_t launch_fp4_write(const Fp4Params& p, int dtype, hipStream_t st);
 hipError_t launch_fp4_read(const Fp4Params& p, int dtype, hipStream_t st);
 hipError_t launch_fp4_gather(const Fp4GatherParams& p, int dtype, hipStream_t st);
 hipError_t launch_qk_rope(RopeParams p, int dtype, int cache, hipStream_t st);
+hipError_t launch_rope_table(const RopeTableParams& p, int dtype, hipStream_t st);
+hipError_t launch_verify(const VerifyParams& p, int dtype, bool probs, hipStream_t st);
 hipError_t launch_step_tables(const StepTablesParams& p, hipStream_t st);
 hipError_t launch_merge(const MergeParams& p, hipStream_t st);
 hipError_t launch_cache_write(const CacheParams& p, bool slots_i64, hipStream_t st);

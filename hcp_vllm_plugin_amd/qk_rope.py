@@ -6,12 +6,15 @@ every query and key head, the rotation of its first columns by the token's
 position, and (given a cache) the write that ``kv_cache.reshape_and_cache`` would
 do, into either 16-bit layout or the 4-bit cache.  The reference leaves the first
 two to the model and does the third in ``do_kv_cache_update``
-(hcp_vllm_plugin/ring_backend.py:501-539).
+(hcp_vllm_plugin/ring_backend.py:501-539).  ``rope_table`` makes the table of
+cosines and sines that it reads, for contexts past the trained one too.
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
+from collections.abc import Mapping
 
 import torch
 
@@ -19,7 +22,7 @@ from . import _lib
 from .kv_cache import _cache_desc, check_slots
 from .varlen import fp4_desc, rows_apart
 
-__all__ = ["qk_norm_rope"]
+__all__ = ["qk_norm_rope", "rope_table"]
 
 _INDEX = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
@@ -166,3 +169,96 @@ def qk_norm_rope(
         fp4, t, eps, h, hkv, d, rot, code, code if w_type == dt else _lib.DTYPE_F32,
         _lib.DTYPE_F32 if wide_table else code, pos_code, slot_code, bool(interleaved), kind, 0))
     return query_out, key_out
+
+
+_SCALINGS = {"default": 0, "linear": 1, "llama3": 2, "yarn": 3, "dynamic": 0, "longrope": 4}
+
+
+def _scaling_fields(scaling: Mapping, rot: int, base: float, positions: int):
+    """(base, kind, factor, original, low, high, fast, slow, attention factor, divisors)."""
+    kind = scaling.get("rope_type", scaling.get("type"))
+    if kind not in _SCALINGS:
+        raise ValueError(f"rope_type {kind!r} is none of {', '.join(_SCALINGS)}")
+    number = {k: float(x) for k, x in scaling.items() if isinstance(x, (int, float))}
+
+    def need(name):
+        if name not in number:
+            raise ValueError(f"scaling {kind!r} needs {name!r}")
+        return number[name]
+
+    factor = need("factor") if kind in ("linear", "llama3", "yarn", "dynamic") else 1.0
+    trained = need("original_max_position_embeddings") if kind not in ("default", "linear") else 0.0
+    low = high = fast = slow = 0.0
+    attention, divisors = 1.0, None
+    if kind == "llama3":
+        low, high = need("low_freq_factor"), need("high_freq_factor")
+    elif kind == "yarn":
+        fast, slow = number.get("beta_fast", 32.0), number.get("beta_slow", 1.0)
+        attention = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    elif kind == "dynamic":
+        if not trained > 0 or not factor >= 1 or rot == 2:
+            raise ValueError("dynamic: factor from 1 and a context above 0")
+        if positions > trained:
+            base *= (factor * positions / trained - (factor - 1)) ** (rot / (rot - 2))
+    elif kind == "longrope":
+        if not trained > 1:
+            raise ValueError("longrope: a context above 1")
+        name = "long_factor" if positions > trained else "short_factor"
+        given = scaling.get(name)
+        if given is None or len(given) != rot // 2:
+            raise ValueError(f"longrope needs {name!r}, rot / 2 numbers")
+        divisors = (ctypes.c_double * (rot // 2))(*given)
+        ratio = number.get("factor", positions / trained)
+        attention = math.sqrt(1 + math.log(ratio) / math.log(trained)) if ratio > 1 else 1.0
+    attention = number.get("attention_factor", attention)
+    return base, _SCALINGS[kind], factor, trained, low, high, fast, slow, attention, divisors
+
+
+def rope_table(
+    max_positions: int,
+    rot: int,
+    *,
+    base: float = 10000.0,
+    scaling: Mapping | None = None,
+    dtype: torch.dtype = torch.float32,
+    device: torch.device | str | int = "cuda",
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The table ``[max_positions, rot]`` that ``qk_norm_rope`` reads: row t holds ``rot / 2``
+    cosines of ``t f_i``, then as many sines, ``f_i = base ** (-2 i / rot)``; angles in 64
+    bits, values to 2^-22, rounded to ``dtype`` (float32, fp16 or bf16).
+
+    ``scaling`` is a model's ``rope_scaling``, by its "rope_type": "linear" ("factor"),
+    "llama3" ("factor", "low_freq_factor", "high_freq_factor",
+    "original_max_position_embeddings"), "yarn" ("factor", the same context; "beta_fast" 32,
+    "beta_slow" 1), "dynamic" ("factor", the context; another base for tables longer than
+    that), "longrope" ("short_factor" and "long_factor", rot / 2 divisors each, the context:
+    the long ones for tables longer than that), or "default".  "yarn" and "longrope"
+    multiply cosines and sines by ``0.1 ln(factor) + 1`` and ``sqrt(1 + ln(factor) /
+    ln(context))``, or by "attention_factor" where that is given ("longrope" without a
+    "factor": ``max_positions`` over the context).
+
+    ``out`` is written where it is given ``[max_positions, rot]``, of its dtype."""
+    if rot <= 0 or rot % 16 or rot > 256:
+        raise ValueError("rot must be a multiple of 16 up to 256")
+    if max_positions < 0:
+        raise ValueError("max_positions must not be negative")
+    if not (base > 1 and math.isfinite(base)):
+        raise ValueError("base must be finite and above 1")
+    fields = (base, 0, 1.0, 0.0, 0.0, 0.0, 0.0, 0.0, 1.0, None) if scaling is None else \
+        _scaling_fields(scaling, rot, base, max_positions)
+    if out is None:
+        out = torch.empty(max_positions, rot, dtype=dtype, device=device)
+    elif out.shape != (max_positions, rot) or out.stride(1) != 1:
+        raise ValueError("out must be [max_positions, rot] with contiguous rows")
+    code = _lib.DTYPE_F32 if out.dtype == torch.float32 else _TYPES.get(out.dtype)
+    if code is None:
+        raise ValueError("the table must be float32, float16 or bfloat16")
+    index = out.get_device()
+    if index < 0:
+        raise ValueError("the table must be on a GPU")
+    base, kind, factor, trained, low, high, fast, slow, attention, divisors = fields
+    _lib.launch(_lib.lib().hcp_rope_table, index, "hcp_rope_table", _lib.pack_rope_table(
+        out.data_ptr(), out.stride(0), max_positions, base, factor, trained, low, high, fast, slow,
+        attention, 0 if divisors is None else ctypes.addressof(divisors), rot, code, kind, 0))
+    return out

@@ -845,6 +845,110 @@ typedef struct hcp_step_tables_args {
 
 int hcp_step_tables(const hcp_step_tables_args* args, void* stream);
 
+/*
+ * ---- A decode step with drafted tokens ----
+ *
+ * Split-KV decode of sequences with up to max_tokens query tokens each, the last ones
+ * of their keys: token t of sequence r's n = row_starts[r + 1] - row_starts[r] (its row
+ * of q and out row_starts[r] + t) sees keys j < seq_lens[r] - n + 1 + t, of these the
+ * last `window`.  No counterpart in the reference, which runs such rows through its
+ * prefill kernel.  decode: as for hcp_decode_paged (fp4 0) or hcp_decode_fp4 (fp4 1),
+ * seq_starts NULL; its lse [num_heads][lse_stride_head] by rows, keep_nan not read (a
+ * NaN score makes its row NaN).
+ *   row_starts   DEVICE [num_seqs + 1], of lens_dtype
+ *   q_rows       rows of q; tokens in rows past them, or past max_tokens of their
+ *                sequence, are not run, and no other row of out and lse is written
+ * A row that sees no key gets 0 and LSE -inf.  What a row does not see does not reach
+ * it, whatever it is.  max_tokens is at most HCP_DRAFTS_MAX_TOKENS.
+ */
+#define HCP_DRAFTS_MAX_TOKENS 64
+typedef struct hcp_decode_drafts_args {
+  hcp_decode_paged_args decode;
+  const void* row_starts;
+  int64_t q_rows;
+  int32_t max_tokens;
+  int32_t fp4;
+} hcp_decode_drafts_args;
+
+size_t hcp_decode_drafts_workspace(int32_t num_seqs, int32_t max_tokens, int32_t num_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, int32_t fp4);
+int hcp_decode_drafts(const hcp_decode_drafts_args* args, void* stream);
+
+/*
+ * Verification of drafted tokens.  Sequence r has rows row_starts[r] .. row_starts[r + 1]
+ * - 1 of target and tokens, n of them (max_tokens at most are looked at): its newest
+ * token and n - 1 drafts.  Row i has weights w = exp((x - max x) / temperature[r]) with
+ * sum Z (probs: w = x, below 0 or infinite 0; -inf and NaN have no weight) and judges
+ * the token d in the row after it: it is accepted while uniform[r][i] q(d) Z < w(d), q =
+ * draft_probs[r][i] or 1.  One token more comes from max(w - q Z, 0) of the row that
+ * refused (w without d where there is no q; w where nothing is left), or from the last
+ * row's w: the first index at which the running sum passes uniform[r][max_tokens - 1]
+ * times the whole.  With a temperature that is not above 0 the row's largest entry, the
+ * lowest index of equal ones, is what a draft has to be, and the token.  All of it as in
+ * 64 bits.
+ *   target       DEVICE [num_rows, vocab] F16 / BF16 / F32, rows row_stride elements apart
+ *   tokens       DEVICE [num_rows] I32 / I64; a draft that is no token is refused
+ *   row_starts   DEVICE [num_seqs + 1] I32 / I64
+ *   uniform      DEVICE float [num_seqs][max_tokens], rows uniform_stride apart, in [0, 1)
+ *   draft_probs  DEVICE float [num_seqs][max_tokens - 1][vocab], or NULL
+ *   temperature  DEVICE float [num_seqs], or NULL: 1
+ *   out          [num_seqs][max_tokens], as tokens: the accepted ones, the one more, -1
+ *   num_out      int32 [num_seqs]: how many (a row without any weight gives no token, a
+ *                sequence without rows 0)
+ * workspace: hcp_verify_workspace bytes, 16-byte aligned.
+ */
+#define HCP_VERIFY_MAX_TOKENS 64
+typedef struct hcp_verify_args {
+  const void* target;
+  int64_t row_stride, num_rows;
+  const void* tokens;
+  const void* row_starts;
+  const float* uniform;
+  int64_t uniform_stride;
+  const float* draft_probs;
+  int64_t q_stride_seq, q_stride_row;
+  const float* temperature;
+  void* out;
+  int32_t* num_out;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t vocab, num_seqs, max_tokens;
+  int32_t dtype, tokens_dtype, starts_dtype, probs, reserved;
+} hcp_verify_args;
+
+size_t hcp_verify_workspace(int32_t num_seqs, int32_t max_tokens, int32_t vocab);
+int hcp_verify_drafts(const hcp_verify_args* args, void* stream);
+
+/*
+ * The table that hcp_qk_norm_rope reads: out [num_positions, rot], rows `stride`
+ * elements apart, row t = cos(t f_i) a for i < rot / 2, then sin(t f_i) a; angles in 64
+ * bits, values to 2^-22, then rounded.  f_i = base^(-2 i / rot), by `scaling`:
+ *   0 none
+ *   1 linear   f / factor
+ *   2 llama3   f / factor where a wave is longer than original / low_freq, f where it is
+ *              shorter than original / high_freq, between them mixed by (original f /
+ *              2 pi - low_freq) / (high_freq - low_freq)
+ *   3 yarn     f and f / factor mixed by a ramp over i, from the dimension that turns
+ *              beta_fast times in `original` positions to the one that turns beta_slow
+ *              times, both rounded outwards
+ *   4 divided  f_i / divisors[i] (HOST [rot / 2])
+ * and a = attention_factor.  rot a multiple of 16 up to 256; rows 16-byte aligned.
+ */
+#define HCP_ROPE_SCALING_NONE 0
+#define HCP_ROPE_SCALING_LINEAR 1
+#define HCP_ROPE_SCALING_LLAMA3 2
+#define HCP_ROPE_SCALING_YARN 3
+#define HCP_ROPE_SCALING_DIVIDED 4
+typedef struct hcp_rope_table_args {
+  void* out;
+  int64_t stride, num_positions;
+  double base, factor, original, low_freq, high_freq, beta_fast, beta_slow, attention_factor;
+  const double* divisors;
+  int32_t rot, dtype, scaling, reserved;
+} hcp_rope_table_args;
+
+int hcp_rope_table(const hcp_rope_table_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
