@@ -2023,7 +2023,7 @@ int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
     return fail(HCP_EUNSUPPORTED, "%s: rot %d (a multiple of 16 up to 256)", who, a->rot);
   if (!dtype16(a->dtype) && a->dtype != HCP_DTYPE_F32)
     return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
-  // (positions times frequencies stay exact to 2^-24 of a turn)
+  // (a frequency in 64 bits is off by 2^-56 turns at most, a position by 2^-28)
   if (a->num_positions < 0 || a->num_positions > int64_t{1} << 28)
     return fail(HCP_EINVAL, "%s: bad sizes", who);
   const bool scaled = a->scaling != HCP_ROPE_SCALING_NONE;
@@ -2089,7 +2089,8 @@ int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
       }
       default: break;
     }
-    p.turns[i] = f / kTurn;
+    const double turns = std::ldexp(std::fmod(f / kTurn, 1.0), 64);
+    p.turns[i] = turns < 0x1p64 ? static_cast<uint64_t>(turns) : 0;
   }
   return launch_status(hcp::launch_rope_table(p, a->dtype, static_cast<hipStream_t>(stream)), who);
 }

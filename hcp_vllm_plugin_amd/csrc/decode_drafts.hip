@@ -650,8 +650,9 @@ __device__ __forceinline__ void drafts_split_body(
 
   // ---- combine the W waves, a tile at a time in the chunk buffers ----
   wait_vmcnt<0>();  // the last loads still write there
-  constexpr int HW = W / 2;
-  static_assert(sizeof(float) * HW * 16 * (D + 4) <= W * K::BYTES, "combine staging");
+  // (all of them in bufO where there is room)
+  constexpr int HW = sizeof(float) * W * 16 * (D + 4) <= W * K::BYTES ? 0 : W / 2;
+  static_assert(sizeof(float) * (W - HW) * 16 * (D + 4) <= W * K::BYTES, "combine staging");
   float (*const so_e)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(&bufE[0][0]);
   float (*const so_o)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(&bufO[0][0]);
   float (*const mine)[D + 4] = wave < HW ? so_e[wave] : so_o[wave - HW];
@@ -671,19 +672,23 @@ __device__ __forceinline__ void drafts_split_body(
         *reinterpret_cast<f32x4*>(&mine[c16][NU * (4 * g4 + j) + u]) =
             f32x4{oacc[i][u][j], oacc[i][u + 1][j], oacc[i][u + 2][j], oacc[i][u + 3][j]};
     __syncthreads();
-    for (int idx = tid; idx < 16 * D; idx += 64 * W) {
-      const int h = idx / D, d = idx % D, rho = rho0 + 16 * i + h;
+    for (int idx = tid; idx < 16 * (D / 4); idx += 64 * W) {
+      const int h = idx / (D / 4), d = idx % (D / 4) * 4, rho = rho0 + 16 * i + h;
       if (rho >= rows) break;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < W; ++w) M = fmaxf(M, sm_m[w][16 * i + h]);
-      const float Mu = M == -INFINITY ? 0.f : M;
-      float L = 0.f, O = 0.f;
+      float mw[W], M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float sc = fast_exp2(sm_m[w][16 * i + h] - Mu);
+        mw[w] = sm_m[w][16 * i + h];
+        M = fmaxf(M, mw[w]);
+      }
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+      f32x4 O{};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float sc = fast_exp2(mw[w] - Mu);
         L += sm_l[w][16 * i + h] * sc;
-        O += (w < HW ? so_e[w] : so_o[w - HW])[h][d] * sc;
+        O += *reinterpret_cast<const f32x4*>(&(w < HW ? so_e[w] : so_o[w - HW])[h][d]) * sc;
       }
       const int t = rho / G, hq = kvh * G + rho - t * G;
       if (*sm_odd) {  // what clean_v took out, for the rows that see it
@@ -691,12 +696,13 @@ __device__ __forceinline__ void drafts_split_body(
         for (int x0 = kb; x0 < ke; x0 += 32) {
           if (!(x0 + 32 > edge_hi || x0 < edge_lo)) continue;
           for (int key = x0 > lo ? x0 : lo; key < x0 + 32 && key < hi; ++key)
-            O += keys.odd_value(key, d);
+            for (int j = 0; j < 4; ++j) O[j] += keys.odd_value(key, d + j);
         }
       }
       const int64_t at = (static_cast<int64_t>(slot) * p.max_tokens + t) * p.p.d.num_heads + hq;
       const bool some = L != 0.f;  // a NaN too: it is the row's result
-      global_ptr(p.p.d.ws_o)[at * D + d] = some ? O / L : 0.f;
+      const float inv = some ? 1.f / L : 0.f;
+      *global_ptr(reinterpret_cast<f32x4*>(p.p.d.ws_o + at * D + d)) = some ? O * inv : f32x4{};
       if (d == 0) global_ptr(p.p.d.ws_lse)[at] = some ? M * kLn2 + __logf(L) : -INFINITY;
     }
   }
@@ -829,24 +835,33 @@ hipError_t launch_drafts16(const DraftParams& p, int tiles, int dtype, hipStream
   return launch_drafts_d<Keys16>(p, tiles, dtype, st);
 }
 
+// The largest of the wave's lanes, a NaN left out.
+__device__ __forceinline__ float wave_max32(float x) {
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
+  return x;
+}
+
 // Merge of a row's partials, a wave to each (sequence, token, head): out = sum_i w_i
 // O_i / sum_i w_i, w_i = exp(lse_i - max).  Lane i holds weight i, and every lane D /
-// 64 columns.  Bound by latency: the partials were just written.
+// 64 columns.  Bound by latency: the row's place and slots are fetched at once, then the
+// LSEs with the first 16 partials' columns, before any weight is known.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void drafts_reduce_kernel(DraftParams p, DraftOut o) {
-  constexpr int N = D / 64;
+  constexpr int N = D / 64, U = 16;
+  typedef float vf __attribute__((ext_vector_type(N == 1 ? 2 : N)));  // (of one: its first)
   const int lane = threadIdx.x & 63;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int heads = p.p.d.num_heads;
-  const int64_t st = unit / heads;
-  const int head = static_cast<int>(unit - st * heads);
-  const int seq = static_cast<int>(st / p.max_tokens), t = static_cast<int>(st % p.max_tokens);
+  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int st = unit / heads, head = unit - st * heads;
+  const int seq = st / p.max_tokens, t = st - seq * p.max_tokens;
   if (seq >= p.p.num_seqs) return;
-  int row0 = 0;
-  if (t >= draft_rows(p, draft_start(p, seq), draft_start(p, seq + 1), row0)) return;
+  const int64_t from = draft_start(p, seq), to = draft_start(p, seq + 1);
   // kept inside the workspace whatever stands there: a caller that changes the lengths
   // while the split kernel reads them leaves pairs unwritten
   const int a = p.p.seq_slots[2 * seq], z = p.p.seq_slots[2 * seq + 1];
+  int row0 = 0;
+  if (t >= draft_rows(p, from, to, row0)) return;
   const int p0 = a < 0 ? 0 : a < p.num_slots ? a : p.num_slots;
   const int n = (z < -2 ? -2 : z < p.num_slots ? z : p.num_slots - 1) - p0 + 1;
   if (n < 0) return;  // not run
@@ -854,41 +869,45 @@ __global__ __launch_bounds__(256) void drafts_reduce_kernel(DraftParams p, Draft
   const int64_t at = (static_cast<int64_t>(p0) * p.max_tokens + t) * heads + head;
   const float* lcol = p.p.d.ws_lse + at;
   const float* ocol = p.p.d.ws_o + at * D + N * lane;
-  float m = -INFINITY, S = 0.f, O[N] = {};
+  auto column = [&](int64_t i) __attribute__((always_inline)) {
+    vf x;
+    if constexpr (N == 1)
+      x = vf{*global_ptr(ocol + i * step * D), 0.f};
+    else
+      x = *global_ptr(reinterpret_cast<const vf*>(ocol + i * step * D));
+    return x;
+  };
+  float m = -INFINITY, S = 0.f;
+  vf O{};
   for (int i0 = 0; i0 < n; i0 += 64) {
     const int some = n - i0 < 64 ? n - i0 : 64;
-    const float l = lane < some ? lcol[(i0 + lane) * step] : -INFINITY;
-    float mn = l;  // (fmaxf leaves a NaN out: its weight is NaN whatever the maximum)
+    const float l = lane < some ? global_ptr(lcol)[(i0 + lane) * step] : -INFINITY;
+    vf v[U];
+    auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor(mn, x));
-    mn = fmaxf(m, mn);
+      for (int k = 0; k < U; ++k) v[k] = column(i0 + (i + k < some ? i + k : some - 1));
+    };
+    fetch(0);
+    // (the maximum leaves a NaN out: its weight is NaN whatever that is)
+    const float mn = fmaxf(m, wave_max32(l));
     const float ref = mn == -INFINITY ? 0.f : mn;
-    const float sc = m == -INFINITY ? 0.f : __expf(m - ref);
-    const float w = __expf(l - ref);
     // (what came before, where a NaN may stand with m still -inf, is kept)
-    S = m == -INFINITY ? S : S * sc;
-#pragma unroll
-    for (int j = 0; j < N; ++j) O[j] = m == -INFINITY ? O[j] : O[j] * sc;
+    const float sc = m == -INFINITY ? 1.f : __expf(m - ref);
+    const float w = __expf(l - ref);
+    S *= sc;
+    O *= sc;
     m = mn;
     float ws = w;
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) ws += __shfl_xor(ws, x);
     S += ws;
-    constexpr int U = 8;
     for (int i = 0; i < some; i += U) {
-      float v[U][N];
+      if (i > 0) fetch(i);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int q = i + k < some ? i + k : some - 1;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[k][j] = ocol[(i0 + q) * step * D + j];
-      }
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (i + k >= some) break;
-        const float wk = __shfl(w, i + k);
-#pragma unroll
-        for (int j = 0; j < N; ++j) O[j] = __builtin_fmaf(wk, v[k][j], O[j]);
+        const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (i + k) & 63));
+        // (past the last: not summed, whatever its columns hold)
+        O = i + k < some ? O + v[k] * wk : O;
       }
     }
   }
@@ -904,6 +923,7 @@ __global__ __launch_bounds__(256) void drafts_reduce_kernel(DraftParams p, Draft
 }
 
 hipError_t launch_drafts_reduce(const DraftParams& p, const DraftOut& o, int dtype, hipStream_t st) {
+  // (under 2^31: sequences, tokens and heads are bounded)
   const int64_t units = static_cast<int64_t>(p.p.num_seqs) * p.max_tokens * p.p.d.num_heads;
   const dim3 g(static_cast<unsigned>((units + 3) / 4)), b(256);
   const bool bf = dtype == HCP_DTYPE_BF16;

@@ -173,8 +173,8 @@ struct RopeTableParams {
   void* out;
   int64_t stride, num_positions;
   int32_t rot;
-  float factor;                       // of the cosines and sines
-  double turns[kRopeMaxFrequencies];  // frequencies over 2 pi
+  float factor;  // of the cosines and sines
+  uint64_t turns[kRopeMaxFrequencies];  // frequencies over 2 pi, the fraction times 2^64
 };
 
 // Verification of drafted tokens (verify.hip).
@@ -187,7 +187,7 @@ struct VerifyStat {  // of a slice of a row
 };
 struct VerifyRow {  // what a sequence's last token is drawn from
   int64_t row;      // of the target; -1: nothing to draw
-  double inverse;   // 1 / temperature
+  double rate;      // log2 e / temperature
   float top;
   int32_t taken;    // drafts accepted
   int32_t draft;    // the refused one, -1: none, or no token

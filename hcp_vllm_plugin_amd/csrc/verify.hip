@@ -38,51 +38,88 @@ __device__ __forceinline__ u32x4 ldg16_u(const void* p) {
   return *reinterpret_cast<gu32x4_u*>(reinterpret_cast<uintptr_t>(p));
 }
 
-// Elements 8 g .. 8 g + 7 of a row of v, `fill` past its end.
+// Elements 8 g .. 8 g + 7 of a row, all of them there.
+template <typename T>
+__device__ __forceinline__ void load8_full(const void* row, int g, float (&x)[8]) {
+  const T* const at = reinterpret_cast<const T*>(row) + 8 * static_cast<int64_t>(g);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 w = ldg16_u(at + 4 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * h + j] = __uint_as_float(w[j]);
+    }
+  } else {
+    const u32x4 w = ldg16_u(at);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = Elem<T>::to_float(static_cast<uint16_t>(w[j] & 0xffffu));
+      x[2 * j + 1] = Elem<T>::to_float(static_cast<uint16_t>(w[j] >> 16));
+    }
+  }
+}
+// The same of a row of v, `fill` past its end.
 template <typename T>
 __device__ __forceinline__ void load8(const void* row, int g, int v, float fill, float (&x)[8]) {
+  if (8 * g + 8 <= v) return load8_full<T>(row, g, x);
   const T* const at = reinterpret_cast<const T*>(row) + 8 * static_cast<int64_t>(g);
-  if (8 * g + 8 <= v) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4 w = ldg16_u(at + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * h + j] = __uint_as_float(w[j]);
-      }
-    } else {
-      const u32x4 w = ldg16_u(at);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = Elem<T>::to_float(static_cast<uint16_t>(w[j] & 0xffffu));
-        x[2 * j + 1] = Elem<T>::to_float(static_cast<uint16_t>(w[j] >> 16));
-      }
-    }
-    return;
-  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     x[j] = fill;
     if (8 * g + j < v) x[j] = static_cast<float>(global_ptr(at)[j]);
   }
 }
+// N of them, groups g, g + kVerThreads, ..; `end`: past the workgroup's last element.  (A
+// branch around every load would have each waited for by itself: 64 x 5 rows of 152064
+// bf16 took 21 us.)
+template <typename T, int N>
+__device__ __forceinline__ void load8s(const void* row, int g, int end, int v, float fill,
+                                       float (&x)[N][8]) {
+  if (end <= v) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) load8_full<T>(row, g + k * kVerThreads, x[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) load8<T>(row, g + k * kVerThreads, v, fill, x[k]);
+  }
+}
 
-// The weight of an entry x of a row with maximum `top`: of logits in 64 bits.  -inf and
-// NaN have none (and the target's probabilities below 0, or infinite).
+// 2^y for y <= 0 in 64 bits: the fraction's polynomial (Chebyshev interpolation on +-1/2,
+// off by 3.2e-16 of it), scaled.  Below -1100, and for a NaN: 0.  (As fast as a 32-bit
+// one would be: additions and products of 64 bits take no longer here.)
+__device__ __forceinline__ double exp2_64(double y) {
+  y = __builtin_fmax(y, -1100.0);
+  const double n = __builtin_rint(y), r = y - n;
+  double p = 7.072585949269224e-09;
+  p = __builtin_fma(p, r, 1.0208690299958306e-07);
+  p = __builtin_fma(p, r, 1.321544258792169e-06);
+  p = __builtin_fma(p, r, 1.5252657260200837e-05);
+  p = __builtin_fma(p, r, 0.0001540353044173605);
+  p = __builtin_fma(p, r, 0.0013333558230164974);
+  p = __builtin_fma(p, r, 0.009618129107606888);
+  p = __builtin_fma(p, r, 0.05550410866444772);
+  p = __builtin_fma(p, r, 0.24022650695910097);
+  p = __builtin_fma(p, r, 0.69314718055995);
+  p = __builtin_fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
+}
+
+// The weight of an entry x of a row with maximum `top`: of logits 2^((x - top) rate), rate =
+// log2 e / temperature.  -inf and NaN have none (they come out of the maximum above as
+// -1100), and next to an infinity nothing else has; probabilities below 0, or infinite,
+// have none.
 template <bool PROBS>
-__device__ __forceinline__ double weight(float x, float top, double inverse) {
+__device__ __forceinline__ double weight(float x, float top, double rate) {
   if constexpr (PROBS) return x > 0.f && x < INFINITY ? static_cast<double>(x) : 0.0;
-  if (!(x > -INFINITY)) return 0.0;
-  if (x == top) return 1.0;  // (an infinity too, and then nothing else)
-  if (top == INFINITY) return 0.0;
-  return exp((static_cast<double>(x) - static_cast<double>(top)) * inverse);
+  if (top == INFINITY) return x == INFINITY ? 1.0 : 0.0;
+  return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * rate);
 }
 
 struct VerifySeq {  // of one sequence, in LDS or registers
   int64_t row0;
   int n;       // its rows
   bool greedy;
-  double inverse;  // 1 / temperature
+  double rate;  // log2 e / temperature
 };
 __device__ __forceinline__ VerifySeq verify_seq(const VerifyParams& p, int b) {
   VerifySeq s;
@@ -99,7 +136,7 @@ __device__ __forceinline__ VerifySeq verify_seq(const VerifyParams& p, int b) {
   s.n = a < 0 || z <= a ? 0 : z - a < p.max_tokens ? static_cast<int>(z - a) : p.max_tokens;
   const float t = p.temperature != nullptr ? global_ptr(p.temperature)[b] : 1.f;
   s.greedy = !(t > 0.f);
-  s.inverse = s.greedy ? 1.0 : 1.0 / static_cast<double>(t);
+  s.rate = 1.4426950408889634 / (s.greedy ? 1.0 : static_cast<double>(t));
   return s;
 }
 __device__ __forceinline__ const char* target_row(const VerifyParams& p, int64_t row) {
@@ -110,6 +147,47 @@ __device__ __forceinline__ int64_t draft_token(const VerifyParams& p, int64_t ro
                        : global_ptr(reinterpret_cast<const int32_t*>(p.tokens))[row];
 }
 
+// Prefix sums over the wave's lanes (and their whole, by the last lane) by DPP moves: two
+// and an addition a step, where a shuffle through LDS takes as long as ten of them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(w), CTRL, ROWS, 0xf, false);
+  const uint32_t hi =
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(w >> 32), CTRL, ROWS, 0xf, false);
+  return x + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_prefix64(double x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr:1
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast:15
+  return dpp_add<0x143, 0xc>(x);  // row_bcast:31
+}
+__device__ __forceinline__ double last_lane(double x) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(w), 63);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(w >> 32), 63);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double x) { return last_lane(wave_prefix64(x)); }
+// Maximum over the wave's lanes; no NaN among them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float x) {
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(
+                      __float_as_int(-INFINITY), __float_as_int(x), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = dpp_max<0x111, 0xf>(x);
+  x = dpp_max<0x112, 0xf>(x);
+  x = dpp_max<0x114, 0xf>(x);
+  x = dpp_max<0x118, 0xf>(x);
+  x = dpp_max<0x142, 0xa>(x);
+  x = dpp_max<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
 // Larger value, or the lower index of equal ones.
 __device__ __forceinline__ void best_of(float& m, int& i, float om, int oi) {
   if (om > m || (om == m && oi < i)) {
@@ -118,6 +196,16 @@ __device__ __forceinline__ void best_of(float& m, int& i, float om, int oi) {
   }
 }
 
+// The largest of three, in one instruction; anything where one is a NaN.  (fmaxf would have
+// every value of a row made quiet first.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// A thread's 32 values stay in registers between the maximum and the weights.  A greedy
+// row needs the index of its maximum and no weights, another one no index.
 template <typename T, bool PROBS>
 __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyParams p) {
   __shared__ float sm_m[kVerWaves];
@@ -131,61 +219,99 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyParams 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float x[4][8];
   float m = -INFINITY;
+  load8s<T, 4>(row, slice * kStatSlice / 8 + tid, (slice + 1) * kStatSlice, p.vocab, -INFINITY, x);
+  if (!PROBS || s.greedy) {
+    float t = m;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) t = max3(t, x[k][e], x[k][e + 1]);
+    m = t;
+    // a NaN may have taken the place of the maximum
+    bool nan = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) nan |= __builtin_isunordered(x[k][e], x[k][e + 1]);
+    if (__builtin_amdgcn_ballot_w64(nan) != 0) {
+      m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!(x[k][e] > -INFINITY)) x[k][e] = -INFINITY;
+          m = x[k][e] > m ? x[k][e] : m;
+        }
+    }
+    m = wave_max(m);
+    if (lane == 0) sm_m[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kVerWaves; ++w) m = fmaxf(m, sm_m[w]);
+  }
   int at = 0x7fffffff;
+  double d = 0.0;
+  if (s.greedy) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    load8<T>(row, (slice * kStatSlice / 8) + k * kVerThreads + tid, p.vocab, -INFINITY, x[k]);
+    for (int k = 3; k >= 0; --k)
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+      for (int e = 7; e >= 0; --e)
+        if (x[k][e] == m) at = slice * kStatSlice + (k * kVerThreads + tid) * 8 + e;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (x[k][e] > m) {  // (the first of equal ones; no NaN)
-        m = x[k][e];
-        at = slice * kStatSlice + (k * kVerThreads + tid) * 8 + e;
+    for (int w = 32; w > 0; w >>= 1) {
+      const int o = __shfl_xor(at, w);
+      at = o < at ? o : at;
+    }
+    if (lane == 0) sm_i[wave] = at;
+  } else {
+    float sum = 0.f;
+    if constexpr (PROBS) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += x[k][e] > 0.f && x[k][e] < INFINITY ? x[k][e] : 0.f;
+    } else if (m == INFINITY) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += x[k][e] == INFINITY ? 1.f : 0.f;
+    } else if (m > -INFINITY) {
+      // (x - m) c in one fma: what m c loses to rounding is the same power for all
+      const float c = fminf(static_cast<float>(s.rate), 0x1p126f);
+      const float mc = m * c, lost = __builtin_fmaf(m, c, -mc);
+      if (c > 0.f && fabsf(mc) < 0x1p100f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += fast_exp2(__builtin_fmaf(x[k][e], c, -mc));
+        sum *= fast_exp2(-lost);
+      } else {  // (a NaN, of -inf times 0, to 0)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += fast_exp2(fmaxf((x[k][e] - m) * c, -INFINITY));
       }
-#pragma unroll
-  for (int w = 32; w > 0; w >>= 1) best_of(m, at, __shfl_xor(m, w), __shfl_xor(at, w));
-  if (lane == 0) {
-    sm_m[wave] = m;
-    sm_i[wave] = at;
+    }
+    d = wave_sum(sum);
+    if (lane == 0) sm_s[wave] = d;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kVerWaves; ++w) best_of(m, at, sm_m[w], sm_i[w]);
-  const float c = static_cast<float>(s.inverse * 1.4426950408889634);
-  float sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (PROBS)
-        sum += x[k][e] > 0.f && x[k][e] < INFINITY ? x[k][e] : 0.f;
-      else
-        sum += !(x[k][e] > -INFINITY) ? 0.f
-               : x[k][e] == m         ? 1.f
-               : m == INFINITY        ? 0.f
-                                      : fast_exp2((x[k][e] - m) * c);
-    }
-  double d = sum;
-#pragma unroll
-  for (int w = 32; w > 0; w >>= 1) d += __shfl_xor(d, w);
-  if (lane == 0) sm_s[wave] = d;
-  __syncthreads();
   if (tid == 0) {
-    d = 0.0;
+    VerifyStat o{m, 0x7fffffff, 0.0};
 #pragma unroll
-    for (int w = 0; w < kVerWaves; ++w) d += sm_s[w];
-    VerifyStat& o = p.stats[static_cast<int64_t>(unit) * p.stat_slices + slice];
-    o.top = m;
-    o.index = at;
-    o.sum = d;
+    for (int w = 0; w < kVerWaves; ++w) {
+      if (s.greedy)
+        o.index = sm_i[w] < o.index ? sm_i[w] : o.index;
+      else
+        o.sum += sm_s[w];
+    }
+    p.stats[static_cast<int64_t>(unit) * p.stat_slices + slice] = o;
   }
 }
 
 // Sum over the workgroup of every thread's x, in a fixed order.
 __device__ __forceinline__ double block_sum(double x, double* sm) {
-#pragma unroll
-  for (int w = 32; w > 0; w >>= 1) x += __shfl_xor(x, w);
+  x = wave_sum(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = x;
   __syncthreads();
@@ -204,28 +330,43 @@ template <typename T, bool PROBS>
 __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams p) {
   __shared__ float sm_top[kVerMaxTokens];
   __shared__ int sm_at[kVerMaxTokens];
-  __shared__ double sm_z[kVerMaxTokens];
+  __shared__ double sm_z[kVerMaxTokens], sm_uq[kVerMaxTokens], sm_w[kVerMaxTokens];
   __shared__ double sm_s[kVerWaves];
+  __shared__ uint64_t sm_ok, sm_near;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VerifySeq s = verify_seq(p, b);
+  // lane i of every wave looks at draft i: fetched while the slices' sums are
+  const bool mine = lane + 1 < s.n;
+  const int64_t d = mine ? draft_token(p, s.row0 + lane + 1) : -1;
+  const bool token = d >= 0 && d < p.vocab;
+  float xd = -INFINITY;
+  double uq = 0.0;
+  if (token && !s.greedy) {
+    xd = static_cast<float>(
+        global_ptr(reinterpret_cast<const T*>(target_row(p, s.row0 + lane)))[d]);
+    uq = global_ptr(p.uniform)[b * p.uniform_stride + lane];
+    if (p.draft_probs != nullptr)
+      uq *= static_cast<double>(
+          global_ptr(p.draft_probs)[b * p.q_stride_seq + lane * p.q_stride_row + d]);
+  }
   // the rows' maxima and sums from those of their slices
   for (int j = wave; j < s.n; j += kVerWaves) {
     const VerifyStat* const st =
         p.stats + (static_cast<int64_t>(b) * p.max_tokens + j) * p.stat_slices;
-    float m = -INFINITY;
-    int at = 0x7fffffff;
-    for (int i = lane; i < p.stat_slices; i += 64) best_of(m, at, st[i].top, st[i].index);
+    VerifyStat own{-INFINITY, 0x7fffffff, 0.0};  // of this lane's first slice
+    if (lane < p.stat_slices) own = global_ptr(st)[lane];
+    float m = own.top;
+    int at = own.index;
+    for (int i = lane + 64; i < p.stat_slices; i += 64)
+      best_of(m, at, global_ptr(st)[i].top, global_ptr(st)[i].index);
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) best_of(m, at, __shfl_xor(m, w), __shfl_xor(at, w));
-    double z = 0.0;
-    for (int i = lane; i < p.stat_slices; i += 64) {
-      if constexpr (PROBS)
-        z += st[i].sum;
-      else if (st[i].sum > 0.0)
-        z += st[i].sum * weight<false>(st[i].top, m, s.inverse);
-    }
-#pragma unroll
-    for (int w = 32; w > 0; w >>= 1) z += __shfl_xor(z, w);
+    auto part = [&](const VerifyStat& o) __attribute__((always_inline)) {
+      return PROBS ? o.sum : o.sum > 0.0 ? o.sum * weight<false>(o.top, m, s.rate) : 0.0;
+    };
+    double z = part(own);
+    for (int i = lane + 64; i < p.stat_slices; i += 64) z += part(global_ptr(st)[i]);
+    z = wave_sum(z);
     if (lane == 0) {
       sm_top[j] = m;
       sm_at[j] = at;
@@ -233,81 +374,90 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams
     }
   }
   __syncthreads();
+  if (wave == 0) {
+    bool ok = false, near = false;
+    if (token) {
+      if (s.greedy) {
+        ok = sm_at[lane] == d;
+      } else {
+        const double w = weight<PROBS>(xd, sm_top[lane], s.rate), v = uq * sm_z[lane];
+        ok = v < w;
+        near = fabs(v - w) <= kSumError * w;
+        sm_uq[lane] = uq;
+        sm_w[lane] = w;
+      }
+    }
+    const uint64_t oks = __builtin_amdgcn_ballot_w64(ok), nears = __builtin_amdgcn_ballot_w64(near);
+    if (lane == 0) {
+      sm_ok = oks;
+      sm_near = nears;
+    }
+  }
+  __syncthreads();
   int taken = 0;
   for (; taken + 1 < s.n; ++taken) {  // (the same in every thread)
-    const int j = taken;
-    const int64_t d = draft_token(p, s.row0 + j + 1);
-    if (d < 0 || d >= p.vocab) break;
-    if (s.greedy) {
-      if (sm_at[j] != d) break;
-      continue;
-    }
-    const char* const row = target_row(p, s.row0 + j);
-    const double w =
-        weight<PROBS>(static_cast<float>(global_ptr(reinterpret_cast<const T*>(row))[d]), sm_top[j],
-                      s.inverse);
-    double uq = global_ptr(p.uniform)[b * p.uniform_stride + j];
-    if (p.draft_probs != nullptr)
-      uq *= static_cast<double>(
-          global_ptr(p.draft_probs)[b * p.q_stride_seq + j * p.q_stride_row + d]);
-    double z = sm_z[j];
-    if (fabs(uq * z - w) <= kSumError * w) {  // too near to tell: the row in 64 bits
+    if (sm_near >> taken & 1) {  // too near to tell: the row in 64 bits
+      const char* const row = target_row(p, s.row0 + taken);
       double x = 0.0;
       for (int g = tid; g < (p.vocab + 7) / 8; g += kVerThreads) {
         float e[8];
         load8<T>(row, g, p.vocab, -INFINITY, e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x += weight<PROBS>(e[k], sm_top[j], s.inverse);
+        for (int k = 0; k < 8; ++k) x += weight<PROBS>(e[k], sm_top[taken], s.rate);
       }
-      z = block_sum(x, sm_s);
+      if (!(sm_uq[taken] * block_sum(x, sm_s) < sm_w[taken])) break;
+    } else if (!(sm_ok >> taken & 1)) {
+      break;
     }
-    if (!(uq * z < w)) break;
   }
   // tokens, and what the row that is drawn from is
   const float top = s.n > 0 ? sm_top[taken] : -INFINITY;
-  const bool none = s.n == 0 || (PROBS ? !(sm_z[taken] > 0.0) && !(s.greedy && top > -INFINITY)
-                                       : top == -INFINITY);
-  const int64_t own = none ? -1 : s.greedy ? sm_at[taken] : -1;
-  for (int j = tid; j < p.max_tokens; j += kVerThreads) {
-    const int64_t t = j < taken ? draft_token(p, s.row0 + j + 1) : j == taken ? own : -1;
-    const int64_t to = static_cast<int64_t>(b) * p.max_tokens + j;
-    if (p.tokens_wide)
-      reinterpret_cast<int64_t*>(p.out)[to] = t;
-    else
-      reinterpret_cast<int32_t*>(p.out)[to] = static_cast<int32_t>(t);
-  }
-  if (tid == 0) {
-    p.num_out[b] = s.n == 0 ? 0 : taken + !none;
-    VerifyRow& o = p.rows[b];
-    o.row = none || s.greedy ? -1 : s.row0 + taken;
-    o.taken = taken;
-    o.refused = taken + 1 < s.n;
-    o.top = top;
-    o.inverse = s.inverse;
-    const int64_t d = taken + 1 < s.n ? draft_token(p, s.row0 + taken + 1) : -1;
-    o.draft = d >= 0 && d < p.vocab ? static_cast<int32_t>(d) : -1;
+  const bool none = s.n == 0 || (PROBS && !s.greedy ? !(sm_z[taken] > 0.0) : top == -INFINITY);
+  const int64_t own = none || !s.greedy ? -1 : sm_at[taken];
+  if (wave == 0) {  // (lane i holds the draft that would be token i)
+    if (lane < p.max_tokens) {
+      const int64_t t = lane < taken ? d : lane == taken ? own : -1;
+      const int64_t to = static_cast<int64_t>(b) * p.max_tokens + lane;
+      if (p.tokens_wide)
+        reinterpret_cast<int64_t*>(p.out)[to] = t;
+      else
+        reinterpret_cast<int32_t*>(p.out)[to] = static_cast<int32_t>(t);
+    }
+    if (lane == taken) {
+      VerifyRow o;
+      o.row = none || s.greedy ? -1 : s.row0 + taken;
+      o.taken = taken;
+      o.refused = mine;
+      o.top = top;
+      o.rate = s.rate;
+      o.draft = token ? static_cast<int32_t>(d) : -1;
+      p.rows[b] = o;
+      p.num_out[b] = s.n == 0 ? 0 : taken + !none;
+    }
   }
 }
 
-// Entries 8 g .. of what a sequence is drawn from: with WEIGHTS the weights, else the
-// residual r (w where nothing was refused).
+// This thread's 8 entries of a slice of what a sequence is drawn from: with WEIGHTS the
+// weights, else the residual r (w where nothing was refused).
 template <typename T, bool PROBS, bool WEIGHTS>
-__device__ __forceinline__ void drawn8(const VerifyParams& p, const VerifyRow& o, int b, int g,
+__device__ __forceinline__ void drawn8(const VerifyParams& p, const VerifyRow& o, int b, int slice,
                                        double z, double (&r)[8]) {
-  float x[8];
-  load8<T>(target_row(p, o.row), g, p.vocab, PROBS ? 0.f : -INFINITY, x);
+  const int g = slice * kVerThreads + threadIdx.x, end = (slice + 1) * kVerSumSlice;
+  const bool less = !WEIGHTS && o.refused, have = less && p.draft_probs != nullptr;
+  float x[1][8], q[1][8];
+  load8s<T, 1>(target_row(p, o.row), g, end, p.vocab, PROBS ? 0.f : -INFINITY, x);
+  if (have)
+    load8s<float, 1>(p.draft_probs + b * p.q_stride_seq + o.taken * p.q_stride_row, g, end, p.vocab,
+                     0.f, q);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) r[k] = weight<PROBS>(x[k], o.top, o.inverse);
-  if (WEIGHTS || !o.refused) return;
-  if (p.draft_probs != nullptr) {
-    float q[8];
-    load8<float>(p.draft_probs + b * p.q_stride_seq + o.taken * p.q_stride_row, g, p.vocab, 0.f, q);
+  for (int k = 0; k < 8; ++k) r[k] = weight<PROBS>(x[0][k], o.top, o.rate);
+  if (have) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const double y = r[k] - static_cast<double>(q[k]) * z;
+      const double y = r[k] - static_cast<double>(q[0][k]) * z;
       r[k] = y > 0.0 ? y : 0.0;
     }
-  } else {
+  } else if (less) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (8 * g + k == o.draft) r[k] = 0.0;
@@ -322,7 +472,8 @@ __device__ __forceinline__ double slices_sum(const double* part, int n, double* 
 }
 
 // RESIDUAL false: Z of the drawn row, or without draft probabilities the sum of r;
-// true: the sum of r, of a sequence that refused.
+// true: the sum of r, of a sequence that refused.  (One slice to a workgroup: with two or
+// four, 64 x 152064 took as long or longer.)
 template <typename T, bool PROBS, bool RESIDUAL>
 __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(VerifyParams p) {
   __shared__ double sm_s[kVerWaves];
@@ -332,11 +483,10 @@ __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(VerifyParams p
   const double z =
       RESIDUAL ? slices_sum(p.sums + static_cast<int64_t>(b) * p.sum_slices, p.sum_slices, sm_s) : 0.0;
   double r[8], x = 0.0;
-  const int g = slice * kVerThreads + threadIdx.x;
   if (RESIDUAL || p.draft_probs == nullptr)
-    drawn8<T, PROBS, false>(p, o, b, g, z, r);
+    drawn8<T, PROBS, false>(p, o, b, slice, z, r);
   else
-    drawn8<T, PROBS, true>(p, o, b, g, z, r);
+    drawn8<T, PROBS, true>(p, o, b, slice, z, r);
 #pragma unroll
   for (int k = 0; k < 8; ++k) x += r[k];
   x = block_sum(x, sm_s);
@@ -347,11 +497,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(VerifyParams p
 // Prefix sums (inclusive) over the workgroup's threads.
 __device__ __forceinline__ double block_prefix(double x, double* sm) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
-    const double y = __shfl_up(x, w);
-    if (lane >= w) x += y;
-  }
+  x = wave_prefix64(x);
   __syncthreads();
   if (lane == 63) sm[wave] = x;
   __syncthreads();
@@ -364,42 +510,30 @@ __device__ __forceinline__ double block_prefix(double x, double* sm) {
 // The first thread whose running sum passes `want`; where rounding leaves none, the
 // last with a sum above 0 (-1: no such either).  own: the thread's sum, upto: with those
 // before it.
-__device__ __forceinline__ int first_past(double own, double upto, double want, int* sm) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sm[0] = kVerThreads;
-    sm[1] = -1;
+__device__ __forceinline__ int first_past(double own, double upto, double want, int (*sm)[2]) {
+  const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
+  const uint64_t past = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > want);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    sm[wave][0] = past ? 64 * wave + __builtin_ctzll(past) : -1;
+    sm[wave][1] = some ? 64 * wave + 63 - __builtin_clzll(some) : -1;
   }
   __syncthreads();
-  if (own > 0.0) {
-    if (upto > want) atomicMin(&sm[0], static_cast<int>(threadIdx.x));
-    atomicMax(&sm[1], static_cast<int>(threadIdx.x));
+  int first = -1, last = -1;
+#pragma unroll
+  for (int w = kVerWaves - 1; w >= 0; --w) {
+    first = sm[w][0] >= 0 ? sm[w][0] : first;
+    last = last < 0 ? sm[w][1] : last;
   }
-  __syncthreads();
-  return sm[0] < kVerThreads ? sm[0] : sm[1];
-}
-// The same of n values, one after the other; `before` becomes the sum before it.
-template <typename F>
-__device__ __forceinline__ int first_past_of(int n, double want, double& before, F value) {
-  int at = -1;
-  double run = before;
-  for (int i = 0; i < n; ++i) {
-    const double x = value(i);
-    if (x > 0.0) {
-      at = i;
-      before = run;
-      if (run + x > want) break;
-    }
-    run += x;
-  }
-  return at;
+  return first >= 0 ? first : last;
 }
 
 template <typename T, bool PROBS>
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p) {
   __shared__ double sm_s[kVerWaves], sm_c[kVerThreads + 1];
-  __shared__ int sm_f[2], sm_slice;
+  __shared__ int sm_f[kVerWaves][2], sm_g[kVerWaves][2];
   const int b = blockIdx.x, tid = threadIdx.x, n = p.sum_slices;
+  const double u = global_ptr(p.uniform)[b * p.uniform_stride + p.max_tokens - 1];
   const VerifyRow o = p.rows[b];
   if (o.row < 0) return;
   const int64_t to = static_cast<int64_t>(b) * p.max_tokens + o.taken;
@@ -410,71 +544,90 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p
       reinterpret_cast<int32_t*>(p.out)[to] = token;
   };
   const double* const sums = p.sums + static_cast<int64_t>(b) * n;
-  const double* part = sums;
+  const bool residual = o.refused && p.draft_probs != nullptr;
+  const double* part = residual ? p.residuals + static_cast<int64_t>(b) * n : sums;
   bool weights = !o.refused;
-  double z = 0.0;
-  if (o.refused && p.draft_probs != nullptr) {
-    z = slices_sum(sums, n, sm_s);
-    part = p.residuals + static_cast<int64_t>(b) * n;
-  }
-  double total = slices_sum(part, n, sm_s);
+  // every thread adds up some slices in a row
+  const int per = (n + kVerThreads - 1) / kVerThreads, i0 = tid * per;
+  auto owns = [&](const double* of) __attribute__((always_inline)) {
+    double x = 0.0;
+    for (int i = i0; i < i0 + per && i < n; ++i) x += global_ptr(of)[i];
+    return x;
+  };
+  double own = owns(part);
+  const double z = residual ? slices_sum(sums, n, sm_s) : 0.0;
+  double upto = block_prefix(own, sm_s);
+  sm_c[tid + 1] = upto;
+  if (tid == 0) sm_c[0] = 0.0;
+  __syncthreads();
+  double total = sm_c[kVerThreads];
   if (o.refused && !(total > 0.0)) {  // w is nowhere above q Z: drawn from w
-    if (p.draft_probs == nullptr) {   // (which is the draft alone)
+    if (!residual) {                  // (which is the draft alone)
       if (tid == 0) put(o.draft);
       return;
     }
     weights = true;
     part = sums;
-    total = z;
+    own = owns(part);
+    upto = block_prefix(own, sm_s);
+    __syncthreads();
+    sm_c[tid + 1] = upto;
+    __syncthreads();
+    total = sm_c[kVerThreads];
   }
-  const double want =
-      static_cast<double>(global_ptr(p.uniform)[b * p.uniform_stride + p.max_tokens - 1]) * total;
-  // the slice: every thread adds up some in a row
-  const int per = (n + kVerThreads - 1) / kVerThreads, i0 = tid * per;
-  double own = 0.0;
-  for (int i = i0; i < i0 + per && i < n; ++i) own += global_ptr(part)[i];
-  double upto = block_prefix(own, sm_s);
-  if (tid == 0) sm_c[0] = 0.0;
-  sm_c[tid + 1] = upto;
+  const double want = u * total;
   int who = first_past(own, upto, want, sm_f);
   if (who < 0) return;  // (no thread has a sum: not where `total` is above 0)
-  if (tid == who) {
-    double before = sm_c[who];
-    sm_slice = i0 + first_past_of(n - i0 < per ? n - i0 : per, want, before,
-                                  [&](int i) { return global_ptr(part)[i0 + i]; });
-    sm_c[kVerThreads] = before;
+  int slice = who;
+  double before = sm_c[who];
+  if (per > 1) {  // which of its slices
+    double run = before;
+    for (int i = who * per; i < (who + 1) * per && i < n; ++i) {
+      const double x = global_ptr(part)[i];
+      if (x > 0.0) {
+        slice = i;
+        before = run;
+        if (run + x > want) break;
+      }
+      run += x;
+    }
   }
-  __syncthreads();
-  const int slice = sm_slice;
-  double before = sm_c[kVerThreads];
   // the token in it
   double r[8];
-  const int g = slice * kVerThreads + tid;
   if (weights)
-    drawn8<T, PROBS, true>(p, o, b, g, z, r);
+    drawn8<T, PROBS, true>(p, o, b, slice, z, r);
   else
-    drawn8<T, PROBS, false>(p, o, b, g, z, r);
+    drawn8<T, PROBS, false>(p, o, b, slice, z, r);
   own = 0.0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) own += r[k];
   upto = before + block_prefix(own, sm_s);
-  sm_c[tid] = upto;
-  who = first_past(own, upto, want, sm_f);
+  __syncthreads();
+  sm_c[tid + 1] = upto;
+  if (tid == 0) sm_c[0] = before;
+  who = first_past(own, upto, want, sm_g);
   if (tid == who) {
-    before = tid > 0 ? sm_c[tid - 1] : before;
-    const int k = first_past_of(8, want, before, [&](int i) { return r[i]; });
-    put(8 * g + k);
+    double run = sm_c[who];
+    int at = 0;
+    bool past = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {  // the first past `want`, else the last with a weight
+      if (!past && r[k] > 0.0) at = k;
+      run += r[k];
+      past |= r[k] > 0.0 && run > want;
+    }
+    put(kVerSumSlice * slice + 8 * tid + at);
   }
 }
 
 template <typename T, bool PROBS>
 static hipError_t launch_verify_t(const VerifyParams& p, hipStream_t st) {
   const dim3 t(kVerThreads), seqs(static_cast<unsigned>(p.num_seqs));
-  const dim3 slices(static_cast<unsigned>(p.num_seqs * p.sum_slices));
   hipLaunchKernelGGL((verify_stats_kernel<T, PROBS>),
                      dim3(static_cast<unsigned>(p.num_seqs * p.max_tokens * p.stat_slices)), t, 0,
                      st, p);
   hipLaunchKernelGGL((verify_decide_kernel<T, PROBS>), seqs, t, 0, st, p);
+  const dim3 slices(static_cast<unsigned>(p.num_seqs * p.sum_slices));
   hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false>), slices, t, 0, st, p);
   if (p.draft_probs != nullptr)
     hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, true>), slices, t, 0, st, p);
