@@ -441,15 +441,6 @@ __device__ __forceinline__ void decode_split_body(const DecParams& p, int kvh_in
   }
 }
 
-// The kernel's one argument, by a pointer the compiler cannot see through:
-// its loads stay where they are used.
-template <typename P>
-__device__ __forceinline__ const P& fresh_params() {
-  auto k = __builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(k));
-  return *(const P*)k;
-}
-
 // Paged-ness is a property of each entry (a sequence's peer segment is
 // contiguous, its local segment paged), uniform within a workgroup.
 //

@@ -33,10 +33,11 @@ namespace hcp {
 constexpr int kDraftBufWord3 = 0x00020000;
 constexpr int kDraftStreamAux = 2;  // non-temporal: read once per launch
 
-// Keys of the tokens of one tile of 16: visible are [lo, hi).
+// Keys lo .. lo + n - 1.
 struct KeyRange {
-  int lo, hi;
-  __device__ __forceinline__ bool has(int key) const { return key >= lo && key < hi; }
+  int lo;
+  uint32_t n;
+  __device__ __forceinline__ bool has(int key) const { return static_cast<uint32_t>(key - lo) < n; }
 };
 
 // ---- K and V of a chunk of a 16-bit cache ----
@@ -52,7 +53,7 @@ struct Keys16 {
   static constexpr int CHB = 32 * ROWB;
   static constexpr int BYTES = 2 * CHB, LOADS = 4 * OPT;
   static constexpr int W = D == 256 ? 2 : 4;
-  static constexpr int START = 8, LEAST = 2, LATE = 1;  // paged_shares
+  static constexpr int START = 8, LEAST = 2, LATE = 1;  // paged_shares; START of a tile
 
   const char *k, *v;
   const int32_t* bt;
@@ -173,6 +174,7 @@ struct Keys16 {
   __device__ __forceinline__ bool clean_v(HCP_LDS_PTR(char) src, int x0, KeyRange any) const {
     constexpr uint32_t kExp = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
     bool odd = false;
+#pragma unroll 1
     for (int at = 16 * lane; at < CHB; at += 1024) {
       u32x4 x = lds_at<u32x4>(src + CHB + at);
       bool bad = false;
@@ -309,7 +311,7 @@ struct Keys4 {
       id = id < id_max ? id : id_max;
       const int at = (x0 + 16 * t) & (bs - 1);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<char*>(head + id * stride_block), 0, region, kDraftBufWord3);
+          const_cast<char*>(head + id * stride_block), 0, x0 < all ? region : 0, kDraftBufWord3);
       auto load = [&](int to, int o, int so) __attribute__((always_inline)) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rs, reinterpret_cast<HCP_LDS_PTR(void)>(dst + t * Tile::BYTES + to), 16, o, so, 0,
@@ -355,7 +357,7 @@ struct Keys4 {
       const HCP_LDS_PTR(char) const at = src + t * Tile::BYTES + Tile::SC + Tile::SW * 4 + 4 * i;
       const uint32_t w = lds_at<uint32_t>(at);
       uint32_t keep = w;
-#pragma unroll
+#pragma unroll 1
       for (int j = 0; j < 4; ++j) {
         const bool nan = (w >> (8 * j) & 255) == 255, in = any.has(key + j);
         if (nan || !in) keep &= ~(0xffu << (8 * j));
@@ -465,6 +467,7 @@ __device__ __forceinline__ void drafts_split_body(
   const bool some = x < ke;
   const int last = x + (ke - 1 - x) / ST * ST;
   auto upto = [&](int y) __attribute__((always_inline)) { return y < last ? y : last; };
+  auto next = [&]() __attribute__((always_inline)) { return x + ST <= last ? x + ST : all; };
 #if HCP_DRAFTS_FP4
   constexpr bool small = false;
 #else
@@ -502,13 +505,14 @@ __device__ __forceinline__ void drafts_split_body(
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     const int rho = rho0 + 16 * i + c16;
-    see[i].hi = rho < rows ? all - n + 1 + rho / G : 0;
-    see[i].lo = window > 0 ? see[i].hi - window : 0;
+    const int hi = rho < rows ? all - n + 1 + rho / G : 0;
+    see[i].lo = window > 0 && hi > window ? hi - window : 0;
+    see[i].n = hi > 0 ? hi - see[i].lo : 0;
   }
   // chunks that reach past `edge_hi`, or begin before `edge_lo`, hold keys that not
   // every token sees
   const int edge_hi = all - n + 1, edge_lo = window > 0 ? all - window : 0;
-  const KeyRange any{first, all};
+  const KeyRange any{first, static_cast<uint32_t>(all - first)};
   if (tid == 0) *sm_odd = 0;
   __syncthreads();
 
@@ -558,13 +562,19 @@ __device__ __forceinline__ void drafts_split_body(
       });
     }
     if (edge) {
+      // (opaque: the comparisons are made here, not ahead of the branch for every chunk)
+      int at = x0 + 4 * g4;
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (!see[i].has(x0 + 16 * t + 4 * g4 + j)) s[i][t][j] = -INFINITY;
+            if (!see[i].has(at + 16 * t + j)) s[i][t][j] = -INFINITY;
+          // (a few masks at a time: many would push the loop's scalars out of their registers)
+          __builtin_amdgcn_sched_barrier(0);
+        }
       if (keys.clean_v(src, x0, any)) *sm_odd = 1;
     }
     V8 pf[RT], rf[RT];
@@ -622,19 +632,23 @@ __device__ __forceinline__ void drafts_split_body(
 
   // The block ids of the chunk after the next are fetched, the next one's bytes
   // loaded, and when only those are outstanding the current one has landed.  (Loads
-  // without a branch around them: past the last chunk they repeat it.)
+  // without a branch around them, or the compiler's own waits for the ids would be for
+  // everything: past the last chunk they are out of their descriptor's range and fetch
+  // nothing.  Repeating the last chunk, as a single-token split does, cost 24 sequences of
+  // 0.5k-8k keys 2 us.)  With K's buffer filled again as soon as the scores are made, half
+  // a chunk more on its way, 64 x 16k-32k keys took no less (560 us for 550).
   if (some && !small) {
     while (true) {
       ia = keys.fetch_ids(upto(x + 2 * ST));
       __builtin_amdgcn_sched_barrier(0);
-      keys.issue(upto(x + ST), ib, bo);
+      keys.issue(next(), ib, bo);
       wait_vmcnt<K::LOADS + 1>();
       compute(x, be);
       x += ST;
       if (x > last) break;
       ib = keys.fetch_ids(upto(x + 2 * ST));
       __builtin_amdgcn_sched_barrier(0);
-      keys.issue(upto(x + ST), ia, be);
+      keys.issue(next(), ia, be);
       wait_vmcnt<K::LOADS + 1>();
       compute(x, bo);
       x += ST;
@@ -650,6 +664,7 @@ __device__ __forceinline__ void drafts_split_body(
 
   // ---- combine the W waves, a tile at a time in the chunk buffers ----
   wait_vmcnt<0>();  // the last loads still write there
+  const DraftParams& po = fresh_params<DraftParams>();  // (not held across the loop)
   // (all of them in bufO where there is room)
   constexpr int HW = sizeof(float) * W * 16 * (D + 4) <= W * K::BYTES ? 0 : W / 2;
   static_assert(sizeof(float) * (W - HW) * 16 * (D + 4) <= W * K::BYTES, "combine staging");
@@ -699,11 +714,11 @@ __device__ __forceinline__ void drafts_split_body(
             for (int j = 0; j < 4; ++j) O[j] += keys.odd_value(key, d + j);
         }
       }
-      const int64_t at = (static_cast<int64_t>(slot) * p.max_tokens + t) * p.p.d.num_heads + hq;
+      const int64_t at = (static_cast<int64_t>(slot) * po.max_tokens + t) * po.p.d.num_heads + hq;
       const bool some = L != 0.f;  // a NaN too: it is the row's result
       const float inv = some ? 1.f / L : 0.f;
-      *global_ptr(reinterpret_cast<f32x4*>(p.p.d.ws_o + at * D + d)) = some ? O * inv : f32x4{};
-      if (d == 0) global_ptr(p.p.d.ws_lse)[at] = some ? M * kLn2 + __logf(L) : -INFINITY;
+      *global_ptr(reinterpret_cast<f32x4*>(po.p.d.ws_o + at * D + d)) = some ? O * inv : f32x4{};
+      if (d == 0) global_ptr(po.p.d.ws_lse)[at] = some ? M * kLn2 + __logf(L) : -INFINITY;
     }
   }
 }
@@ -746,7 +761,7 @@ decode_drafts_kernel(DraftParams p) {
   int64_t starts[EPT + 1];
   paged_lens(p.row_starts, p.p.lens_wide, threadIdx.x * EPT, p.p.num_seqs + 1, starts);
   auto first_chunk = [](int all, int len) { return (all - len) & ~31; };
-  paged_shares<NT, K::START, K::LEAST, K::LATE, false>(
+  paged_shares<NT, K::START * RT, K::LEAST, K::LATE, false>(
       p.p, wg, sm_len, sm_all, sm_w, sm_cut,
       [&](int all, int len) { return len > 0 ? (all - first_chunk(all, len) + 31) >> 5 : 0; },
       [&](const PagedDecParams&, int j, int seen) {
@@ -761,6 +776,7 @@ decode_drafts_kernel(DraftParams p) {
   const int r1 = r0 < 0 ? -2 : __builtin_amdgcn_readfirstlane(sm_cut[2]);  // -1, -2: no share
   const int o1 = __builtin_amdgcn_readfirstlane(sm_cut[3]);
   for (int r = r0; r <= r1; ++r) {
+    const DraftParams& p = fresh_params<DraftParams>();
     const int len = __builtin_amdgcn_readfirstlane(sm_len[r]);
     if (len <= 0) continue;
     const int all = __builtin_amdgcn_readfirstlane(sm_all[r]);
@@ -835,25 +851,21 @@ hipError_t launch_drafts16(const DraftParams& p, int tiles, int dtype, hipStream
   return launch_drafts_d<Keys16>(p, tiles, dtype, st);
 }
 
-// The largest of the wave's lanes, a NaN left out.
-__device__ __forceinline__ float wave_max32(float x) {
-#pragma unroll
-  for (int i = 32; i > 0; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-  return x;
-}
-
-// Merge of a row's partials, a wave to each (sequence, token, head): out = sum_i w_i
-// O_i / sum_i w_i, w_i = exp(lse_i - max).  Lane i holds weight i, and every lane D /
-// 64 columns.  Bound by latency: the row's place and slots are fetched at once, then the
-// LSEs with the first 16 partials' columns, before any weight is known.
-template <int D, typename T>
+// Merge of a row's partials, a wave to HW heads of a (sequence, token): out = sum_i w_i
+// O_i / sum_i w_i, w_i = exp(lse_i - max).  Lane B h + i holds weight i of head h, and
+// every lane D / 64 columns of each head.  Bound by latency: the row's place and slots are
+// fetched at once, then the LSEs with the first partials' columns, before any weight is
+// known.  Four heads to a wave where there are more rows than the machine holds waves at
+// once (48 x 4 rows of 64 heads 6.5 us, 12 with one), one where there are few with many
+// partials (9 x 8 rows of 14 heads 4.3 us, 6.7 with four).
+template <int D, typename T, int HW>
 __global__ __launch_bounds__(256) void drafts_reduce_kernel(DraftParams p, DraftOut o) {
-  constexpr int N = D / 64, U = 16;
+  constexpr int N = D / 64, B = 64 / HW, U = 16 / HW;  // partials of a batch, fetched at once
   typedef float vf __attribute__((ext_vector_type(N == 1 ? 2 : N)));  // (of one: its first)
-  const int lane = threadIdx.x & 63;
-  const int heads = p.p.d.num_heads;
+  const int lane = threadIdx.x & 63, sub = lane / B, mine = lane % B;
+  const int heads = p.p.d.num_heads, hgs = (heads + HW - 1) / HW;
   const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int st = unit / heads, head = unit - st * heads;
+  const int st = unit / hgs, head = (unit - st * hgs) * HW;
   const int seq = st / p.max_tokens, t = st - seq * p.max_tokens;
   if (seq >= p.p.num_seqs) return;
   const int64_t from = draft_start(p, seq), to = draft_start(p, seq + 1);
@@ -869,75 +881,105 @@ __global__ __launch_bounds__(256) void drafts_reduce_kernel(DraftParams p, Draft
   const int64_t at = (static_cast<int64_t>(p0) * p.max_tokens + t) * heads + head;
   const float* lcol = p.p.d.ws_lse + at;
   const float* ocol = p.p.d.ws_o + at * D + N * lane;
-  auto column = [&](int64_t i) __attribute__((always_inline)) {
+  const int have = heads - head < HW ? heads - head : HW;
+  auto column = [&](int64_t i, int h) __attribute__((always_inline)) {
+    const float* c = ocol + (i * step + (h < have ? h : 0)) * D;
     vf x;
     if constexpr (N == 1)
-      x = vf{*global_ptr(ocol + i * step * D), 0.f};
+      x = vf{*global_ptr(c), 0.f};
     else
-      x = *global_ptr(reinterpret_cast<const vf*>(ocol + i * step * D));
+      x = *global_ptr(reinterpret_cast<const vf*>(c));
     return x;
   };
-  float m = -INFINITY, S = 0.f;
-  vf O{};
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int some = n - i0 < 64 ? n - i0 : 64;
-    const float l = lane < some ? global_ptr(lcol)[(i0 + lane) * step] : -INFINITY;
-    vf v[U];
+  auto lane_of = [&](float x, int l) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
+  };
+  float m = -INFINITY, S = 0.f;  // of this lane's head
+  vf O[HW] = {};
+  for (int i0 = 0; i0 < n; i0 += B) {
+    const int some = n - i0 < B ? n - i0 : B;
+    const float l =
+        mine < some && sub < have ? global_ptr(lcol)[(i0 + mine) * step + sub] : -INFINITY;
+    vf v[U][HW];
     auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) v[k] = column(i0 + (i + k < some ? i + k : some - 1));
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int h = 0; h < HW; ++h) v[k][h] = column(i0 + (i + k < some ? i + k : some - 1), h);
     };
     fetch(0);
     // (the maximum leaves a NaN out: its weight is NaN whatever that is)
-    const float mn = fmaxf(m, wave_max32(l));
+    float mn = l;
+#pragma unroll
+    for (int x = B / 2; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor(mn, x));
+    mn = fmaxf(m, mn);
     const float ref = mn == -INFINITY ? 0.f : mn;
     // (what came before, where a NaN may stand with m still -inf, is kept)
     const float sc = m == -INFINITY ? 1.f : __expf(m - ref);
     const float w = __expf(l - ref);
-    S *= sc;
-    O *= sc;
-    m = mn;
     float ws = w;
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) ws += __shfl_xor(ws, x);
-    S += ws;
+    for (int x = B / 2; x > 0; x >>= 1) ws += __shfl_xor(ws, x);
+    S = S * sc + ws;
+    m = mn;
+#pragma unroll
+    for (int h = 0; h < HW; ++h) O[h] *= lane_of(sc, B * h);
     for (int i = 0; i < some; i += U) {
       if (i > 0) fetch(i);
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (i + k) & 63));
-        // (past the last: not summed, whatever its columns hold)
-        O = i + k < some ? O + v[k] * wk : O;
-      }
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int h = 0; h < HW; ++h) {
+          const float wk = lane_of(w, (B * h + i + k) & 63);
+          // (past the last: not summed, whatever its columns hold)
+          O[h] = i + k < some ? O[h] + v[k][h] * wk : O[h];
+        }
     }
   }
   const int64_t row = static_cast<int64_t>(row0) + t;
-  const bool any = S != 0.f;
-  uint16_t* orow = reinterpret_cast<uint16_t*>(o.out) + row * o.stride_tok + head * o.stride_head;
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (N * lane + j < p.p.d.head_dim)
-      orow[N * lane + j] = Elem<T>::from_float(any ? O[j] / S : 0.f);
-  if (o.lse != nullptr && lane == 0)
-    o.lse[head * o.lse_stride_head + row] = any ? m + __logf(S) : -INFINITY;
+  for (int h = 0; h < HW; ++h) {
+    if (h >= have) break;
+    const float sum = lane_of(S, B * h);
+    uint16_t* orow =
+        reinterpret_cast<uint16_t*>(o.out) + row * o.stride_tok + (head + h) * o.stride_head;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (N * lane + j < p.p.d.head_dim)
+        orow[N * lane + j] = Elem<T>::from_float(sum != 0.f ? O[h][j] / sum : 0.f);
+  }
+  if (o.lse != nullptr && mine == 0 && sub < have)
+    o.lse[(head + sub) * o.lse_stride_head + row] = S != 0.f ? m + __logf(S) : -INFINITY;
+}
+
+template <int D, typename T>
+static void launch_drafts_reduce_t(const DraftParams& p, const DraftOut& o, hipStream_t st) {
+  const int64_t rows = static_cast<int64_t>(p.p.num_seqs) * p.max_tokens, heads = p.p.d.num_heads;
+  const bool many = rows * heads > 4096;
+  const int64_t units = rows * (many ? (heads + 3) / 4 : heads);
+  const dim3 g(static_cast<unsigned>((units + 3) / 4)), b(256);
+  if (many)
+    hipLaunchKernelGGL((drafts_reduce_kernel<D, T, 4>), g, b, 0, st, p, o);
+  else
+    hipLaunchKernelGGL((drafts_reduce_kernel<D, T, 1>), g, b, 0, st, p, o);
 }
 
 hipError_t launch_drafts_reduce(const DraftParams& p, const DraftOut& o, int dtype, hipStream_t st) {
-  // (under 2^31: sequences, tokens and heads are bounded)
-  const int64_t units = static_cast<int64_t>(p.p.num_seqs) * p.max_tokens * p.p.d.num_heads;
-  const dim3 g(static_cast<unsigned>((units + 3) / 4)), b(256);
   const bool bf = dtype == HCP_DTYPE_BF16;
-#define HCP_REDUCE(D)                                                                 \
-  if (bf)                                                                             \
-    hipLaunchKernelGGL((drafts_reduce_kernel<D, __bf16>), g, b, 0, st, p, o);         \
-  else                                                                                \
-    hipLaunchKernelGGL((drafts_reduce_kernel<D, _Float16>), g, b, 0, st, p, o)
   switch (padded_head_dim(p.p.d.head_dim)) {
-    case 256: HCP_REDUCE(256); break;
-    case 128: HCP_REDUCE(128); break;
-    default: HCP_REDUCE(64); break;
+    case 256:
+      bf ? launch_drafts_reduce_t<256, __bf16>(p, o, st)
+         : launch_drafts_reduce_t<256, _Float16>(p, o, st);
+      break;
+    case 128:
+      bf ? launch_drafts_reduce_t<128, __bf16>(p, o, st)
+         : launch_drafts_reduce_t<128, _Float16>(p, o, st);
+      break;
+    default:
+      bf ? launch_drafts_reduce_t<64, __bf16>(p, o, st)
+         : launch_drafts_reduce_t<64, _Float16>(p, o, st);
+      break;
   }
-#undef HCP_REDUCE
   return hipGetLastError();
 }
 #endif

@@ -6,6 +6,15 @@
 
 namespace hcp {
 
+// The kernel's one argument, by a pointer the compiler cannot see through:
+// its loads stay where they are used.
+template <typename P>
+__device__ __forceinline__ const P& fresh_params() {
+  auto k = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(k));
+  return *(const P*)k;
+}
+
 // Inclusive prefix sum over the wave's lanes, by DPP moves (inside rows of 16
 // lanes, then row 0 -> 1 and 2 -> 3, then the lower half into the upper):
 // an add each, where six shuffles through LDS take about 100 cycles each.
