@@ -28,6 +28,7 @@ namespace hcp {
 
 constexpr int kVerThreads = 256;
 constexpr int kVerWaves = kVerThreads / 64;
+constexpr int kVerSmall = 65536;  // a vocabulary that one workgroup goes over
 constexpr int kStatSlice = kVerStatSlice;  // 32 values to a thread
 static_assert(kStatSlice == 32 * kVerThreads && kVerSumSlice == 8 * kVerThreads, "slices");
 
@@ -309,7 +310,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyParams 
   }
 }
 
-// Sum over the workgroup of every thread's x, in a fixed order.
+// Sum over a workgroup of W waves of every thread's x, in a fixed order.
+template <int W = kVerWaves>
 __device__ __forceinline__ double block_sum(double x, double* sm) {
   x = wave_sum(x);
   __syncthreads();
@@ -317,7 +319,7 @@ __device__ __forceinline__ double block_sum(double x, double* sm) {
   __syncthreads();
   double r = 0.0;
 #pragma unroll
-  for (int w = 0; w < kVerWaves; ++w) r += sm[w];
+  for (int w = 0; w < W; ++w) r += sm[w];
   return r;
 }
 
@@ -326,14 +328,22 @@ __device__ __forceinline__ double block_sum(double x, double* sm) {
 // 150000 tokens, 24 at most here); the additions in a thread by 32 steps of 2^-24.
 constexpr double kSumError = 1e-5;
 
-template <typename T, bool PROBS>
-__global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams p) {
-  __shared__ float sm_top[kVerMaxTokens];
-  __shared__ int sm_at[kVerMaxTokens];
-  __shared__ double sm_z[kVerMaxTokens], sm_uq[kVerMaxTokens], sm_w[kVerMaxTokens];
-  __shared__ double sm_s[kVerWaves];
-  __shared__ uint64_t sm_ok, sm_near;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+template <int W>
+struct DecideShared {
+  float top[kVerMaxTokens];
+  int at[kVerMaxTokens];
+  double z[kVerMaxTokens], uq[kVerMaxTokens], w[kVerMaxTokens];
+  double sums[W];
+  uint64_t ok, near;
+  VerifyRow row;
+};
+
+// Which drafts of sequence b are accepted, by a workgroup of W waves: gives what the one
+// token more is drawn from, and with `write` writes the tokens and their number.
+template <typename T, bool PROBS, int W>
+__device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, DecideShared<W>& sm,
+                                            bool write = true) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VerifySeq s = verify_seq(p, b);
   // lane i of every wave looks at draft i: fetched while the slices' sums are
   const bool mine = lane + 1 < s.n;
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams
           global_ptr(p.draft_probs)[b * p.q_stride_seq + lane * p.q_stride_row + d]);
   }
   // the rows' maxima and sums from those of their slices
-  for (int j = wave; j < s.n; j += kVerWaves) {
+  for (int j = wave; j < s.n; j += W) {
     const VerifyStat* const st =
         p.stats + (static_cast<int64_t>(b) * p.max_tokens + j) * p.stat_slices;
     VerifyStat own{-INFINITY, 0x7fffffff, 0.0};  // of this lane's first slice
@@ -368,9 +378,9 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams
     for (int i = lane + 64; i < p.stat_slices; i += 64) z += part(global_ptr(st)[i]);
     z = wave_sum(z);
     if (lane == 0) {
-      sm_top[j] = m;
-      sm_at[j] = at;
-      sm_z[j] = z;
+      sm.top[j] = m;
+      sm.at[j] = at;
+      sm.z[j] = z;
     }
   }
   __syncthreads();
@@ -378,44 +388,44 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams
     bool ok = false, near = false;
     if (token) {
       if (s.greedy) {
-        ok = sm_at[lane] == d;
+        ok = sm.at[lane] == d;
       } else {
-        const double w = weight<PROBS>(xd, sm_top[lane], s.rate), v = uq * sm_z[lane];
+        const double w = weight<PROBS>(xd, sm.top[lane], s.rate), v = uq * sm.z[lane];
         ok = v < w;
         near = fabs(v - w) <= kSumError * w;
-        sm_uq[lane] = uq;
-        sm_w[lane] = w;
+        sm.uq[lane] = uq;
+        sm.w[lane] = w;
       }
     }
     const uint64_t oks = __builtin_amdgcn_ballot_w64(ok), nears = __builtin_amdgcn_ballot_w64(near);
     if (lane == 0) {
-      sm_ok = oks;
-      sm_near = nears;
+      sm.ok = oks;
+      sm.near = nears;
     }
   }
   __syncthreads();
   int taken = 0;
   for (; taken + 1 < s.n; ++taken) {  // (the same in every thread)
-    if (sm_near >> taken & 1) {  // too near to tell: the row in 64 bits
+    if (sm.near >> taken & 1) {  // too near to tell: the row in 64 bits
       const char* const row = target_row(p, s.row0 + taken);
       double x = 0.0;
-      for (int g = tid; g < (p.vocab + 7) / 8; g += kVerThreads) {
+      for (int g = tid; g < (p.vocab + 7) / 8; g += 64 * W) {
         float e[8];
         load8<T>(row, g, p.vocab, -INFINITY, e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x += weight<PROBS>(e[k], sm_top[taken], s.rate);
+        for (int k = 0; k < 8; ++k) x += weight<PROBS>(e[k], sm.top[taken], s.rate);
       }
-      if (!(sm_uq[taken] * block_sum(x, sm_s) < sm_w[taken])) break;
-    } else if (!(sm_ok >> taken & 1)) {
+      if (!(sm.uq[taken] * block_sum<W>(x, sm.sums) < sm.w[taken])) break;
+    } else if (!(sm.ok >> taken & 1)) {
       break;
     }
   }
   // tokens, and what the row that is drawn from is
-  const float top = s.n > 0 ? sm_top[taken] : -INFINITY;
-  const bool none = s.n == 0 || (PROBS && !s.greedy ? !(sm_z[taken] > 0.0) : top == -INFINITY);
-  const int64_t own = none || !s.greedy ? -1 : sm_at[taken];
+  const float top = s.n > 0 ? sm.top[taken] : -INFINITY;
+  const bool none = s.n == 0 || (PROBS && !s.greedy ? !(sm.z[taken] > 0.0) : top == -INFINITY);
+  const int64_t own = none || !s.greedy ? -1 : sm.at[taken];
   if (wave == 0) {  // (lane i holds the draft that would be token i)
-    if (lane < p.max_tokens) {
+    if (write && lane < p.max_tokens) {
       const int64_t t = lane < taken ? d : lane == taken ? own : -1;
       const int64_t to = static_cast<int64_t>(b) * p.max_tokens + lane;
       if (p.tokens_wide)
@@ -431,37 +441,53 @@ __global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams
       o.top = top;
       o.rate = s.rate;
       o.draft = token ? static_cast<int32_t>(d) : -1;
-      p.rows[b] = o;
-      p.num_out[b] = s.n == 0 ? 0 : taken + !none;
+      sm.row = o;
+      if (write) p.num_out[b] = s.n == 0 ? 0 : taken + !none;
     }
   }
+  __syncthreads();
+  return sm.row;
 }
 
-// This thread's 8 entries of a slice of what a sequence is drawn from: with WEIGHTS the
-// weights, else the residual r (w where nothing was refused).
-template <typename T, bool PROBS, bool WEIGHTS>
-__device__ __forceinline__ void drawn8(const VerifyParams& p, const VerifyRow& o, int b, int slice,
-                                       double z, double (&r)[8]) {
-  const int g = slice * kVerThreads + threadIdx.x, end = (slice + 1) * kVerSumSlice;
-  const bool less = !WEIGHTS && o.refused, have = less && p.draft_probs != nullptr;
-  float x[1][8], q[1][8];
-  load8s<T, 1>(target_row(p, o.row), g, end, p.vocab, PROBS ? 0.f : -INFINITY, x);
-  if (have)
-    load8s<float, 1>(p.draft_probs + b * p.q_stride_seq + o.taken * p.q_stride_row, g, end, p.vocab,
-                     0.f, q);
+template <typename T, bool PROBS>
+__global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams p) {
+  __shared__ DecideShared<kVerWaves> sm;
+  const VerifyRow o = decide<T, PROBS, kVerWaves>(p, blockIdx.x, sm);
+  if (threadIdx.x == 0) p.rows[blockIdx.x] = o;
+}
+
+// What 8 entries of a sequence's drawn row come to, x from the target and q from the draft
+// (where `have`), the first of them entry 8 g: with `weights` the weights, else the residual
+// r (w where nothing was refused).
+template <bool PROBS>
+__device__ __forceinline__ void drawn8(const VerifyRow& o, bool weights, bool have, int g, double z,
+                                       const float (&x)[8], const float (&q)[8], double (&r)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) r[k] = weight<PROBS>(x[0][k], o.top, o.rate);
+  for (int k = 0; k < 8; ++k) r[k] = weight<PROBS>(x[k], o.top, o.rate);
+  if (weights || !o.refused) return;
   if (have) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const double y = r[k] - static_cast<double>(q[0][k]) * z;
+      const double y = r[k] - static_cast<double>(q[k]) * z;
       r[k] = y > 0.0 ? y : 0.0;
     }
-  } else if (less) {
+  } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (8 * g + k == o.draft) r[k] = 0.0;
   }
+}
+// The same from memory; `end`: past the workgroup's last entry.
+template <typename T, bool PROBS>
+__device__ __forceinline__ void drawn8(const VerifyParams& p, const VerifyRow& o, int b,
+                                       bool weights, int g, int end, double z, double (&r)[8]) {
+  float x[1][8], q[1][8];
+  const bool have = p.draft_probs != nullptr && o.refused && !weights;
+  load8s<T, 1>(target_row(p, o.row), g, end, p.vocab, PROBS ? 0.f : -INFINITY, x);
+  if (have)
+    load8s<float, 1>(p.draft_probs + b * p.q_stride_seq + o.taken * p.q_stride_row, g, end, p.vocab,
+                     0.f, q);
+  drawn8<PROBS>(o, weights, have, g, z, x[0], q[0], r);
 }
 
 // Sum of the slices' sums, in a fixed order, in every thread.
@@ -474,19 +500,25 @@ __device__ __forceinline__ double slices_sum(const double* part, int n, double* 
 // RESIDUAL false: Z of the drawn row, or without draft probabilities the sum of r;
 // true: the sum of r, of a sequence that refused.  (One slice to a workgroup: with two or
 // four, 64 x 152064 took as long or longer.)
-template <typename T, bool PROBS, bool RESIDUAL>
+// DECIDE: with step 2 before it, in every workgroup.
+template <typename T, bool PROBS, bool RESIDUAL, bool DECIDE>
 __global__ __launch_bounds__(kVerThreads) void verify_sums_kernel(VerifyParams p) {
   __shared__ double sm_s[kVerWaves];
   const int slice = blockIdx.x % p.sum_slices, b = blockIdx.x / p.sum_slices;
-  const VerifyRow o = p.rows[b];
+  VerifyRow o;
+  if constexpr (DECIDE) {
+    __shared__ DecideShared<kVerWaves> sm;
+    o = decide<T, PROBS, kVerWaves>(p, b, sm, slice == 0);
+    if (slice == 0 && threadIdx.x == 0) p.rows[b] = o;
+  } else {
+    o = p.rows[b];
+  }
   if (o.row < 0 || (RESIDUAL && !o.refused)) return;
   const double z =
       RESIDUAL ? slices_sum(p.sums + static_cast<int64_t>(b) * p.sum_slices, p.sum_slices, sm_s) : 0.0;
   double r[8], x = 0.0;
-  if (RESIDUAL || p.draft_probs == nullptr)
-    drawn8<T, PROBS, false>(p, o, b, slice, z, r);
-  else
-    drawn8<T, PROBS, true>(p, o, b, slice, z, r);
+  const int g = slice * kVerThreads + threadIdx.x, end = (slice + 1) * kVerSumSlice;
+  drawn8<T, PROBS>(p, o, b, !RESIDUAL && p.draft_probs != nullptr, g, end, z, r);
 #pragma unroll
   for (int k = 0; k < 8; ++k) x += r[k];
   x = block_sum(x, sm_s);
@@ -528,6 +560,117 @@ __device__ __forceinline__ int first_past(double own, double upto, double want, 
   return first >= 0 ? first : last;
 }
 
+// The first of 8 entries at which the running sum passes `want`, else the last above 0.
+__device__ __forceinline__ int first_of8(const double (&r)[8], double run, double want) {
+  int at = 0;
+  bool past = false;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (!past && r[k] > 0.0) at = k;
+    run += r[k];
+    past |= r[k] > 0.0 && run > want;
+  }
+  return at;
+}
+__device__ __forceinline__ void put_token(const VerifyParams& p, const VerifyRow& o, int b, int token) {
+  const int64_t to = static_cast<int64_t>(b) * p.max_tokens + o.taken;
+  if (p.tokens_wide)
+    reinterpret_cast<int64_t*>(p.out)[to] = token;
+  else
+    reinterpret_cast<int32_t*>(p.out)[to] = token;
+}
+
+// Steps 2 to 5 in one workgroup of 16 waves to a sequence, for vocabularies up to
+// kVerSmall: 8192 entries at a time, the sums of every wave's 512 kept, of which the one
+// with the token is gone over again by its wave.
+template <typename T, bool PROBS>
+__global__ __launch_bounds__(1024) void verify_finish_kernel(VerifyParams p) {
+  constexpr int W = 16, kAt = 64 * W * 8, kIts = kVerSmall / kAt;
+  __shared__ DecideShared<W> sm;
+  __shared__ double sm_seg[kIts * W];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const double u = global_ptr(p.uniform)[b * p.uniform_stride + p.max_tokens - 1];
+  const VerifyRow o = decide<T, PROBS, W>(p, b, sm);
+  if (o.row < 0) return;
+  const int its = (p.vocab + kAt - 1) / kAt;
+  const bool residual = o.refused && p.draft_probs != nullptr;
+  auto added = [&](const double (&r)[8]) __attribute__((always_inline)) {
+    return ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+  };
+  // f(it, sum of this thread's entries) over the row
+  auto over = [&](bool weights, double z, auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int it = 0; it < its; ++it) {
+      double r[8];
+      drawn8<T, PROBS>(p, o, b, weights, it * 64 * W + tid, (it + 1) * kAt, z, r);
+      f(it, added(r));
+    }
+  };
+  double z = 0.0;
+  if (residual) {
+    over(true, 0.0, [&](int, double x) __attribute__((always_inline)) { z += x; });
+    z = block_sum<W>(z, sm.sums);
+  }
+  bool weights = !o.refused;
+  double total = 0.0;
+  for (int again = 0; again < 2; ++again) {
+    over(weights, z, [&](int it, double x) __attribute__((always_inline)) {
+      x = wave_sum(x);
+      if (lane == 0) sm_seg[it * W + wave] = x;
+    });
+    __syncthreads();
+    total = 0.0;
+    for (int i = lane; i < its * W; i += 64) total += sm_seg[i];
+    total = wave_sum(total);
+    if (total > 0.0 || !o.refused || again) break;
+    // nothing is left of w where q is not below it: drawn from w (and without draft
+    // probabilities there is the draft alone)
+    if (!residual) {
+      if (tid == 0) put_token(p, o, b, o.draft);
+      return;
+    }
+    weights = true;
+    __syncthreads();  // (every wave has read the sums)
+  }
+  // the wave's 512 entries in which the running sum passes `want`, in every wave alike;
+  // where rounding leaves none, the last with a sum
+  const double want = u * total;
+  int seg = -1, last = -1;
+  double before = 0.0, before_last = 0.0, run = 0.0;
+  for (int i0 = 0; i0 < its * W && seg < 0; i0 += 64) {
+    const double own = i0 + lane < its * W ? sm_seg[i0 + lane] : 0.0;
+    const double upto = run + wave_prefix64(own);
+    double ahead = __shfl_up(upto, 1);  // (by all lanes: one that is off gives nothing)
+    ahead = lane > 0 ? ahead : run;
+    const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > want);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      seg = i0 + l;
+      before = __shfl(ahead, l);
+    } else if (some) {
+      const int l = 63 - __builtin_clzll(some);
+      last = i0 + l;
+      before_last = __shfl(ahead, l);
+    }
+    run = last_lane(upto);
+  }
+  if (seg < 0) {
+    seg = last;
+    before = before_last;
+  }
+  if (seg < 0 || wave != seg % W) return;
+  double r[8];
+  drawn8<T, PROBS>(p, o, b, weights, seg / W * 64 * W + tid, (seg / W + 1) * kAt, z, r);
+  const double own = added(r), upto = before + wave_prefix64(own);
+  const double ahead = __shfl_up(upto, 1);
+  const uint64_t some = __builtin_amdgcn_ballot_w64(own > 0.0);
+  const uint64_t past = __builtin_amdgcn_ballot_w64(own > 0.0 && upto > want);
+  const int who = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  if (lane == who)
+    put_token(p, o, b, seg / W * kAt + 8 * tid + first_of8(r, lane > 0 ? ahead : before, want));
+}
+
 template <typename T, bool PROBS>
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p) {
   __shared__ double sm_s[kVerWaves], sm_c[kVerThreads + 1];
@@ -536,13 +679,6 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p
   const double u = global_ptr(p.uniform)[b * p.uniform_stride + p.max_tokens - 1];
   const VerifyRow o = p.rows[b];
   if (o.row < 0) return;
-  const int64_t to = static_cast<int64_t>(b) * p.max_tokens + o.taken;
-  auto put = [&](int token) __attribute__((always_inline)) {
-    if (p.tokens_wide)
-      reinterpret_cast<int64_t*>(p.out)[to] = token;
-    else
-      reinterpret_cast<int32_t*>(p.out)[to] = token;
-  };
   const double* const sums = p.sums + static_cast<int64_t>(b) * n;
   const bool residual = o.refused && p.draft_probs != nullptr;
   const double* part = residual ? p.residuals + static_cast<int64_t>(b) * n : sums;
@@ -563,7 +699,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p
   double total = sm_c[kVerThreads];
   if (o.refused && !(total > 0.0)) {  // w is nowhere above q Z: drawn from w
     if (!residual) {                  // (which is the draft alone)
-      if (tid == 0) put(o.draft);
+      if (tid == 0) put_token(p, o, b, o.draft);
       return;
     }
     weights = true;
@@ -594,10 +730,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p
   }
   // the token in it
   double r[8];
-  if (weights)
-    drawn8<T, PROBS, true>(p, o, b, slice, z, r);
-  else
-    drawn8<T, PROBS, false>(p, o, b, slice, z, r);
+  const int g = slice * kVerThreads + tid, end = (slice + 1) * kVerSumSlice;
+  drawn8<T, PROBS>(p, o, b, weights, g, end, z, r);
   own = 0.0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) own += r[k];
@@ -606,18 +740,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyParams p
   sm_c[tid + 1] = upto;
   if (tid == 0) sm_c[0] = before;
   who = first_past(own, upto, want, sm_g);
-  if (tid == who) {
-    double run = sm_c[who];
-    int at = 0;
-    bool past = false;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {  // the first past `want`, else the last with a weight
-      if (!past && r[k] > 0.0) at = k;
-      run += r[k];
-      past |= r[k] > 0.0 && run > want;
-    }
-    put(kVerSumSlice * slice + 8 * tid + at);
-  }
+  if (tid == who)
+    put_token(p, o, b, kVerSumSlice * slice + 8 * tid + first_of8(r, sm_c[who], want));
 }
 
 template <typename T, bool PROBS>
@@ -626,11 +750,23 @@ static hipError_t launch_verify_t(const VerifyParams& p, hipStream_t st) {
   hipLaunchKernelGGL((verify_stats_kernel<T, PROBS>),
                      dim3(static_cast<unsigned>(p.num_seqs * p.max_tokens * p.stat_slices)), t, 0,
                      st, p);
-  hipLaunchKernelGGL((verify_decide_kernel<T, PROBS>), seqs, t, 0, st, p);
-  const dim3 slices(static_cast<unsigned>(p.num_seqs * p.sum_slices));
-  hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false>), slices, t, 0, st, p);
+  // Many sequences over a vocabulary that one workgroup goes over soon enough: steps 2 to 5
+  // at once (200 x 50257 of probabilities 20 us for 27).  Few of them: step 2 in every
+  // workgroup of step 3, a launch less.
+  if (p.vocab <= kVerSmall && p.num_seqs >= 64) {
+    hipLaunchKernelGGL((verify_finish_kernel<T, PROBS>), seqs, dim3(1024), 0, st, p);
+    return hipGetLastError();
+  }
+  const int64_t n = static_cast<int64_t>(p.num_seqs) * p.sum_slices;
+  const dim3 slices(static_cast<unsigned>(n));
+  if (n <= 1024) {
+    hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false, true>), slices, t, 0, st, p);
+  } else {
+    hipLaunchKernelGGL((verify_decide_kernel<T, PROBS>), seqs, t, 0, st, p);
+    hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false, false>), slices, t, 0, st, p);
+  }
   if (p.draft_probs != nullptr)
-    hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, true>), slices, t, 0, st, p);
+    hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, true, false>), slices, t, 0, st, p);
   hipLaunchKernelGGL((verify_pick_kernel<T, PROBS>), seqs, t, 0, st, p);
   return hipGetLastError();
 }

@@ -39,13 +39,16 @@ def run(dev, c):
     return verify_drafts(**{k: x.to(dev) if isinstance(x, torch.Tensor) else x for k, x in c.items()})
 
 
-def compare(dev, c):
+def compare_(dev, c):
     want = verify(c["target"], c["tokens"], c["query_start_loc"], c["uniform"], c["draft_probs"],
                   c["temperature"], c["probs"])
     got = run(dev, c)
     assert got.tokens.dtype == c["tokens"].dtype and got.num_tokens.dtype == torch.int32
     check_verified(got, want, c["uniform"].shape[1])
     return want
+
+
+compare = compare_
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -65,6 +68,19 @@ def test_drafts(dev, q, probs, most):
     gen = torch.Generator().manual_seed(most)
     counts = [1 + (i * 7) % most for i in range(12)]
     compare(dev, case(gen, counts, 1000, torch.float32, most, q=q, probs=probs, greedy=0.2))
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("q", [True, False])
+@pytest.mark.parametrize("v", [1, 9, 513, 8192, 9000, 33000, 65536, 65537])
+def test_many_sequences(dev, v, q, probs):
+    """As many as get a workgroup each, and vocabularies on either side of what one takes."""
+    gen = torch.Generator().manual_seed(v)
+    counts = [1 + i % 3 for i in range(70)]
+    compare(dev, case(gen, counts, v, torch.float32, 3, q=q, probs=probs, greedy=0.2))
+    flat = case(gen, [1] * 70, v, torch.bfloat16, 1, q=False, spread=0.0)
+    flat["temperature"] = None
+    compare(dev, flat)
 
 
 def test_a_long_flat_row(dev):
@@ -158,11 +174,12 @@ def test_near_borders(dev):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("q", [True, False])
-def test_infinities_and_nan(dev, dtype, q):
+@pytest.mark.parametrize("more", [0, 60])
+def test_infinities_and_nan(dev, dtype, q, more):
     """Entries cut off by -inf or the type's lowest value, NaN, infinities; rows of
-    nothing else."""
+    nothing else.  With sequences of one row behind them, another kernel's share."""
     gen = torch.Generator().manual_seed(9)
-    c = case(gen, [3] * 9, 3000, dtype, 3, q=q)
+    c = case(gen, [3] * 9 + [1] * more, 3000, dtype, 3, q=q)
     x = c["target"]
     x[0:3, 100:] = -INF
     x[3:6, 7:] = torch.finfo(dtype).min
@@ -175,7 +192,7 @@ def test_infinities_and_nan(dev, dtype, q):
     x[18:21, :] = torch.finfo(dtype).min
     x[22] = -INF
     x[24:27, 40] = torch.finfo(dtype).max
-    for temperature in (None, torch.tensor([1.0, 0.0] * 4 + [0.25])):
+    for temperature in (None, torch.tensor([1.0, 0.0] * 4 + [0.25] + [1.0] * more)):
         for warm in (1.0, 1e-3, INF):
             t = None if temperature is None else temperature * warm
             t = t if t is None else torch.nan_to_num(t, nan=0.0, posinf=INF)
@@ -193,8 +210,17 @@ def test_drafts_that_are_no_tokens(dev):
         compare(dev, c)
 
 
-def test_nothing_left_of_the_residual(dev):
+@pytest.mark.parametrize("n", [1, 64])
+def test_nothing_left_of_the_residual(dev, n):
     """q nowhere below p: the token is drawn from p itself."""
+    def compare(dev, c):  # n sequences of the same
+        many = {k: x.repeat(n, *[1] * (x.dim() - 1)) if isinstance(x, torch.Tensor) else x
+                for k, x in c.items()}
+        many["query_start_loc"] = torch.arange(0, 2 * n + 1, 2)
+        want = compare_(dev, many)
+        assert all(w == want[0] for w in want)
+        return want[:1]
+
     p = torch.softmax(torch.arange(10.0), 0)
     for q, u in ((2 * p, 0.75), (torch.full((10,), INF), 0.5), (torch.full((10,), float("nan")), 0.5)):
         c = dict(target=p.expand(2, -1), tokens=torch.tensor([0, 9]), query_start_loc=torch.tensor([0, 2]),
