@@ -1870,7 +1870,9 @@ int hcp_decode_drafts(const hcp_decode_drafts_args* args, void* stream) {
   if (!drafts_sizes(a->num_seqs, args->max_tokens, a->num_heads, a->num_kv_heads, a->head_dim))
     return fail(HCP_EUNSUPPORTED, "%s: more than %d sequences, %d tokens of one, or %d heads", who,
                 HCP_DECODE_PAGED_MAX_SEQS, HCP_DRAFTS_MAX_TOKENS, 1 << 16);
-  if (args->q_rows > INT32_MAX) return fail(HCP_EUNSUPPORTED, "%s: too many rows", who);
+  if (args->q_rows > INT32_MAX ||
+      static_cast<int64_t>(a->num_seqs) * args->max_tokens * a->num_heads > INT32_MAX)
+    return fail(HCP_EUNSUPPORTED, "%s: too many rows", who);
   if (!a->q || !a->out || !a->seq_lens || !args->row_starts || !a->kv.block_table)
     return fail(HCP_EINVAL, "%s: null pointer", who);
   if (a->seq_starts) return fail(HCP_EUNSUPPORTED, "%s: seq_starts", who);

@@ -48,8 +48,8 @@ def decode_drafts(
     Lengths (int32 / int64 ``[S]``), row starts (``[S + 1]``, of their dtype) and block ids
     are read on the device when the call executes; a length past its table row counts as
     the row's keys, a block id past the cache as its last block.  A token that sees no
-    key gets out 0 and LSE -inf, one with a NaN score NaN; a key that it does not see
-    cannot reach it, whatever it holds.  Rows of ``out`` that belong to no sequence are
+    key (or none with a score above -inf) gets out 0 and LSE -inf, one with a NaN score NaN;
+    a key that it does not see cannot reach it, whatever it holds.  Rows of ``out`` that belong to no sequence are
     left as they were.  Returns out (and lse float32 ``[H, T]``), to be merged with other
     keys' by ``merge_attn_states``."""
     dt, index = q.dtype, q.get_device()

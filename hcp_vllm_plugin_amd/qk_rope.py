@@ -171,7 +171,17 @@ def qk_norm_rope(
     return query_out, key_out
 
 
-_SCALINGS = {"default": 0, "linear": 1, "llama3": 2, "yarn": 3, "dynamic": 0, "longrope": 4}
+_CONTEXT = "original_max_position_embeddings"
+# of each type: the library's kind, and the entries it goes by
+_SCALINGS = {
+    "default": (0, ()),
+    "linear": (1, ("factor",)),
+    "llama3": (2, ("factor", "low_freq_factor", "high_freq_factor", _CONTEXT)),
+    "yarn": (3, ("factor", _CONTEXT, "beta_fast", "beta_slow", "attention_factor", "mscale",
+                 "mscale_all_dim")),
+    "dynamic": (0, ("factor", _CONTEXT)),
+    "longrope": (4, ("short_factor", "long_factor", _CONTEXT, "factor", "attention_factor")),
+}
 
 
 def _scaling_fields(scaling: Mapping, rot: int, base: float, positions: int):
@@ -179,6 +189,10 @@ def _scaling_fields(scaling: Mapping, rot: int, base: float, positions: int):
     kind = scaling.get("rope_type", scaling.get("type"))
     if kind not in _SCALINGS:
         raise ValueError(f"rope_type {kind!r} is none of {', '.join(_SCALINGS)}")
+    code, known = _SCALINGS[kind]
+    other = set(scaling) - set(known) - {"rope_type", "type"}
+    if other:
+        raise ValueError(f"scaling {kind!r} does not go by {', '.join(sorted(other))}")
     number = {k: float(x) for k, x in scaling.items() if isinstance(x, (int, float))}
 
     def need(name):
@@ -187,14 +201,17 @@ def _scaling_fields(scaling: Mapping, rot: int, base: float, positions: int):
         return number[name]
 
     factor = need("factor") if kind in ("linear", "llama3", "yarn", "dynamic") else 1.0
-    trained = need("original_max_position_embeddings") if kind not in ("default", "linear") else 0.0
+    trained = need(_CONTEXT) if _CONTEXT in known else 0.0
     low = high = fast = slow = 0.0
     attention, divisors = 1.0, None
     if kind == "llama3":
         low, high = need("low_freq_factor"), need("high_freq_factor")
     elif kind == "yarn":
         fast, slow = number.get("beta_fast", 32.0), number.get("beta_slow", 1.0)
-        attention = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+        if factor > 1:
+            far, all_dim = number.get("mscale", 0.0), number.get("mscale_all_dim", 0.0)
+            attention = 0.1 * math.log(factor) + 1 if not (far and all_dim) else \
+                (0.1 * far * math.log(factor) + 1) / (0.1 * all_dim * math.log(factor) + 1)
     elif kind == "dynamic":
         if not trained > 0 or not factor >= 1 or rot == 2:
             raise ValueError("dynamic: factor from 1 and a context above 0")
@@ -211,7 +228,7 @@ def _scaling_fields(scaling: Mapping, rot: int, base: float, positions: int):
         ratio = number.get("factor", positions / trained)
         attention = math.sqrt(1 + math.log(ratio) / math.log(trained)) if ratio > 1 else 1.0
     attention = number.get("attention_factor", attention)
-    return base, _SCALINGS[kind], factor, trained, low, high, fast, slow, attention, divisors
+    return base, code, factor, trained, low, high, fast, slow, attention, divisors
 
 
 def rope_table(
@@ -234,9 +251,11 @@ def rope_table(
     "beta_slow" 1), "dynamic" ("factor", the context; another base for tables longer than
     that), "longrope" ("short_factor" and "long_factor", rot / 2 divisors each, the context:
     the long ones for tables longer than that), or "default".  "yarn" and "longrope"
-    multiply cosines and sines by ``0.1 ln(factor) + 1`` and ``sqrt(1 + ln(factor) /
+    multiply cosines and sines by ``0.1 ln(factor) + 1`` (with "mscale" and "mscale_all_dim" by
+    the ratio of ``0.1 mscale ln(factor) + 1`` of the two) and ``sqrt(1 + ln(factor) /
     ln(context))``, or by "attention_factor" where that is given ("longrope" without a
-    "factor": ``max_positions`` over the context).
+    "factor": ``max_positions`` over the context).  An entry that its type does not go by is
+    refused, not passed over.
 
     ``out`` is written where it is given ``[max_positions, rot]``, of its dtype."""
     if rot <= 0 or rot % 16 or rot > 256:

@@ -87,6 +87,9 @@ def test_c_decode_drafts_refuses(L, fp4):
         a = _drafts_args(fp4)
         setattr(a.decode, field, x)
         assert L.hcp_decode_drafts(ctypes.addressof(a), None) == status, (field, x)
+    a = _drafts_args(fp4)
+    a.decode.num_seqs, a.decode.num_heads, a.decode.num_kv_heads, a.max_tokens = 1024, 65536, 65536, 64
+    assert L.hcp_decode_drafts(ctypes.addressof(a), None) == U  # more merging waves than a launch has
     for field, x, status in (("row_starts", 0, E), ("q_rows", -1, E), ("q_rows", 1 << 31, U),
                              ("max_tokens", 0, E), ("max_tokens", 65, U)):
         a = _drafts_args(fp4)
@@ -208,6 +211,10 @@ def test_python_refuses():
                 {"base": math.nan}, {"dtype": torch.float64, "device": "cpu"}, {"device": "cpu"},
                 {"out": torch.zeros(10, 32)}, {"scaling": {"rope_type": "other"}}, {"scaling": {}},
                 {"scaling": {"rope_type": "linear"}},
+                {"scaling": {"rope_type": "linear", "factor": 2.0, "rope_theta": 5e5}},
+                {"scaling": {"rope_type": "default", "factor": 2.0}},
+                {"scaling": {"rope_type": "yarn", "factor": 4.0, "truncate": False,
+                             "original_max_position_embeddings": 8}},
                 {"scaling": {"rope_type": "yarn", "factor": 4.0}},
                 {"scaling": {"rope_type": "llama3", "factor": 4.0, "low_freq_factor": 1.0,
                              "original_max_position_embeddings": 8}},

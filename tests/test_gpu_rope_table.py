@@ -44,6 +44,8 @@ def frequencies(rot, base, scaling, positions):
         fs.append(f)
     if kind == "yarn":
         a = 0.1 * math.log(x) + 1
+        if "mscale" in s:
+            a = (1 + s["mscale"] * math.log(x) / 10) / (1 + s["mscale_all_dim"] * math.log(x) / 10)
     elif kind == "longrope":
         ratio = s.get("factor", positions / trained)
         a = math.sqrt(1 + math.log(ratio) / math.log(trained)) if ratio > 1 else 1.0
@@ -77,12 +79,15 @@ def test_sizes(dev, dtype, rot, positions):
     None, {"rope_type": "default"}, {"type": "linear", "rope_type": "linear", "factor": 2.5}, LLAMA3,
     {**LLAMA3, "low_freq_factor": 2.0, "factor": 32}, YARN, {**YARN, "beta_fast": 16, "beta_slow": 2},
     {**YARN, "attention_factor": 0.75}, {**YARN, "original_max_position_embeddings": 64},
+    {**YARN, "factor": 40, "mscale": 0.7, "mscale_all_dim": 1.2},
     {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 1000},
     {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 9000},
     {"rope_type": "longrope", "short_factor": [1.0] * 32, "long_factor": [1 + i / 3 for i in range(32)],
      "original_max_position_embeddings": 4096},
     {"rope_type": "longrope", "short_factor": [1.5] * 32, "long_factor": [9.0] * 32,
-     "original_max_position_embeddings": 5000, "factor": 32.0}])
+     "original_max_position_embeddings": 5000, "factor": 32.0},
+    {"rope_type": "longrope", "short_factor": [0.01] * 32, "long_factor": [0.1] * 32,
+     "original_max_position_embeddings": 9000, "attention_factor": 2.0}])
 @pytest.mark.parametrize("base", [10000.0, 500000.0])
 def test_scalings(dev, scaling, base):
     t = rope_table(5000, 64, base=base, scaling=scaling, device=dev)
