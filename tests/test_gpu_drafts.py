@@ -352,3 +352,68 @@ def test_merged_with_staged_keys(dev):
     # largest value)
     tol = 2.0 ** -8 * (3 * want.abs() + torch.cat([v.double(), lv]).abs().max())
     assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+def placed(dev, kind, k, v, dtype, kv=None):
+    """One sequence with these keys and values: (cache, table, what they (or kv) stand for)."""
+    n, hkv, d = k.shape
+    nb = -(-n // 16) + 1
+    cache = empty_cache(kind, nb, hkv, 16, d, dtype, dev)
+    reshape_and_cache(k.to(dev), v.to(dev), cache, torch.arange(n, device=dev))
+    k, v = kv or (k, v)
+    kv = (f4.stand_for(k), f4.stand_for(v)) if kind == "fp4" else (k.double(), v.double())
+    return cache, torch.arange(nb, dtype=torch.int32, device=dev)[None], kv
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_small_weights(dev, kind, dtype):
+    """A key in the first 32 of each wave far above 32764 others, 2^-14 of it each:
+    together they weigh half as much, so a bias of their weights shows.  (As many KV
+    heads, with the same keys, as leave a workgroup to each.)"""
+    gen, n, heads = torch.Generator().manual_seed(17), 32768, 512
+    k = (torch.randn(n, 1, 32, generator=gen) * 0.05).to(dtype)
+    v = (1 + 0.1 * torch.randn(n, 1, 32, generator=gen)).to(dtype)
+    k[5:128:32], v[5:128:32] = 0.375, -1.0
+    q = torch.ones(2, heads, 32, dtype=dtype)
+    cache, bt, kv = placed(dev, kind, k.to(dev).expand(n, heads, 32), v.to(dev).expand(n, heads, 32),
+                           dtype, (k, v))
+    out, lse = decode_drafts(q.to(dev), cache, bt, torch.tensor([n], device=dev),
+                             torch.tensor([0, 2], device=dev), 2, 0.81, with_lse=True)
+    assert (out == out[:, :1]).all() and (lse == lse[:1]).all()
+    check((out[:, :1], lse[:1]), q[:, :1], [2], [kv], 0.81, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["v031", "fp4"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("slope", [0.01, 0.04, -0.04, 0.3, 3.0])
+def test_scores_that_rise_and_fall(dev, kind, dtype, d, slope):
+    """Scores (of half of the query heads) that climb by ``slope`` a key, past the
+    maximum so far by less or by more than it is let stand, or fall."""
+    gen = torch.Generator().manual_seed(d)
+    n = 900
+    k = randn(gen, (n, 2, d), dtype) * 0.1
+    k[:, :, :32] = (slope * torch.arange(n) / 32)[:, None, None].to(dtype)
+    v = randn(gen, (n, 2, d), dtype)
+    q = randn(gen, (3, 8, d), dtype)
+    q[:, ::2, :32] = 1.0
+    cache, bt, kv = placed(dev, kind, k.to(dtype), v, dtype)
+    got = decode_drafts(q.to(dev), cache, bt, torch.tensor([n], device=dev),
+                        torch.tensor([0, 3], device=dev), 3, 1.0, with_lse=True)
+    check(got, q, [3], [kv], 1.0, dtype)
+
+
+def test_rows_of_out_on_top_of_each_other_are_refused(dev):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=dev)
+    cache = torch.zeros(2, 2, 16, 128, dtype=torch.bfloat16, device=dev)
+    bt, lens = torch.zeros(2, 1, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int64, device=dev)
+    starts = torch.tensor([0, 1, 2], device=dev)
+    room = torch.zeros(4096, dtype=torch.bfloat16, device=dev)
+    for strides in ((255, 64, 1), (256, 63, 1), (64, 127, 1), (0, 64, 1), (256, 0, 1)):
+        with pytest.raises(ValueError, match="out"):
+            decode_drafts(q, cache, bt, lens, starts, 1, 0.1, out=room.as_strided((2, 4, 64), strides))
+    heads_first = room.as_strided((2, 4, 64), (64, 128, 1))
+    assert decode_drafts(q, cache, bt, lens, starts, 1, 0.1, out=heads_first) is heads_first
+    assert decode_drafts(q[:0], cache, bt, lens, starts, 1, 0.1).shape == (0, 4, 64)
+    assert decode_drafts(q, cache, bt, lens[:0], starts[:1], 1, 0.1).shape == (2, 4, 64)
