@@ -22,6 +22,17 @@
 // Only the chunks around the tokens' own positions (and a window's start) hold
 // keys that some rows see and others do not: there infinities and NaN of V become
 // zeros in LDS, and are added to the rows that see them when the waves are combined.
+//
+// Bound by HBM at long contexts: 64 x 5 tokens over 16k-32k keys, 28 / 4 heads of 128
+// columns in bf16 (3.27 GB), 506 us and 7 to join, 6.4 TB/s; with the arithmetic left out
+// it takes 513 in all.  After many launches in a row the clock falls, and with
+// it the products' rate: 538.  A window of 4096 at 16 / 8 x 256 (502 MB) 86 us, 5.9
+// TB/s.  Over the 4-bit cache the products and conversions bound it: 48 x 4 tokens over
+// 8k-32k keys, 64 / 8 x 128 (907 MB), 200 us, 253 at the low clock, 167 without
+// arithmetic.  24 x 1-6 tokens over 512-8192 keys (211 MB) 45 us, where the bytes take 32:
+// what a split begins and ends with.  One sequence of 900 keys 10 us, waits all of them.
+// Loading K one and a half chunks ahead, through LDS freed by the scores, was no faster
+// (560 us for 550 of the first, on one card).
 #include "decode_fp4.h"
 
 namespace hcp {

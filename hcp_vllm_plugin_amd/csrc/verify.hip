@@ -20,8 +20,16 @@
 //    2048.
 //  4 verify_residual (with q): the sum of r.
 //  5 verify_pick: the slice, and in it the token.
+// Few slices are decided by every workgroup of verify_sums for itself (1 x 4 rows of 32000:
+// 18 us a call for 20); at 64 sequences or more with up to 65536 tokens a workgroup does 2
+// to 5 for its sequence (verify_finish: 200 x 1-8 rows of 50257 float32 56 us a call for 74).
 // Sums are added in an order that the sizes alone decide, so that a call gives the same
 // tokens every time.
+//
+// 64 x 5 rows of 152064 bf16 logits with q (97 MB of logits read, 39 MB of the drawn
+// rows' q): 19 us, 6, 11, 10 and 5; the two sums in 64 bits are bound by their
+// exponentials and by starting behind one another.  200 x 1-8 rows of 50257
+// probabilities: 29 us (177 MB) and 20.
 #include "params.h"
 
 namespace hcp {
