@@ -21,8 +21,8 @@
 //  4 verify_residual (with q): the sum of r.
 //  5 verify_pick: the slice, and in it the token.
 // Few slices are decided by every workgroup of verify_sums for itself (1 x 4 rows of 32000:
-// 18 us a call for 20); at 64 sequences or more with up to 65536 tokens a workgroup does 2
-// to 5 for its sequence (verify_finish: 200 x 1-8 rows of 50257 float32 56 us a call for 74).
+// 18 us a call for 20); in small vocabularies a workgroup does 2 to 5 for its sequence
+// (verify_finish: 200 x 1-8 rows of 50257 float32 probabilities 56 us a call for 74).
 // Sums are added in an order that the sizes alone decide, so that a call gives the same
 // tokens every time.
 //
@@ -400,7 +400,8 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
       } else {
         const double w = weight<PROBS>(xd, sm.top[lane], s.rate), v = uq * sm.z[lane];
         ok = v < w;
-        near = fabs(v - w) <= kSumError * w;
+        // (probabilities may pass 32 bits' range in a thread's sum)
+        near = fabs(v - w) <= kSumError * w || !(sm.z[lane] < INFINITY);
         sm.uq[lane] = uq;
         sm.w[lane] = w;
       }
@@ -758,16 +759,21 @@ static hipError_t launch_verify_t(const VerifyParams& p, hipStream_t st) {
   hipLaunchKernelGGL((verify_stats_kernel<T, PROBS>),
                      dim3(static_cast<unsigned>(p.num_seqs * p.max_tokens * p.stat_slices)), t, 0,
                      st, p);
-  // Many sequences over a vocabulary that one workgroup goes over soon enough: steps 2 to 5
-  // at once (200 x 50257 of probabilities 20 us for 27).  Few of them: step 2 in every
-  // workgroup of step 3, a launch less.
-  if (p.vocab <= kVerSmall && p.num_seqs >= 64) {
+  // Steps 2 to 5 at once where one workgroup goes over the vocabulary as soon as four launches
+  // do: one round of 8192 logits (1 x 4000 16 us for 19, 128 x 8192 16 for 20; but 1 x
+  // 12000 20 for 18, 64 x 50257 48 for 34, their exponentials), four of probabilities (1 x
+  // 32000 15.0 for 15.3, 64 x 24000 19 for 23), eight of them for many sequences (64 x 65000
+  // 34.4 for 34.5, 128 x 50257 40 for 46, but 16 x 50257 21 for 18).
+  if (p.vocab <= (PROBS ? p.num_seqs >= 64 ? kVerSmall : kVerSmall / 2 : kVerSmall / 8)) {
     hipLaunchKernelGGL((verify_finish_kernel<T, PROBS>), seqs, dim3(1024), 0, st, p);
     return hipGetLastError();
   }
   const int64_t n = static_cast<int64_t>(p.num_seqs) * p.sum_slices;
   const dim3 slices(static_cast<unsigned>(n));
-  if (n <= 1024) {
+  // Few slices: step 2 in every workgroup of step 3, a launch less, of which all are on
+  // the chip at once (1200 slices of logits 27 us for 28, 2048 39.7 for 37.6; 2048 of
+  // probabilities 32 for 35, 3200 47 for 46).
+  if (n <= (PROBS ? 2048 : 1536)) {
     hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false, true>), slices, t, 0, st, p);
   } else {
     hipLaunchKernelGGL((verify_decide_kernel<T, PROBS>), seqs, t, 0, st, p);

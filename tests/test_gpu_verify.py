@@ -289,3 +289,70 @@ def test_captured_replayed_and_on_two_streams(dev):
     torch.cuda.synchronize()
     for o in outs:
         check_verified(o, want, 5)
+
+
+@pytest.mark.parametrize("front,back", [(0, 40000), (33001, 0), (9000, 31000)])
+@pytest.mark.parametrize("edges", [
+    test_borders, test_near_borders, test_drafts_that_are_no_tokens, test_sequences_without_rows,
+    test_equal_entries_go_to_the_lowest_index])
+def test_edges_in_large_vocabularies(dev, monkeypatch, edges, front, back):
+    """The same among tokens without weight, so many that a sequence's row takes several
+    workgroups: the tokens of the small ones, `front` further on."""
+    def wider(dev, c):
+        pad = torch.nn.functional.pad
+        more = {**c, "target": pad(c["target"], (front, back), value=0.0 if c["probs"] else -INF)}
+        if c["draft_probs"] is not None:
+            more["draft_probs"] = pad(c["draft_probs"], (front, back))
+        d, v = c["tokens"], c["target"].shape[1]
+        more["tokens"] = torch.where((d >= 0) & (d < v), d + front, torch.full_like(d, -1))
+        want, small = compare_(dev, more), verify(
+            c["target"], c["tokens"], c["query_start_loc"], c["uniform"], c["draft_probs"],
+            c["temperature"], c["probs"])
+        assert [[t - front for t in w] for w in want] == small
+        return small
+
+    monkeypatch.setitem(globals(), "compare", wider)
+    edges(dev)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q", [True, False])
+@pytest.mark.parametrize("v", [20000, 70001])
+def test_infinities_and_nan_in_large_vocabularies(dev, dtype, q, v):
+    gen = torch.Generator().manual_seed(13)
+    c = case(gen, [3] * 9 + [1] * 3, v, dtype, 3, q=q)
+    x = c["target"]
+    x[0:3, 100:] = -INF
+    x[3:6, :v - 7] = torch.finfo(dtype).min
+    x[6:9, ::3] = float("nan")
+    x[9] = -INF
+    x[10:12] = float("nan")
+    x[12:15, [5, v - 1]] = INF
+    x[15:18] = -INF
+    x[15:18, v - 1234] = -5.0
+    x[18:21] = torch.finfo(dtype).min
+    x[21:24, 8192:] = float("nan")
+    compare(dev, c)
+    c["temperature"][:] = 0
+    compare(dev, c)
+    if q:
+        c["temperature"][:] = 0.9
+        c["draft_probs"][0] = 0.0
+        c["draft_probs"][1, :, ::2] = float("nan")
+        compare(dev, c)
+
+
+@pytest.mark.parametrize("v", [100, 3000, 40000])
+def test_probabilities_of_any_size(dev, v):
+    """Weights whose sum passes 32 bits' range, and subnormal ones."""
+    for w in (3e38, 1e-42):
+        x = torch.full((6, v), w)
+        x[:, ::7] = 0.0
+        x[2:4, 3] = w / 4
+        dp = torch.full((3, 1, v), 1.0 / v)
+        for u in (0.1, 0.9):
+            c = dict(target=x, tokens=torch.tensor([0, 1, 0, 3, 0, 7]),
+                     query_start_loc=torch.arange(0, 7, 2), uniform=torch.tensor([[u, 0.37]] * 3),
+                     draft_probs=dp, temperature=None, probs=True)
+            compare(dev, c)
+            compare(dev, {**c, "draft_probs": None})
