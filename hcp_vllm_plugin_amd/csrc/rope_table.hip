@@ -9,7 +9,7 @@
 // leading terms x and 1 - x^2 / 2), off by 2^-28 and 2^-31, so that 32-bit rounding is
 // what counts: 2^-22.9 and 2^-23.4 measured over 2 million angles, 4.9e-8 on average where a
 // float32's rounding alone is 2.1e-8.  (With angle and polynomials in 64 bits a float32 table of
-// 131072 x 128 took 13.7 us for 12.3; no model's rotation is that exact behind the table.)
+// 131072 x 128 took 13.7 us for 12.3; what is rotated with it is rounded to 16 bits or fewer.)
 //
 // Bound by the writes: nothing is read but the frequencies, which are kernel arguments.  A
 // pair takes 24 instructions; reduced in 64-bit floating point to quarters of a turn it
