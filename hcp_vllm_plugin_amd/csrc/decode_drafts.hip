@@ -775,12 +775,15 @@ decode_drafts_kernel(DraftParams p) {
   paged_shares<NT, K::START * RT, K::LEAST, K::LATE, false>(
       p.p, wg, sm_len, sm_all, sm_w, sm_cut,
       [&](int all, int len) { return len > 0 ? (all - first_chunk(all, len) + 31) >> 5 : 0; },
-      [&](const PagedDecParams&, int j, int seen) {
+      [&](const PagedDecParams&, int j, int& all, int) __attribute__((always_inline)) {
         int row0;
         const int n = draft_rows(p, starts[j], starts[j + 1], row0);
+        if (n == 0) return 0;
+        // (keys of tokens that are not run are behind those that are)
+        const int64_t rest = starts[j + 1] - starts[j] - n;
+        all = rest < all ? all - static_cast<int>(rest) : 0;
         const uint32_t reach = static_cast<uint32_t>(p.window) + n - 1;  // of the first token's window
-        return n == 0 ? 0 : p.window > 0 && static_cast<uint32_t>(seen) > reach
-                                ? static_cast<int>(reach) : seen;
+        return p.window > 0 && static_cast<uint32_t>(all) > reach ? static_cast<int>(reach) : all;
       });
   const int r0 = __builtin_amdgcn_readfirstlane(sm_cut[0]);
   const int o0 = __builtin_amdgcn_readfirstlane(sm_cut[1]);

@@ -55,10 +55,11 @@ __device__ __forceinline__ void paged_lens(const void* lens, bool wide, int r, i
 // workgroup of NT threads gets its share in sm_cut: first sequence (-1: none) and
 // first chunk of it, last sequence and the end in its chunks; sm_len / sm_all
 // [kDecMaxSeqs] get the keys of every sequence (sm_all -1: HCP_LEN_NOT_RUN).
-// STARTS: p.starts counts.  last(p, j, seen): how many of its `seen` keys the
-// thread's j-th sequence looks at, the last ones.  Ends with a barrier.
+// STARTS: p.starts counts.  last(p, j, all, seen): how many of its `seen` keys the
+// thread's j-th sequence looks at, the last ones; may make `all` less.  Ends with a
+// barrier.
 struct LastWindow {
-  __device__ __forceinline__ int operator()(const PagedDecParams& p, int, int seen) const {
+  __device__ __forceinline__ int operator()(const PagedDecParams& p, int, int, int seen) const {
     return p.window > 0 && seen > p.window ? p.window : seen;
   }
 };
@@ -82,7 +83,7 @@ __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, i
   for (int j = 0; j < EPT; ++j) {
     const int r = tid * EPT + j;
     const int64_t given = r < n ? lens[j] : 0;
-    const int all =  // keys that the sequence's query sees; max_len < 2^31
+    int all =  // keys that the sequence's query sees; max_len < 2^31
         static_cast<int>(given < 0 ? 0 : given < p_.max_len ? given : p_.max_len);
     int seen = all;
     if constexpr (STARTS) {
@@ -91,7 +92,7 @@ __device__ __forceinline__ void paged_shares(const PagedDecParams& p_, int wg, i
         seen = s <= 0 ? all : s < all ? all - static_cast<int>(s) : 0;
       }
     }
-    const int len = last(p_, j, seen);
+    const int len = last(p_, j, all, seen);
     if (r < n) {
       sm_all[r] = given == HCP_LEN_NOT_RUN ? -1 : all;
       sm_len[r] = len;

@@ -41,8 +41,8 @@ def decode_drafts(
     """Attention of q ``[T, H, D]`` (fp16 / bf16), whose rows ``query_start_loc[r]`` ..
     ``query_start_loc[r + 1] - 1`` are the last n tokens of sequence r, over a paged cache
     that holds their keys: token i of them sees keys ``[0, seq_lens[r] - n + 1 + i)`` of
-    row r of ``block_table``, the last ``window`` of them.  n is at most ``max_tokens``
-    (1 to 64); what a sequence has past that, and rows past q's, are not run.
+    row r of ``block_table``, the last ``window`` of them.  The first ``max_tokens`` (1 to
+    64) of a sequence's n are run; the others, and those in rows past q's, are not.
 
     ``kv_cache`` is of q's dtype, in either 16-bit layout, or a 4-bit cache (uint8).
     Lengths (int32 / int64 ``[S]``), row starts (``[S + 1]``, of their dtype) and block ids

@@ -857,7 +857,8 @@ int hcp_step_tables(const hcp_step_tables_args* args, void* stream);
  * NaN score makes its row NaN).
  *   row_starts   DEVICE [num_seqs + 1], of lens_dtype
  *   q_rows       rows of q; tokens in rows past them, or past max_tokens of their
- *                sequence, are not run, and no other row of out and lse is written
+ *                sequence, are not run (n counts them all the same), and no other row of
+ *                out and lse is written
  * A row that sees no key gets 0 and LSE -inf.  What a row does not see does not reach
  * it, whatever it is.  max_tokens is at most HCP_DRAFTS_MAX_TOKENS.
  */

@@ -218,6 +218,26 @@ def test_rows_that_are_not_run(dev, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [None, 40])
+def test_the_first_tokens_of_many(dev, kind, window):
+    """max_tokens below a sequence's tokens, and rows past q: those that run see what they
+    would with the others beside them."""
+    gen = torch.Generator().manual_seed(13)
+    lens, counts = [300, 200, 30, 5, 90], [9, 3, 5, 7, 6]
+    q, cache, bt, starts, kvs = batch(gen, dev, lens, counts, 8, 2, 64, 16, torch.bfloat16, kind)
+    for most, rows in ((4, 30), (9, 26), (1, 30)):
+        out, lse = decode_drafts(q[:rows].to(dev), cache, bt.to(dev),
+                                 torch.tensor(lens, dtype=torch.int32, device=dev), starts.to(dev),
+                                 most, scale_for(64), window=window, with_lse=True)
+        for r, n in enumerate(counts):
+            ran, at = min(n, most, max(0, rows - int(starts[r]))), int(starts[r])
+            left = max(0, lens[r] - (n - ran))  # (five keys of seven tokens: the first see none)
+            kv = tuple(x[:left] for x in kvs[r])
+            check((out[at:at + ran], lse[:, at:at + ran]), q[at:at + ran], [ran], [kv], scale_for(64),
+                  torch.bfloat16, window)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_lengths_past_the_table_and_ids_past_the_cache(dev, kind):
     gen = torch.Generator().manual_seed(6)
     b = batch(gen, dev, [64, 64], [3, 2], 8, 2, 128, 16, torch.bfloat16, kind)
