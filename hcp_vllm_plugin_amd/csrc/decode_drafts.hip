@@ -758,6 +758,8 @@ decode_drafts_kernel(DraftParams p) {
   __shared__ __attribute__((aligned(16))) char sm_q[RT * K::QSTEPS <= 8 ? 16 : 16 * RT * 2 * D];
   __shared__ float sm_m[W][16 * RT], sm_l[W][16 * RT];
   __shared__ int sm_len[kDecMaxSeqs], sm_all[kDecMaxSeqs];  // keys seen, in the cache (-1: not run)
+  __shared__ int sm_row0[kDecMaxSeqs];    // rows that are run: the first, their number
+  __shared__ uint8_t sm_n[kDecMaxSeqs];
   __shared__ int sm_w[2][W];
   __shared__ int sm_cut[4], sm_odd;
   int kvh_;
@@ -779,6 +781,8 @@ decode_drafts_kernel(DraftParams p) {
         int row0;
         const int n = draft_rows(p, starts[j], starts[j + 1], row0);
         if (n == 0) return 0;
+        sm_row0[threadIdx.x * EPT + j] = row0;
+        sm_n[threadIdx.x * EPT + j] = static_cast<uint8_t>(n);
         // (keys of tokens that are not run are behind those that are)
         const int64_t rest = starts[j + 1] - starts[j] - n;
         all = rest < all ? all - static_cast<int>(rest) : 0;
@@ -801,11 +805,9 @@ decode_drafts_kernel(DraftParams p) {
       if (b == 0) global_ptr(p.p.seq_slots)[2 * r] = wg + r;
       if (e == c) global_ptr(p.p.seq_slots)[2 * r + 1] = wg + r;
     }
-    int row0 = 0;
-    const int n = __builtin_amdgcn_readfirstlane(
-        draft_rows(p, draft_start(p, r), draft_start(p, r + 1), row0));
+    const int n = __builtin_amdgcn_readfirstlane(sm_n[r]);
     if (16 * RT * chunk >= n * p.p.d.group) continue;  // this chunk of rows is empty
-    row0 = __builtin_amdgcn_readfirstlane(row0);
+    const int row0 = __builtin_amdgcn_readfirstlane(sm_row0[r]);
     const int end = base + 32 * e;
     drafts_split_body<Keys, D, T, RT>(p, kvh, chunk, wg + r, r, row0, n, all - len, all,
                                       base + 32 * b, end < all ? end : all, bufE, bufO, sm_q, sm_m,
