@@ -353,28 +353,34 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
                                             bool write = true) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const VerifySeq s = verify_seq(p, b);
-  // lane i of every wave looks at draft i: fetched while the slices' sums are
+  // lane i of every wave looks at draft i.  Its token is fetched with the slices' sums of
+  // the wave's first row, its numbers while those are added up
   const bool mine = lane + 1 < s.n;
+  auto stats_of = [&](int j) __attribute__((always_inline)) {
+    return p.stats + (static_cast<int64_t>(b) * p.max_tokens + j) * p.stat_slices;
+  };
+  auto first_of = [&](int j) __attribute__((always_inline)) {  // of this lane's first slice
+    VerifyStat o{-INFINITY, 0x7fffffff, 0.0};
+    if (j < s.n && lane < p.stat_slices) o = global_ptr(stats_of(j))[lane];
+    return o;
+  };
+  VerifyStat slice = first_of(wave);
   const int64_t d = mine ? draft_token(p, s.row0 + lane + 1) : -1;
   const bool token = d >= 0 && d < p.vocab;
-  float xd = -INFINITY;
-  double uq = 0.0;
+  float xd = -INFINITY, ud = 0.f, qd = 1.f;
   if (token && !s.greedy) {
     xd = static_cast<float>(
         global_ptr(reinterpret_cast<const T*>(target_row(p, s.row0 + lane)))[d]);
-    uq = global_ptr(p.uniform)[b * p.uniform_stride + lane];
+    ud = global_ptr(p.uniform)[b * p.uniform_stride + lane];
     if (p.draft_probs != nullptr)
-      uq *= static_cast<double>(
-          global_ptr(p.draft_probs)[b * p.q_stride_seq + lane * p.q_stride_row + d]);
+      qd = global_ptr(p.draft_probs)[b * p.q_stride_seq + lane * p.q_stride_row + d];
   }
   // the rows' maxima and sums from those of their slices
   for (int j = wave; j < s.n; j += W) {
-    const VerifyStat* const st =
-        p.stats + (static_cast<int64_t>(b) * p.max_tokens + j) * p.stat_slices;
-    VerifyStat own{-INFINITY, 0x7fffffff, 0.0};  // of this lane's first slice
-    if (lane < p.stat_slices) own = global_ptr(st)[lane];
-    float m = own.top;
-    int at = own.index;
+    const VerifyStat* const st = stats_of(j);
+    if (j > wave) slice = first_of(j);
+    float m = slice.top;
+    int at = slice.index;
     for (int i = lane + 64; i < p.stat_slices; i += 64)
       best_of(m, at, global_ptr(st)[i].top, global_ptr(st)[i].index);
 #pragma unroll
@@ -382,7 +388,7 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
     auto part = [&](const VerifyStat& o) __attribute__((always_inline)) {
       return PROBS ? o.sum : o.sum > 0.0 ? o.sum * weight<false>(o.top, m, s.rate) : 0.0;
     };
-    double z = part(own);
+    double z = part(slice);
     for (int i = lane + 64; i < p.stat_slices; i += 64) z += part(global_ptr(st)[i]);
     z = wave_sum(z);
     if (lane == 0) {
@@ -393,6 +399,7 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
   }
   __syncthreads();
   if (wave == 0) {
+    const double uq = static_cast<double>(ud) * static_cast<double>(qd);
     bool ok = false, near = false;
     if (token) {
       if (s.greedy) {
