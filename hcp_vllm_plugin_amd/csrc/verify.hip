@@ -78,18 +78,18 @@ __device__ __forceinline__ void load8(const void* row, int g, int v, float fill,
     if (8 * g + j < v) x[j] = static_cast<float>(global_ptr(at)[j]);
   }
 }
-// N of them, groups g, g + kVerThreads, ..; `end`: past the workgroup's last element.  (A
+// N of them, groups g, g + STEP, ..; `end`: past the workgroup's last element.  (A
 // branch around every load would have each waited for by itself: 64 x 5 rows of 152064
 // bf16 took 21 us.)
-template <typename T, int N>
+template <typename T, int N, int STEP = kVerThreads>
 __device__ __forceinline__ void load8s(const void* row, int g, int end, int v, float fill,
                                        float (&x)[N][8]) {
   if (end <= v) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) load8_full<T>(row, g + k * kVerThreads, x[k]);
+    for (int k = 0; k < N; ++k) load8_full<T>(row, g + k * STEP, x[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) load8<T>(row, g + k * kVerThreads, v, fill, x[k]);
+    for (int k = 0; k < N; ++k) load8<T>(row, g + k * STEP, v, fill, x[k]);
   }
 }
 
@@ -273,34 +273,36 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyParams 
     }
     if (lane == 0) sm_i[wave] = at;
   } else {
-    float sum = 0.f;
+    // (six additions deep: what their rounding may come to is in kSumError)
+    float sums[8] = {};
+    auto add = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[e] += f(x[k][e]);
+    };
+    float scale = 1.f;
     if constexpr (PROBS) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += x[k][e] > 0.f && x[k][e] < INFINITY ? x[k][e] : 0.f;
+      add([](float v) __attribute__((always_inline)) { return v > 0.f && v < INFINITY ? v : 0.f; });
     } else if (m == INFINITY) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += x[k][e] == INFINITY ? 1.f : 0.f;
+      add([](float v) __attribute__((always_inline)) { return v == INFINITY ? 1.f : 0.f; });
     } else if (m > -INFINITY) {
       // (x - m) c in one fma: what m c loses to rounding is the same power for all
       const float c = fminf(static_cast<float>(s.rate), 0x1p126f);
       const float mc = m * c, lost = __builtin_fmaf(m, c, -mc);
       if (c > 0.f && fabsf(mc) < 0x1p100f) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum += fast_exp2(__builtin_fmaf(x[k][e], c, -mc));
-        sum *= fast_exp2(-lost);
+        add([&](float v) __attribute__((always_inline)) {
+          return fast_exp2(__builtin_fmaf(v, c, -mc));
+        });
+        scale = fast_exp2(-lost);
       } else {  // (a NaN, of -inf times 0, to 0)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum += fast_exp2(fmaxf((x[k][e] - m) * c, -INFINITY));
+        add([&](float v) __attribute__((always_inline)) {
+          return fast_exp2(fmaxf((v - m) * c, -INFINITY));
+        });
       }
     }
+    const float sum = scale * (((sums[0] + sums[1]) + (sums[2] + sums[3])) +
+                               ((sums[4] + sums[5]) + (sums[6] + sums[7])));
     d = wave_sum(sum);
     if (lane == 0) sm_s[wave] = d;
   }
@@ -331,10 +333,12 @@ __device__ __forceinline__ double block_sum(double x, double* sm) {
   return r;
 }
 
-// How far the 32-bit sums may be off, relative: a weight by 2^-22 and its argument's
-// share, 2^-23 of |log2 w|, which over a row averages to its entropy (17.2 bits at
-// 150000 tokens, 24 at most here); the additions in a thread by 32 steps of 2^-24.
-constexpr double kSumError = 1e-5;
+// How far the 32-bit sums may be off, relative.  A weight's argument, log2 w, by 2^-23 of
+// itself (its factor's rounding and its own; 3 2^-24 where the products are large): the
+// weight by ln 2 times that, which over the weights of a slice, the largest of them 1, averages
+// to no more than its entropy, 13 bits; 1.6e-6.  The exponential and the factor of the
+// whole by 2^-23 and 2^-22, six additions and a product by 2^-24 each: 0.8e-6.
+constexpr double kSumError = 2.5e-6;
 
 template <int W>
 struct DecideShared {
@@ -408,7 +412,7 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
         const double w = weight<PROBS>(xd, sm.top[lane], s.rate), v = uq * sm.z[lane];
         ok = v < w;
         // (probabilities may pass 32 bits' range in a thread's sum)
-        near = fabs(v - w) <= kSumError * w || !(sm.z[lane] < INFINITY);
+        near = w > 0.0 && (fabs(v - w) <= kSumError * w || !(sm.z[lane] < INFINITY));
         sm.uq[lane] = uq;
         sm.w[lane] = w;
       }
@@ -424,14 +428,16 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
   for (; taken + 1 < s.n; ++taken) {  // (the same in every thread)
     if (sm.near >> taken & 1) {  // too near to tell: the row in 64 bits
       const char* const row = target_row(p, s.row0 + taken);
-      double x = 0.0;
-      for (int g = tid; g < (p.vocab + 7) / 8; g += 64 * W) {
-        float e[8];
-        load8<T>(row, g, p.vocab, -INFINITY, e);
+      double x[4] = {};
+      for (int g = tid; g < (p.vocab + 7) / 8; g += 4 * 64 * W) {  // four on their way
+        float e[4][8];
+        load8s<T, 4, 64 * W>(row, g, 8 * (g + 3 * 64 * W + 1), p.vocab, -INFINITY, e);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x += weight<PROBS>(e[k], sm.top[taken], s.rate);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[i] += weight<PROBS>(e[i][k], sm.top[taken], s.rate);
       }
-      if (!(sm.uq[taken] * block_sum<W>(x, sm.sums) < sm.w[taken])) break;
+      if (!(sm.uq[taken] * block_sum<W>((x[0] + x[1]) + (x[2] + x[3]), sm.sums) < sm.w[taken])) break;
     } else if (!(sm.ok >> taken & 1)) {
       break;
     }
@@ -465,10 +471,12 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
   return sm.row;
 }
 
+// (16 waves to a sequence for the drafts that are too near: a row of 152064 logits in 35 us, 49
+// with four; one in 10^5 is)
 template <typename T, bool PROBS>
-__global__ __launch_bounds__(kVerThreads) void verify_decide_kernel(VerifyParams p) {
-  __shared__ DecideShared<kVerWaves> sm;
-  const VerifyRow o = decide<T, PROBS, kVerWaves>(p, blockIdx.x, sm);
+__global__ __launch_bounds__(1024) void verify_decide_kernel(VerifyParams p) {
+  __shared__ DecideShared<16> sm;
+  const VerifyRow o = decide<T, PROBS, 16>(p, blockIdx.x, sm);
   if (threadIdx.x == 0) p.rows[blockIdx.x] = o;
 }
 
@@ -783,7 +791,7 @@ static hipError_t launch_verify_t(const VerifyParams& p, hipStream_t st) {
   if (n <= (PROBS ? 2048 : 1536)) {
     hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false, true>), slices, t, 0, st, p);
   } else {
-    hipLaunchKernelGGL((verify_decide_kernel<T, PROBS>), seqs, t, 0, st, p);
+    hipLaunchKernelGGL((verify_decide_kernel<T, PROBS>), seqs, dim3(1024), 0, st, p);
     hipLaunchKernelGGL((verify_sums_kernel<T, PROBS, false, false>), slices, t, 0, st, p);
   }
   if (p.draft_probs != nullptr)
