@@ -13,17 +13,19 @@
 //
 // Bound by the writes: nothing is read but the frequencies, which are kernel arguments.  A
 // pair takes 24 instructions; reduced in 64-bit floating point to quarters of a turn it
-// took 40, and a 1000003 x 128 bf16 table (256 MB) 59 us; so 40 (6.4 TB/s).  131072 x 128 in
-// float32 (67 MB) 11 us, as long as a fill; 4096 x 64 2.6.
+// took 40, and a 1000003 x 128 bf16 table (256 MB) 59 us; so 39 into one buffer, 43 a call into
+// others (a fill takes 36.6 and 38.5).  131072 x 128 in float32 (67 MB) 12, a fill 11.3; 4096 x 64
+// 2.6.
 #include "params.h"
 
 namespace hcp {
 
 constexpr int kTableThreads = 256;
-// Twice as many workgroups as are on the chip at once, each with rows in a row (five tables of
-// 1000003 x 128 in turn 47 us, 52 with half as many; 48 with 2048 workgroups that take
-// rows far apart, and 13.7 for 12.7 of 131072 x 128 float32).
-constexpr int kTableBlocks = 4096;
+// A workgroup makes four passes over rows in a row, fewer where that leaves less than eight
+// workgroups to a CU.  (1000003 x 128 bf16 into another buffer each time 43 us; with three, five
+// and eight passes 45, 49 and 50, with 2048 workgroups that take rows far apart 48.  131072 x
+// 128 float32 11.8 for 12.)
+constexpr int kTableBlocks = 2048, kTablePasses = 4;
 
 // A workgroup writes `rows` rows in a row, a thread 16 bytes of cosines and 16 of sines of
 // every step-th of them.
@@ -74,7 +76,8 @@ __global__ __launch_bounds__(kTableThreads) void rope_table_kernel(RopeTablePara
 hipError_t launch_rope_table(const RopeTableParams& p, int dtype, hipStream_t st) {
   const int64_t per = p.rot / 2 / (dtype == HCP_DTYPE_F32 ? 4 : 8);
   const int64_t step = kTableThreads / per;  // rows of a workgroup's pass
-  const int64_t passes = (p.num_positions + step * kTableBlocks - 1) / (step * kTableBlocks);
+  const int64_t some = (p.num_positions + step * kTableBlocks - 1) / (step * kTableBlocks);
+  const int64_t passes = some < kTablePasses ? some : kTablePasses;
   const int rows = static_cast<int>(step * passes);
   const dim3 g(static_cast<unsigned>((p.num_positions + rows - 1) / rows)), b(kTableThreads);
   if (dtype == HCP_DTYPE_F32)
