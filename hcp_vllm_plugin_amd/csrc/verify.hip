@@ -27,7 +27,7 @@
 // tokens every time.
 //
 // 64 x 5 rows of 152064 bf16 logits with q (97 MB of logits read, 39 MB of the drawn
-// rows' q): 19 us, 6, 11, 10 and 5; the two sums in 64 bits are bound by their
+// rows' q): 18 us, 5, 11, 10 and 5; the two sums in 64 bits are bound by their
 // exponentials and by starting behind one another.  200 x 1-8 rows of 50257
 // probabilities: 29 us (177 MB) and 20.
 #include "params.h"
