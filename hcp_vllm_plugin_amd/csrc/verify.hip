@@ -287,17 +287,20 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyParams 
     } else if (m == INFINITY) {
       add([](float v) __attribute__((always_inline)) { return v == INFINITY ? 1.f : 0.f; });
     } else if (m > -INFINITY) {
-      // (x - m) c in one fma: what m c loses to rounding is the same power for all
+      // (x - m) c in one fma: what m c loses to rounding, 1/8 at most, is the same power for
+      // all.  (Without that bound it would pass the exponent's range: m = 30 at a temperature
+      // of 10^-8 has lost = 200.)
       const float c = fminf(static_cast<float>(s.rate), 0x1p126f);
       const float mc = m * c, lost = __builtin_fmaf(m, c, -mc);
-      if (c > 0.f && fabsf(mc) < 0x1p100f) {
+      if (c > 0.f && fabsf(mc) < 0x1p22f) {
         add([&](float v) __attribute__((always_inline)) {
           return fast_exp2(__builtin_fmaf(v, c, -mc));
         });
         scale = fast_exp2(-lost);
-      } else {  // (a NaN, of -inf times 0, to 0)
+      } else {  // (halves where v - m may pass 32 bits' range; a NaN, of -inf times 0, to 0)
+        const float h = fabsf(m) < 0x1p100f ? 1.f : 0.5f, ch = c / h, mh = m * h;
         add([&](float v) __attribute__((always_inline)) {
-          return fast_exp2(fmaxf((v - m) * c, -INFINITY));
+          return fast_exp2(fmaxf(__builtin_fmaf(v, h, -mh) * ch, -INFINITY));
         });
       }
     }
@@ -334,11 +337,13 @@ __device__ __forceinline__ double block_sum(double x, double* sm) {
 }
 
 // How far the 32-bit sums may be off, relative.  A weight's argument, log2 w, by 2^-23 of
-// itself (its factor's rounding and its own; 3 2^-24 where the products are large): the
-// weight by ln 2 times that, which over the weights of a slice, the largest of them 1, averages
-// to no more than its entropy, 13 bits; 1.6e-6.  The exponential and the factor of the
-// whole by 2^-23 and 2^-22, six additions and a product by 2^-24 each: 0.8e-6.
-constexpr double kSumError = 2.5e-6;
+// itself (its factor's rounding and its own, and 2^-27 for what m c lost; 3 2^-24 where the
+// products are large): the weight by ln 2 times that, which over the weights of a slice, the
+// largest of them 1, averages to no more than its entropy, 13 bits; 1.6e-6.  The exponential
+// and the factor of the whole by 2^-23 and 2^-22, six additions and a product by 2^-24 each:
+// 0.8e-6.  For rates of kLeastRate to kMostRate, which the kernel's 32-bit factor holds to
+// 2^-24.
+constexpr double kSumError = 2.5e-6, kLeastRate = 0x1p-126, kMostRate = 0x1p126;
 
 template <int W>
 struct DecideShared {
@@ -411,8 +416,11 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
       } else {
         const double w = weight<PROBS>(xd, sm.top[lane], s.rate), v = uq * sm.z[lane];
         ok = v < w;
-        // (probabilities may pass 32 bits' range in a thread's sum)
-        near = w > 0.0 && (fabs(v - w) <= kSumError * w || !(sm.z[lane] < INFINITY));
+        // (probabilities may pass 32 bits' range in a thread's sum; the largest weight of
+        // logits is 1, so that a sum below that would be none)
+        near = w > 0.0 && (fabs(v - w) <= kSumError * w || !(sm.z[lane] < INFINITY) ||
+                           (!PROBS && !(sm.z[lane] >= 0.5 && s.rate >= kLeastRate &&
+                                        s.rate <= kMostRate)));
         sm.uq[lane] = uq;
         sm.w[lane] = w;
       }
