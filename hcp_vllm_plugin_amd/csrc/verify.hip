@@ -412,7 +412,7 @@ __device__ __forceinline__ VerifyRow decide(const VerifyParams& p, int b, Decide
     bool ok = false, near = false;
     if (token) {
       if (s.greedy) {
-        ok = sm.at[lane] == d;
+        ok = sm.at[lane] == d && sm.top[lane] > -INFINITY;  // (a row without entries has 0 there)
       } else {
         const double w = weight<PROBS>(xd, sm.top[lane], s.rate), v = uq * sm.z[lane];
         ok = v < w;
