@@ -2025,8 +2025,8 @@ int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
     return fail(HCP_EUNSUPPORTED, "%s: rot %d (a multiple of 16 up to 256)", who, a->rot);
   if (!dtype16(a->dtype) && a->dtype != HCP_DTYPE_F32)
     return fail(HCP_EUNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
-  // (a frequency in 64 bits is off by 2^-56 turns at most, a position by 2^-28)
-  if (a->num_positions < 0 || a->num_positions > int64_t{1} << 28)
+  constexpr int64_t kFarthest = int64_t{1} << 28;
+  if (a->num_positions < 0 || a->num_positions > kFarthest)
     return fail(HCP_EINVAL, "%s: bad sizes", who);
   const bool scaled = a->scaling != HCP_ROPE_SCALING_NONE;
   if (a->scaling < 0 || a->scaling > HCP_ROPE_SCALING_DIVIDED)
@@ -2091,6 +2091,10 @@ int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
       }
       default: break;
     }
+    // (a frequency in 64 bits is off by 2^-53 of itself, and by 2^-64 turns: the angle of
+    // the last position by 2^-25 and 2^-33)
+    if (!(f * static_cast<double>(a->num_positions) <= static_cast<double>(kFarthest)))
+      return fail(HCP_EINVAL, "%s: frequency %d times the positions passes 2^28", who, i);
     const double turns = std::ldexp(std::fmod(f / kTurn, 1.0), 64);
     p.turns[i] = turns < 0x1p64 ? static_cast<uint64_t>(turns) : 0;
   }

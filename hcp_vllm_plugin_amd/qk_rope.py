@@ -243,7 +243,8 @@ def rope_table(
 ) -> torch.Tensor:
     """The table ``[max_positions, rot]`` that ``qk_norm_rope`` reads: row t holds ``rot / 2``
     cosines of ``t f_i``, then as many sines, ``f_i = base ** (-2 i / rot)``; angles in 64
-    bits, values to 2^-22, rounded to ``dtype`` (float32, fp16 or bf16).
+    bits, values to 2^-22, rounded to ``dtype`` (float32, fp16 or bf16).  Neither
+    ``max_positions`` nor its product with a frequency may pass 2^28.
 
     ``scaling`` is a model's ``rope_scaling``, by its "rope_type": "linear" ("factor"),
     "llama3" ("factor", "low_freq_factor", "high_freq_factor",

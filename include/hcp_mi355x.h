@@ -933,7 +933,8 @@ int hcp_verify_drafts(const hcp_verify_args* args, void* stream);
  *              beta_fast times in `original` positions to the one that turns beta_slow
  *              times, both rounded outwards
  *   4 divided  f_i / divisors[i] (HOST [rot / 2])
- * and a = attention_factor.  rot a multiple of 16 up to 256; rows 16-byte aligned.
+ * and a = attention_factor.  rot a multiple of 16 up to 256; rows 16-byte aligned; no
+ * frequency times num_positions past 2^28, nor these: 64 bits hold no more of an angle.
  */
 #define HCP_ROPE_SCALING_NONE 0
 #define HCP_ROPE_SCALING_LINEAR 1
