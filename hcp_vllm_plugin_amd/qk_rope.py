@@ -225,6 +225,9 @@ def _scaling_fields(scaling: Mapping, rot: int, base: float, positions: int):
         if given is None or len(given) != rot // 2:
             raise ValueError(f"longrope needs {name!r}, rot / 2 numbers")
         divisors = (ctypes.c_double * (rot // 2))(*given)
+        if not (positions > trained or "factor" in number or "attention_factor" in number):
+            raise ValueError("longrope needs 'factor' or 'attention_factor' for a table no longer "
+                             "than its context, which says nothing of the model's")
         ratio = number.get("factor", positions / trained)
         attention = math.sqrt(1 + math.log(ratio) / math.log(trained)) if ratio > 1 else 1.0
     attention = number.get("attention_factor", attention)
@@ -254,9 +257,10 @@ def rope_table(
     the long ones for tables longer than that), or "default".  "yarn" and "longrope"
     multiply cosines and sines by ``0.1 ln(factor) + 1`` (with "mscale" and "mscale_all_dim" by
     the ratio of ``0.1 mscale ln(factor) + 1`` of the two) and ``sqrt(1 + ln(factor) /
-    ln(context))``, or by "attention_factor" where that is given ("longrope" without a
-    "factor": ``max_positions`` over the context).  An entry that its type does not go by is
-    refused, not passed over.
+    ln(context))``, or by "attention_factor" where that is given.  "longrope" without a
+    "factor" takes ``max_positions`` for the model's own context, and is refused where that is
+    not above the trained one.  An entry that its type does not go by is refused, not passed
+    over.
 
     ``out`` is written where it is given ``[max_positions, rot]``, of its dtype."""
     if rot <= 0 or rot % 16 or rot > 256:

@@ -1,10 +1,12 @@
 """CPU: scalings that ``rope_table`` refuses, for what they would make of the frequencies."""
 
 import ctypes
+import math
 
 import pytest
 
 from hcp_vllm_plugin_amd import _lib
+from hcp_vllm_plugin_amd.qk_rope import _scaling_fields
 
 
 def args(positions, **kw):
@@ -34,3 +36,18 @@ def test_frequencies_past_what_64_bits_hold(positions, least):
         d[at] = least * f
         a = args(positions, scaling=4, divisors=ctypes.addressof(d))
         assert L.hcp_rope_table(ctypes.addressof(a), None) == _lib.HCP_EINVAL, at
+
+
+@pytest.mark.parametrize("positions", [1, 4095, 4096])
+def test_longrope_needs_the_models_factor(positions):
+    """A table no longer than the trained context says nothing of the model's own."""
+    s = {"rope_type": "longrope", "short_factor": [1.0] * 32, "long_factor": [2.0] * 32,
+         "original_max_position_embeddings": 4096}
+    for more in ({}, {"factor": None}, {"attention_factor": None}):
+        with pytest.raises(ValueError, match="factor"):
+            _scaling_fields({**s, **more}, 64, 1e4, positions)
+    for more, a in (({"factor": 32.0}, math.sqrt(1 + 5 / 12)), ({"factor": 1.0}, 1.0),
+                    ({"attention_factor": 1.25}, 1.25), ({"factor": 8.0, "attention_factor": 1.0}, 1.0)):
+        assert _scaling_fields({**s, **more}, 64, 1e4, positions)[8] == pytest.approx(a, rel=1e-15)
+    # a longer one is taken for the model's context
+    assert _scaling_fields(s, 64, 1e4, 16384)[8] == pytest.approx(math.sqrt(1 + 2 / 12), rel=1e-15)
