@@ -93,14 +93,14 @@ struct Keys16 {
 #pragma unroll
     for (int i = 0; i < OPT; ++i) off[i] = piece(i * KPI + lane / CPR);
   }
-  // Byte of a tile that this lane fetches in its row: a slot past the row's dv
-  // columns fetches the first instead (it meets zeros of Q, or columns of O that
-  // are not stored).
-  __device__ __forceinline__ int slot16(int row) const {
-    const int ch = (lane % CPR) ^ (row & M);
-    return ch < dv / 8 ? 16 * ch : 0;
+  // The 16-byte slot of a row that this lane fetches; past the row's dv columns it has to
+  // read as zeros, as Q does there (the first slot's infinities would be NaN next to those):
+  // a place past any descriptor's range.
+  static constexpr int kPast = 0x7fffff00;
+  __device__ __forceinline__ int slot(int row) const { return (lane % CPR) ^ (row & M); }
+  __device__ __forceinline__ int piece(int row) const {
+    return slot(row) < dv / 8 ? row * rowb + 16 * slot(row) : kPast;
   }
-  __device__ __forceinline__ int piece(int row) const { return row * rowb + slot16(row); }
 
   __device__ __forceinline__ uint32_t fetch_ids(int x0) const {
     const int x = x0 + (lane & 32) / 2;
@@ -139,8 +139,9 @@ struct Keys16 {
       x = x < all ? x : all - 1;  // past the sequence: its last key, which has no weight here
       uint32_t id = static_cast<uint32_t>(global_ptr(bt)[x >> bs_shift]);
       id = id < id_max ? id : id_max;
-      const int64_t o =
-          id * stride_block + static_cast<int64_t>(x & (bs - 1)) * rowb + slot16(row & 15);
+      const int c = slot(row & 15);
+      const int64_t o = id * stride_block + static_cast<int64_t>(x & (bs - 1)) * rowb +
+                        (c < dv / 8 ? 16 * c : 0);  // (clear_past)
       ka[j] = k + o;
       va[j] = v + o;
     }
@@ -155,6 +156,15 @@ struct Keys16 {
               reinterpret_cast<uintptr_t>(va[j])),
           reinterpret_cast<HCP_LDS_PTR(void)>(dst + CHB + j * 1024), 16, 0, kDraftStreamAux);
     }
+  }
+  // Zeros in K past the rows' dv columns, once what issue_small loaded has landed.
+  __device__ __forceinline__ void clear_past(HCP_LDS_PTR(char) dst) const {
+    if (dv == D) return;
+    asm volatile("" ::: "memory");  // (not ahead of the wait for them)
+#pragma unroll
+    for (int j = 0; j < 2 * OPT; ++j)
+      if (slot((j * KPI + lane / CPR) & 15) >= dv / 8)
+        *reinterpret_cast<HCP_LDS_PTR(u32x4)>(dst + j * 1024 + 16 * lane) = u32x4{0, 0, 0, 0};
   }
   // Q's 16-byte slot of k-step s
   __device__ __forceinline__ int q_slot(int s) const { return 4 * s + g4; }
@@ -315,6 +325,7 @@ struct Keys4 {
     return static_cast<uint32_t>(global_ptr(bt)[(x < all ? x : all - 1) >> bs_shift]);
   }
   __device__ __forceinline__ void issue_small(int, HCP_LDS_PTR(char)) const {}
+  __device__ __forceinline__ void clear_past(HCP_LDS_PTR(char)) const {}
   __device__ __forceinline__ void issue(int x0, uint32_t ids, HCP_LDS_PTR(char) dst) const {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -668,6 +679,7 @@ __device__ __forceinline__ void drafts_split_body(
   } else if (some) {
     for (; x <= last; x += ST) {
       wait_vmcnt<0>();
+      keys.clear_past(be);
       compute(x, be);
       keys.issue_small(upto(x + ST), be);
     }
