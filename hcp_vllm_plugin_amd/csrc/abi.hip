@@ -1870,8 +1870,9 @@ int hcp_decode_drafts(const hcp_decode_drafts_args* args, void* stream) {
   if (!drafts_sizes(a->num_seqs, args->max_tokens, a->num_heads, a->num_kv_heads, a->head_dim))
     return fail(HCP_EUNSUPPORTED, "%s: more than %d sequences, %d tokens of one, or %d heads", who,
                 HCP_DECODE_PAGED_MAX_SEQS, HCP_DRAFTS_MAX_TOKENS, 1 << 16);
-  if (args->q_rows > INT32_MAX ||
-      static_cast<int64_t>(a->num_seqs) * args->max_tokens * a->num_heads > INT32_MAX)
+  // (the merge: a wave to four heads of a row)
+  if (args->q_rows > INT32_MAX || static_cast<int64_t>(a->num_seqs) * args->max_tokens *
+                                          ((a->num_heads + 3) / 4) > kMostThreads / 64)
     return fail(HCP_EUNSUPPORTED, "%s: too many rows", who);
   if (!a->q || !a->out || !a->seq_lens || !args->row_starts || !a->kv.block_table)
     return fail(HCP_EINVAL, "%s: null pointer", who);
@@ -1981,8 +1982,9 @@ int hcp_verify_drafts(const hcp_verify_args* a, void* stream) {
       !a->num_out)
     return fail(HCP_EINVAL, "%s: null pointer", who);
   const VerifyPlan v = plan_verify(a->num_seqs, a->max_tokens, a->vocab);
-  if (static_cast<int64_t>(a->num_seqs) * a->max_tokens * v.stat_slices > INT32_MAX ||
-      static_cast<int64_t>(a->num_seqs) * v.sum_slices > INT32_MAX)
+  constexpr int64_t kMostSlices = kMostThreads / hcp::kVerThreads;
+  if (static_cast<int64_t>(a->num_seqs) * a->max_tokens * v.stat_slices > kMostSlices ||
+      static_cast<int64_t>(a->num_seqs) * v.sum_slices > kMostSlices)
     return fail(HCP_EUNSUPPORTED, "%s: too many rows", who);
   if (!a->workspace || a->workspace_bytes < v.bytes)
     return fail(HCP_EWORKSPACE, "%s: workspace %zu bytes < %zu needed", who,

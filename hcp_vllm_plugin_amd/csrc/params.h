@@ -179,6 +179,7 @@ struct RopeTableParams {
 
 // Verification of drafted tokens (verify.hip).
 constexpr int kVerMaxTokens = HCP_VERIFY_MAX_TOKENS;
+constexpr int kVerThreads = 256;  // of a workgroup
 constexpr int kVerStatSlice = 8192, kVerSumSlice = 2048;  // entries of a row to a workgroup
 struct VerifyStat {  // of a slice of a row
   float top;

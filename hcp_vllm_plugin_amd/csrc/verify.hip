@@ -34,7 +34,6 @@
 
 namespace hcp {
 
-constexpr int kVerThreads = 256;
 constexpr int kVerWaves = kVerThreads / 64;
 constexpr int kVerSmall = 65536;  // a vocabulary that one workgroup goes over
 constexpr int kStatSlice = kVerStatSlice;  // 32 values to a thread
