@@ -2033,8 +2033,10 @@ int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
   const bool scaled = a->scaling != HCP_ROPE_SCALING_NONE;
   if (a->scaling < 0 || a->scaling > HCP_ROPE_SCALING_DIVIDED)
     return fail(HCP_EUNSUPPORTED, "%s: scaling %d", who, a->scaling);
-  if (!(a->base > 1.0) || !std::isfinite(a->base) || !std::isfinite(a->attention_factor))
+  if (!(a->base > 1.0) || !std::isfinite(a->base))
     return fail(HCP_EINVAL, "%s: base must be finite and above 1", who);
+  if (!std::isfinite(static_cast<float>(a->attention_factor)))
+    return fail(HCP_EINVAL, "%s: attention_factor must be finite in 32 bits", who);
   if (scaled && a->scaling != HCP_ROPE_SCALING_DIVIDED &&
       (!(a->factor > 0.0) || !std::isfinite(a->factor)))
     return fail(HCP_EINVAL, "%s: factor must be finite and above 0", who);
@@ -2059,6 +2061,7 @@ int hcp_rope_table(const hcp_rope_table_args* a, void* stream) {
   p.num_positions = a->num_positions;
   p.rot = a->rot;
   p.factor = static_cast<float>(a->attention_factor);
+  p.factor_lo = static_cast<float>(a->attention_factor - p.factor);
   constexpr double kTurn = 6.283185307179586;
   // the dimension whose frequency turns beta times in `original` positions
   auto dim = [&](double beta) {

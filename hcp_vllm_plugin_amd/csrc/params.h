@@ -173,7 +173,7 @@ struct RopeTableParams {
   void* out;
   int64_t stride, num_positions;
   int32_t rot;
-  float factor;  // of the cosines and sines
+  float factor, factor_lo;  // of the cosines and sines: a float, and what is left of it
   uint64_t turns[kRopeMaxFrequencies];  // frequencies over 2 pi, the fraction times 2^64
 };
 

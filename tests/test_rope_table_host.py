@@ -51,3 +51,9 @@ def test_longrope_needs_the_models_factor(positions):
         assert _scaling_fields({**s, **more}, 64, 1e4, positions)[8] == pytest.approx(a, rel=1e-15)
     # a longer one is taken for the model's context
     assert _scaling_fields(s, 64, 1e4, 16384)[8] == pytest.approx(math.sqrt(1 + 2 / 12), rel=1e-15)
+
+
+def test_a_factor_past_32_bits():
+    for x in (1e39, -1e300, float("inf"), float("nan")):
+        a = args(100, attention_factor=x)
+        assert _lib.lib().hcp_rope_table(ctypes.addressof(a), None) == _lib.HCP_EINVAL, x
