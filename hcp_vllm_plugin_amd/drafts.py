@@ -152,9 +152,10 @@ def verify_drafts(
     second size says how many rows of a sequence are looked at, 1 to 64.
 
     ``temperature`` float32 ``[S]`` divides the logits (None: 1); where it is not above 0
-    the largest entry, the lowest index of equal ones, takes the place of the draw.
-    Tokens are as sums in 64 bits give them.  A NaN has no weight; a row without any gives
-    no token, and a draft that is no token of the vocabulary is refused."""
+    the largest entry above -inf, the lowest index of equal ones, takes the place of the
+    draw.  Tokens are as sums in 64 bits give them, at any temperature.  A NaN has no weight and
+    is no entry; a row without any accepts no draft and gives no token, and a draft that is
+    no token of the vocabulary is refused."""
     code, index = _REAL.get(target.dtype), target.get_device()
     if code is None or target.dim() != 2 or (target.shape[1] > 1 and target.stride(1) != 1):
         raise ValueError("target must be float16/bfloat16/float32 [T, V] with contiguous rows")

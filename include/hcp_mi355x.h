@@ -884,9 +884,9 @@ int hcp_decode_drafts(const hcp_decode_drafts_args* args, void* stream);
  * draft_probs[r][i] or 1.  One token more comes from max(w - q Z, 0) of the row that
  * refused (w without d where there is no q; w where nothing is left), or from the last
  * row's w: the first index at which the running sum passes uniform[r][max_tokens - 1]
- * times the whole.  With a temperature that is not above 0 the row's largest entry, the
- * lowest index of equal ones, is what a draft has to be, and the token.  All of it as in
- * 64 bits.
+ * times the whole.  With a temperature that is not above 0 the row's largest entry above
+ * -inf, the lowest index of equal ones, is what a draft has to be, and the token.  All of
+ * it as in 64 bits.
  *   target       DEVICE [num_rows, vocab] F16 / BF16 / F32, rows row_stride elements apart
  *   tokens       DEVICE [num_rows] I32 / I64; a draft that is no token is refused
  *   row_starts   DEVICE [num_seqs + 1] I32 / I64
